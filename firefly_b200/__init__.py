@@ -9,11 +9,29 @@ libfirefly_b200.so (hand-written sm_100a kernels) through a C ABI
 from .fireflykernels import quantize_fp_to_int8
 from .bitLinear import BitLinear, collect_bitlinear_modules
 from .fireflyoptim import FireFlyOptim, FireFlyOptimSR
+from .mxfp4 import (
+    MXFP4Linear,
+    MXFP4SwiGLU,
+    MXFP4Tensor,
+    mxfp4_linear,
+    mxfp4_matmul,
+    mxfp4_swiglu,
+    quantize_fp_to_mxfp4,
+    quantize_fp_to_mxfp4_dual,
+)
 
 __all__ = [
     "BitLinear",
     "FireFlyOptim",
     "FireFlyOptimSR",
+    "MXFP4Linear",
+    "MXFP4SwiGLU",
+    "MXFP4Tensor",
     "collect_bitlinear_modules",
+    "mxfp4_linear",
+    "mxfp4_matmul",
+    "mxfp4_swiglu",
     "quantize_fp_to_int8",
+    "quantize_fp_to_mxfp4",
+    "quantize_fp_to_mxfp4_dual",
 ]

@@ -75,6 +75,14 @@ SIGNATURES = {
                            _D, _D, _D, _D, _D, _D, _D, _D, _U64, _U64, _I64, _P, _P, _P, _P]),
     "ff_dqt_adamw8_peers": (_I, [_P, _P, _I64, _I64, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _I64, _I64,
                                  _D, _D, _D, _D, _D, _D, _D, _D, _U64, _U64, _I64, _P, _P, _P]),
+    "ff_mxfp4_scale_bytes": (_I64, [_I64, _I64]),
+    "ff_mxfp4_colsum_ws_elems": (_I64, [_I64, _I64]),
+    "ff_mxfp4_quant": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P, _P, _P]),
+    "ff_mxfp4_dequant": (_I, [_P, _I64, _P, _I64, _I64, _P, _I, _I64, _P]),
+    "ff_mxfp4_swiglu_quant": (_I, [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P]),
+    "ff_mxfp4_swiglu_bwd_quant": (_I, [_P, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P]),
+    "ff_mxfp4_gemm": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P]),
+    "ff_mxfp4_swiglu_gemm": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P]),
     "ff_ipc_alloc": (_I, [_I64, ctypes.POINTER(ctypes.c_void_p)]),
     "ff_ipc_free": (_I, [_P]),
     "ff_ipc_get_handle": (_I, [_P, ctypes.c_char_p]),
@@ -109,6 +117,8 @@ _KERNELS_PER_CALL = {"ff_quant_rows_i8": 1, "ff_quant_dual_i8": 2, "ff_quant_dua
                      "ff_transpose_i8": 1, "ff_gemm_i8": 1, "ff_gemm_i8_kn": 1, "ff_gemm_i8_ws": 1,
                      "ff_colsum_bf16": 2, "ff_quant_dual_i8_db": 3, "ff_dqt_adamw8": 1, "ff_dqt_adamw8_peers": 1, "ff_update_int8_weight": 1,
                      "ff_adamw8_blockwise": 1,
+                     "ff_mxfp4_quant": 1, "ff_mxfp4_dequant": 1, "ff_mxfp4_swiglu_quant": 1,
+                     "ff_mxfp4_swiglu_bwd_quant": 1, "ff_mxfp4_gemm": 1, "ff_mxfp4_swiglu_gemm": 1,
                      "ff_adamw32_multi": 1}
 
 
@@ -726,6 +736,106 @@ def gemm_i8(a: torch.Tensor, b: torch.Tensor, k: int, scale_a: torch.Tensor | No
             byts = M * int(k) + N * int(k) + M * N * out.element_size() * (2 if out_kind == FF_OUT_BF16_ACCUM else 1)
             GEMM_EVENTS.append((ev[0], ev[1], 2 * M * N * int(k), byts))
     return out
+
+
+# ---------------------------------------------------------------------------
+# MXFP4 (E2M1 codes, one E8M0 scale per 32 values along the contraction)
+# ---------------------------------------------------------------------------
+def _mx_alloc(rows: int, cols: int, dev: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Uninitialised codes ``[rows, 16·ceil(cols/32)]`` and scales of an MXFP4 matrix."""
+    codes = torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=dev)
+    nbytes = (rows + 127) // 128 * 2 * ((cols + 255) // 256) * 512  # ff_mxfp4_scale_bytes(rows, cols)
+    return codes, torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+
+
+def _mx_float(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"MXFP4 quantises float32, bfloat16 or float16 tensors, got {x.dtype}")
+    x, ld = _rows_view(x)
+    if x.shape[1] == 0:
+        raise ValueError("cannot quantise rows of length 0")
+    return x, ld
+
+
+def mxfp4_quant(x: torch.Tensor, rows: bool = True, cols: bool = False, colsum: bool = False):
+    """``(codes, scales)`` of ``x`` [R, C] with blocks along its rows, the same of the transposed
+    matrix [C, R] from the same read, and the fp32 column sums; parts not asked for are ``None``."""
+    dev = _require_cuda(x)
+    x, ldx = _mx_float(x)
+    R, C = x.shape
+    q = s = qt = st = sums = ws = None
+    if rows:
+        q, s = _mx_alloc(R, C, dev)
+    if cols or colsum:
+        qt, st = _mx_alloc(C, R, dev)
+    if colsum:
+        sums = torch.empty((C,), dtype=torch.float32, device=dev)
+        ws = torch.empty(((R + 127) // 128 * C,), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _call("ff_mxfp4_quant", _ptr(x), _dtype_code(x.dtype), R, C, ldx, _ptr(q), (C + 31) // 32 * 16, _ptr(s),
+              _ptr(qt), (R + 31) // 32 * 16, _ptr(st), _ptr(sums), _ptr(ws), _stream(dev))
+    return (None if q is None else (q, s)), (None if qt is None else (qt, st)), sums
+
+
+def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
+    dev = _require_cuda(codes, scales)
+    out = torch.empty((rows, cols), dtype=dtype, device=dev)
+    with torch.cuda.device(dev):
+        _call("ff_mxfp4_dequant", _ptr(codes), codes.stride(0) if rows > 1 else codes.shape[1], _ptr(scales), rows, cols,
+              _ptr(out), _dtype_code(dtype), cols, _stream(dev))
+    return out
+
+
+def mxfp4_gemm(a, b, M: int, N: int, K: int, bias: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``A·Bᵀ (+ bias)`` of two ``(codes, scales)`` pairs with blocks along K."""
+    dev = _require_cuda(a[0], a[1], b[0], b[1], bias)
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"MXFP4 product: output dtype {out_dtype} (bfloat16 or float32)")
+    out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    with torch.cuda.device(dev):
+        _call("ff_mxfp4_gemm", _ptr(a[0]), a[0].shape[1], _ptr(a[1]), _ptr(b[0]), b[0].shape[1], _ptr(b[1]), _ptr(bias),
+              _ptr(out), N, FF_OUT_F32 if out_dtype == torch.float32 else FF_OUT_BF16, M, N, K, _stream(dev))
+    return out
+
+
+def mxfp4_swiglu_gemm(a, b, M: int, F: int, K: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(codes, scales)`` of h = silu(g)·u, [g | u] = A·Bᵀ, B the 2F gate and up rows (F % 128 == 0)."""
+    dev = _require_cuda(a[0], a[1], b[0], b[1])
+    hq, hs = _mx_alloc(M, F, dev)
+    with torch.cuda.device(dev):
+        _call("ff_mxfp4_swiglu_gemm", _ptr(a[0]), a[0].shape[1], _ptr(a[1]), _ptr(b[0]), b[0].shape[1], _ptr(b[1]),
+              _ptr(hq), hq.shape[1], _ptr(hs), M, F, K, _stream(dev))
+    return hq, hs
+
+
+def mxfp4_swiglu_quant(gu: torch.Tensor, cols: bool = False):
+    """Codes of h = bf16(silu(g)·u) [T, F] of ``gu = [g | u]`` and, with ``cols``, of hᵀ."""
+    dev = _require_cuda(gu)
+    gu, ld, F = _swiglu_halves(gu)
+    T = gu.shape[0]
+    q, s = _mx_alloc(T, F, dev)
+    qt, st = _mx_alloc(F, T, dev) if cols else (None, None)
+    with torch.cuda.device(dev):
+        _call("ff_mxfp4_swiglu_quant", _ptr(gu), ld, T, F, _ptr(q), q.shape[1], _ptr(s), _ptr(qt), (T + 31) // 32 * 16,
+              _ptr(st), _stream(dev))
+    return (q, s), (qt, st) if cols else None
+
+
+def mxfp4_swiglu_bwd_quant(dh: torch.Tensor, gu: torch.Tensor, rows: bool = True, cols: bool = True):
+    """Codes of [dg | du] [T, 2F] from dh and ``gu``, and of its transpose."""
+    dev = _require_cuda(dh, gu)
+    gu, ld, F = _swiglu_halves(gu)
+    if dh.dtype != torch.bfloat16 or tuple(dh.shape) != (gu.shape[0], F):
+        raise ValueError(f"expected dh bf16 {(gu.shape[0], F)}, got {dh.dtype} {tuple(dh.shape)}")
+    dh, lddh = _rows_view(dh)
+    T = gu.shape[0]
+    q, s = _mx_alloc(T, 2 * F, dev) if rows else (None, None)
+    qt, st = _mx_alloc(2 * F, T, dev) if cols else (None, None)
+    with torch.cuda.device(dev):
+        _call("ff_mxfp4_swiglu_bwd_quant", _ptr(dh), lddh, _ptr(gu), ld, T, F, _ptr(q), (2 * F + 31) // 32 * 16, _ptr(s),
+              _ptr(qt), (T + 31) // 32 * 16, _ptr(st), _stream(dev))
+    return (q, s) if rows else None, (qt, st) if cols else None
 
 
 def colsum_bf16(x: torch.Tensor) -> torch.Tensor:

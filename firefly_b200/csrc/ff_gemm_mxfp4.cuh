@@ -1,0 +1,462 @@
+// ff_gemm_mxfp4.cuh — product of two MXFP4 operands on the 5th-generation tensor cores.
+//
+//   D[m, n] = sum_k A[m, k] * B[n, k] (+ bias[n])     A: M x K, B: N x K, values as ff_mxfp4.cuh holds them
+//
+// tcgen05.mma kind::mxf4 multiplies E2M1 codes, scales each run of 32 products by the two E8M0
+// scales and accumulates in fp32 in TMEM; nothing is dequantised on the way.  64 values of K per
+// instruction are 32 bytes, so a 128-byte swizzled row is 256 values of K, and the operand tiles
+// and descriptors are those of the int8 kernels (ff_gemm_i8.cuh).  The scales of a k-block travel in
+// the order that the tensor core wants (512-byte chunks of 128 rows x 4 blocks): TMA brings two
+// chunks per 128 rows, tcgen05.cp spreads them over TMEM (lane = row % 32, word = row / 32,
+// repeated for the four lane quarters), and the instruction descriptor says which two of a word's
+// four bytes the current 64 values use.
+//
+// Two kernels:
+//   mx_gemm_narrow_kernel  one CTA per 128 rows of B x up to 128 rows of A, operands swapped (B is the
+//                          MMA's M side), K split over a cluster: few rows of A, a stream over B
+//   mx_gemm_pair_kernel    a CTA pair per 256 x 256 tile (cta_group::2), persistent
+// Either can end in the SwiGLU epilogue of a gate/up projection, whose 32 features of a row are one
+// block of the format: h leaves as codes and scales and is never written in bf16.
+//
+// Waits are time-bounded as in ff_gemm_i8.cuh.
+#pragma once
+
+#include "ff_gemm_i8.cuh"
+#include "ff_mxfp4.cuh"
+
+namespace ff {
+namespace mxg {
+
+using namespace gemm;
+
+constexpr int KB = 256;          // values of K per stage: 128 bytes of codes, two scale chunks
+constexpr int SF_BYTES = 1024;   // scales of 128 rows x KB
+constexpr int ROWS_BYTES = 128 * 128;  // codes of 128 rows x KB
+
+struct Epi {
+  void* D;
+  int64_t ldd, M, N;
+  const float* bias;
+  int out_f32;
+  int vec;        // 16-byte stores of rows allowed
+  int tma_store;  // bf16 output through TMA (pair kernel)
+  // SwiGLU epilogue: codes and scales of h [M, F] and, when gu is given, the activations [g | u] in bf16
+  uint8_t* hq;
+  uint8_t* hs;
+  int64_t ldh, hchunks, F;
+};
+
+// Instruction descriptor, kind::mxf4: A and B E2M1 (1 at bits 7-9 and 10-11), K-major, E8M0 scales
+// (bit 23), N >> 3 at bits 17-22, M >> 7 at bits 27-28, dense K = 64 (bit 31 = 0).
+__host__ __device__ constexpr uint32_t idesc_mx(int m, int n) {
+  return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27);
+}
+// which bytes of the scale words this instruction uses: 0 or 2 (B at bits 4-5, A at bits 29-30)
+__host__ __device__ constexpr uint32_t idesc_sf(uint32_t id) { return (id << 4) | (id << 29); }
+
+// a 512-byte scale chunk: 32 rows of 16 bytes, no swizzle, groups of 8 rows 128 bytes apart
+__device__ __forceinline__ uint64_t sf_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+
+template <int CG>
+__device__ __forceinline__ void sf_copy(uint32_t taddr, uint32_t saddr) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sf_desc(saddr)) : "memory");
+  else
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sf_desc(saddr)) : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_mx(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                       uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ float bf16_round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
+
+// h of one feature from the fp32 sums of its gate and up projections: the activations are bf16
+__device__ __forceinline__ float swiglu_h(float g, float u) {
+  g = bf16_round(g);
+  u = bf16_round(u);
+  return bf16_round(g * mx::sigmoid_f32(g) * u);
+}
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// Few rows of A.  One work item is 128 rows of B (NW = 2: 128 gate rows and the same 128 up rows)
+// against MP rows of A; the CTAs of a cluster take equal runs of its k-blocks.  Their fp32 partial
+// sums meet in shared memory: each warp of the cluster adds its (row of A, 32 columns) pieces over
+// the CTAs in rank order, so the result does not depend on timing and no workspace is needed.
+// ---------------------------------------------------------------------------
+__host__ __device__ constexpr int nr_stage_bytes(int mp, int nw) { return nw * (ROWS_BYTES + SF_BYTES) + mp * 128 + SF_BYTES; }
+// two CTAs per SM where a stage is small, else one
+__host__ __device__ constexpr int nr_stages(int mp, int nw) {
+  return (nw == 1 && mp <= 32 ? 105 * 1024 : 208 * 1024) / nr_stage_bytes(mp, nw) > 8
+             ? 8
+             : (nw == 1 && mp <= 32 ? 105 * 1024 : 208 * 1024) / nr_stage_bytes(mp, nw);
+}
+__host__ __device__ constexpr int nr_smem(int mp, int nw) { return nr_stages(mp, nw) * nr_stage_bytes(mp, nw) + 1024 + 256; }
+__host__ __device__ constexpr int pow2_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512; }
+__host__ __device__ constexpr int nr_tmem(int mp, int nw) { return pow2_cols(nw * mp + nr_stages(mp, nw) * (nw + 1) * 8); }
+
+template <int MP, int NW>
+__global__ void __launch_bounds__(NUM_THREADS)
+    mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW,
+                          const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmSX, int num_kb,
+                          Epi ep) {
+  constexpr int ST = nr_stages(MP, NW), SB = nr_stage_bytes(MP, NW), TC = nr_tmem(MP, NW);
+  static_assert(ST >= 2 && ST * SB >= NW * MP * 128 * 4, "the partial sums reuse the stages");
+  static_assert(NW * MP + ST * (NW + 1) * 8 <= 512, "TMEM columns");
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
+  uint8_t* smem = smem_raw + pad;
+  const uint32_t sbase = raw + pad;
+  // stage: NW x 16 KB of B, MP x 128 B of A (1024-byte aligned for the swizzle), then the scales
+  auto sW = [&](int s, int w) { return sbase + s * SB + w * ROWS_BYTES; };
+  auto sX = [&](int s) { return sbase + s * SB + NW * ROWS_BYTES; };
+  auto sSW = [&](int s, int w) { return sX(s) + MP * 128 + w * SF_BYTES; };
+  auto sSX = [&](int s) { return sX(s) + MP * 128 + NW * SF_BYTES; };
+  uint8_t* ctrl = smem + ST * SB;
+  const uint32_t cbase = sbase + ST * SB;
+  auto full_bar = [&](int s) { return cbase + 8u * s; };
+  auto empty_bar = [&](int s) { return cbase + 8u * (ST + s); };
+  const uint32_t tfull = cbase + 8u * (2 * ST);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (2 * ST + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * ST + 1) + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)blockIdx.x, csize = (int)gridDim.x;  // the cluster spans grid x
+  const int kb0 = (int)((int64_t)num_kb * rank / csize), kb1 = (int)((int64_t)num_kb * (rank + 1) / csize);
+  const int tw = (int)blockIdx.y, tx = (int)blockIdx.z;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(tfull, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmSW);
+    tma_prefetch_desc(&tmX);
+    tma_prefetch_desc(&tmSX);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(TC)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool live = true;  // epilogue warps: the accumulator was complete
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t phase = 0, used = 0, last = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!wait_bar(empty_bar(s), phase ^ 1u, abort_flag)) break;
+        mbar_arrive_expect_tx(full_bar(s), SB);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+          tma_load_2d(sW(s, w), &tmW, kb * 128, (int)(w * ep.F) + tw * 128, full_bar(s));
+          tma_load_2d(sSW(s, w), &tmSW, kb * 256, (int)(w * (ep.F / 128)) + tw, full_bar(s));
+        }
+        tma_load_2d(sX(s), &tmX, kb * 128, tx * MP, full_bar(s));
+        tma_load_2d(sSX(s), &tmSX, kb * 256, tx, full_bar(s));
+        used |= 1u << s;
+        last = (last & ~(1u << s)) | (phase << s);
+        if (++s == ST) {
+          s = 0;
+          phase ^= 1u;
+        }
+      }
+      for (int k = 0; k < ST; ++k)
+        if (used & (1u << k)) drain_bar(full_bar(k), (last >> k) & 1u);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_mx(128, MP);
+      int s = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!wait_bar(full_bar(s), phase, abort_flag)) break;
+        tc_fence_after();
+        // this stage's scales: 8 columns per operand, slots as many as stages
+        const uint32_t sf = tmem + (uint32_t)(NW * MP + s * (NW + 1) * 8);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int w = 0; w < NW; ++w) sf_copy<1>(sf + w * 8 + c * 4, sSW(s, w) + c * 512);
+          sf_copy<1>(sf + NW * 8 + c * 4, sSX(s) + c * 512);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int w = 0; w < NW; ++w)
+            mma_mx<1>(tmem + w * MP, smem_desc_k_sw128(sW(s, w) + k * 32), smem_desc_k_sw128(sX(s) + k * 32),
+                      idesc | idesc_sf((k & 1) * 2), sf + w * 8 + (k >> 1) * 4, sf + NW * 8 + (k >> 1) * 4,
+                      (kb != kb0 || k != 0) ? 1u : 0u);
+        }
+        tc_commit(empty_bar(s));
+        if (++s == ST) {
+          s = 0;
+          phase ^= 1u;
+        }
+      }
+      tc_commit(tfull);
+      drain_bar(tfull, 0);
+    }
+    __syncwarp();
+  } else {
+    const int lg = warp & 3;
+    live = __all_sync(0xffffffffu, wait_bar(tfull, 0, abort_flag)) && !*abort_flag;
+    tc_fence_after();
+    if (live) {
+      const uint32_t tb = tmem + ((uint32_t)(lg * 32) << 16);
+      const int jn = (int)min64(MP, ep.M - (int64_t)tx * MP);
+      if (NW == 1 && csize == 1) {
+        const int64_t n = (int64_t)tw * 128 + lg * 32 + lane;
+        const float b = ep.bias && n < ep.N ? __ldg(ep.bias + n) : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < MP; c += 16) {
+          if (c >= jn) break;
+          uint32_t r[16];
+          tmem_ld16(tb + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (c + j < jn && n < ep.N) {
+              const int64_t at = ((int64_t)tx * MP + c + j) * ep.ldd + n;
+              const float v = __uint_as_float(r[j]) + b;
+              if (ep.out_f32) static_cast<float*>(ep.D)[at] = v;
+              else static_cast<__nv_bfloat16*>(ep.D)[at] = __float2bfloat16_rn(v);
+            }
+          }
+        }
+      } else {
+        // partial sums [w][row of A][128] over the stages' memory (every load has landed and been read)
+        float* part = reinterpret_cast<float*>(smem);
+#pragma unroll 1
+        for (int c = 0; c < NW * MP; c += 16) {
+          if (c % MP >= jn) continue;
+          uint32_t r[16];
+          tmem_ld16(tb + c, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(c + j) * 128 + lg * 32 + lane] = __uint_as_float(r[j]);
+        }
+      }
+    }
+  }
+
+  if (NW == 2 || csize > 1) {
+    cluster_sync_all();
+    if (warp >= 2 && live) {
+      const int jn = (int)min64(MP, ep.M - (int64_t)tx * MP);
+      const int total = jn * 4;
+#pragma unroll 1
+      for (int it = rank * 4 + (warp - 2); it < total; it += csize * 4) {
+        const int j = it >> 2, lq = it & 3;
+        const uint32_t at = sbase + (uint32_t)((j * 128 + lq * 32 + lane) * 4);
+        float v = 0.f, u = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < csize; ++r) {
+          const uint32_t a = mapa_shared(at, (uint32_t)r);
+          v += ld_cluster_f32(a);
+          if constexpr (NW == 2) u += ld_cluster_f32(a + MP * 128 * 4);
+        }
+        const int64_t m = (int64_t)tx * MP + j;
+        if constexpr (NW == 1) {
+          const int64_t n = (int64_t)tw * 128 + lq * 32 + lane;
+          if (n < ep.N) {
+            if (ep.bias) v += __ldg(ep.bias + n);
+            if (ep.out_f32) static_cast<float*>(ep.D)[m * ep.ldd + n] = v;
+            else static_cast<__nv_bfloat16*>(ep.D)[m * ep.ldd + n] = __float2bfloat16_rn(v);
+          }
+        } else {
+          // one block of h: 32 features, a lane each
+          const float h = swiglu_h(v, u);
+          const uint32_t S = mx::scale_code(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7FFFFFFFu));
+          const float t[8] = {h * mx::inv_scale(S), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          uint32_t w = S == mx::kScaleNan ? 0u : (mx::codes8(t) & 0xFu) << (4 * (lane & 7));
+          w |= __shfl_xor_sync(0xffffffffu, w, 1);
+          w |= __shfl_xor_sync(0xffffffffu, w, 2);
+          w |= __shfl_xor_sync(0xffffffffu, w, 4);
+          const int64_t blk = (int64_t)tw * 4 + lq;
+          if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(ep.hq + m * ep.ldh + blk * 16 + (lane >> 3) * 4) = w;
+          if (lane == 0) ep.hs[mx::scale_at(m, blk, ep.hchunks)] = (uint8_t)S;
+        }
+      }
+      if constexpr (NW == 2) {  // the padding chunk of h's scales
+        if (rank == 0 && tw == (int)gridDim.y - 1 && tx % (128 / MP) == 0 && ep.hchunks * 128 > ep.F)
+          reinterpret_cast<uint32_t*>(ep.hs)[((int64_t)(tx * MP / 128) * ep.hchunks + ep.F / 128) * 128 + (threadIdx.x - 64)] = 0;
+      }
+    }
+    cluster_sync_all();  // no CTA leaves while another reads its partial sums
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// scales as a matrix of 32-bit words, one row per 128 rows of the operand: boxes of 256 words
+inline int make_map_sf(CUtensorMap* m, const uint8_t* s, int64_t rows, int64_t cols) {
+  auto fn = encode_fn();
+  if (!fn) return set_error(FF_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  const int64_t words = mx::chunks_of(cols) * 128;
+  cuuint64_t dims[2] = {(cuuint64_t)words, (cuuint64_t)((rows + 127) / 128)};
+  cuuint64_t strides[1] = {(cuuint64_t)(words * 4)};
+  cuuint32_t box[2] = {256, 1}, estr[2] = {1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<uint8_t*>(s), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(FF_ERR_CUDA, "cuTensorMapEncodeTiled (scales) failed (%d)", (int)r);
+  return FF_OK;
+}
+// codes: [rows, K] two to a byte; boxes of 128 bytes x box_rows, zeros outside
+inline int make_map_codes(CUtensorMap* m, const uint8_t* q, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+  return make_map(m, reinterpret_cast<const int8_t*>(q), rows, (cols + 31) / 32 * 16, ld, box_rows);
+}
+
+struct Operand {
+  const uint8_t* q;
+  int64_t ld;
+  const uint8_t* s;
+};
+
+template <int MP, int NW>
+inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int csize, int64_t brows,
+                         cudaStream_t st) {
+  static bool done[64] = {false};
+  int rc = mx::allow_smem(mx_gemm_narrow_kernel<MP, NW>, nr_smem(MP, NW), done, "ff_mxfp4_gemm");
+  if (rc) return rc;
+  CUtensorMap tw, tsw, tx, tsx;
+  if ((rc = make_map_codes(&tw, b.q, brows, K, b.ld, 128))) return rc;
+  if ((rc = make_map_sf(&tsw, b.s, brows, K))) return rc;
+  if ((rc = make_map_codes(&tx, a.q, ep.M, K, a.ld, MP))) return rc;
+  if ((rc = make_map_sf(&tsx, a.s, ep.M, K))) return rc;
+  const int64_t tiles_w = ((NW == 2 ? ep.F : ep.N) + 127) / 128, tiles_x = (ep.M + MP - 1) / MP;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)csize, (unsigned)tiles_w, (unsigned)tiles_x);
+  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.dynamicSmemBytes = nr_smem(MP, NW);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)csize;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_narrow_kernel<MP, NW>, tw, tsw, tx, tsx, (int)((K + KB - 1) / KB), ep),
+              "ff_mxfp4_gemm launch");
+  return check_launch("ff_mxfp4_gemm");
+}
+
+template <int NW>
+inline int launch_narrow_mp(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, cudaStream_t st) {
+  const int64_t num_kb = (K + KB - 1) / KB;
+  const int mp = ep.M <= 16 ? 16 : ep.M <= 32 ? 32 : ep.M <= 64 ? 64 : 128;
+  const int64_t items = ((NW == 2 ? ep.F : ep.N) + 127) / 128 * ((ep.M + mp - 1) / mp);
+  const int nsm = num_sms_current();
+  // split K while the items leave SMs idle or unevenly filled, and every CTA keeps four k-blocks
+  int c = 1;
+  while (c < 8 && items * c < 4 * nsm && num_kb >= 4 * (2 * c)) c *= 2;
+  switch (mp) {
+    case 16: return launch_narrow<16, NW>(a, b, K, ep, c, brows, st);
+    case 32: return launch_narrow<32, NW>(a, b, K, ep, c, brows, st);
+    case 64: return launch_narrow<64, NW>(a, b, K, ep, c, brows, st);
+    default: return launch_narrow<128, NW>(a, b, K, ep, c, brows, st);
+  }
+}
+
+inline int check_operand(const char* name, const char* which, const Operand& o, int64_t K) {
+  FF_REQUIRE(o.q && o.s, FF_ERR_INVALID_ARG, "%s: null pointer (%s)", name, which);
+  FF_REQUIRE(o.ld % 16 == 0 && o.ld >= (K + 31) / 32 * 16 && aligned(o.q, 16) && aligned(o.s, 16), FF_ERR_INVALID_ARG,
+             "%s: %s needs 16-byte alignment and rows of a multiple of 16 bytes that hold every block (ld=%lld)", name, which,
+             (long long)o.ld);
+  return FF_OK;
+}
+
+}  // namespace mxg
+}  // namespace ff
+
+extern "C" int ff_mxfp4_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, const uint8_t* B, int64_t ldb,
+                             const uint8_t* sB, const float* bias, void* D, int64_t ldd, int out_kind, int64_t M, int64_t N,
+                             int64_t K, void* stream) {
+  using namespace ff::mxg;
+  FF_REQUIRE(M >= 0 && N >= 0 && K >= 1, FF_ERR_INVALID_ARG, "ff_mxfp4_gemm: M=%lld N=%lld K=%lld", (long long)M, (long long)N,
+             (long long)K);
+  FF_REQUIRE(out_kind == FF_OUT_F32 || out_kind == FF_OUT_BF16, FF_ERR_INVALID_ARG, "ff_mxfp4_gemm: bad out_kind %d", out_kind);
+  if (M == 0 || N == 0) return FF_OK;
+  FF_REQUIRE(D && ldd >= N, FF_ERR_INVALID_ARG, "ff_mxfp4_gemm: null output or ldd=%lld < N=%lld", (long long)ldd, (long long)N);
+  FF_REQUIRE(M <= 65535 * 128 && N < ((int64_t)1 << 22) && K < ((int64_t)1 << 30), FF_ERR_UNSUPPORTED,
+             "ff_mxfp4_gemm: dimension too large (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
+  const Operand a{A, lda, sA}, b{B, ldb, sB};
+  int rc;
+  if ((rc = check_operand("ff_mxfp4_gemm", "A", a, K)) || (rc = check_operand("ff_mxfp4_gemm", "B", b, K))) return rc;
+  Epi ep{};
+  ep.D = D;
+  ep.ldd = ldd;
+  ep.M = M;
+  ep.N = N;
+  ep.bias = bias;
+  ep.out_f32 = out_kind == FF_OUT_F32;
+  ep.vec = ff::aligned(D, 16) && (ldd * (ep.out_f32 ? 4 : 2)) % 16 == 0;
+  return launch_narrow_mp<1>(a, b, K, ep, N, ff::as_stream(stream));
+}
+
+extern "C" int ff_mxfp4_swiglu_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, const uint8_t* B, int64_t ldb,
+                                    const uint8_t* sB, uint8_t* hq, int64_t ldh, uint8_t* hs, int64_t M, int64_t F, int64_t K,
+                                    void* stream) {
+  using namespace ff::mxg;
+  FF_REQUIRE(M >= 0 && F >= 1 && K >= 1, FF_ERR_INVALID_ARG, "ff_mxfp4_swiglu_gemm: M=%lld F=%lld K=%lld", (long long)M,
+             (long long)F, (long long)K);
+  FF_REQUIRE(F % 128 == 0, FF_ERR_UNSUPPORTED, "ff_mxfp4_swiglu_gemm: F=%lld is not a multiple of 128", (long long)F);
+  if (M == 0) return FF_OK;
+  FF_REQUIRE(M <= 65535 * 128 && F < ((int64_t)1 << 21) && K < ((int64_t)1 << 30), FF_ERR_UNSUPPORTED,
+             "ff_mxfp4_swiglu_gemm: dimension too large (M=%lld F=%lld K=%lld)", (long long)M, (long long)F, (long long)K);
+  const Operand a{A, lda, sA}, b{B, ldb, sB}, h{hq, ldh, hs};
+  int rc;
+  if ((rc = check_operand("ff_mxfp4_swiglu_gemm", "A", a, K)) || (rc = check_operand("ff_mxfp4_swiglu_gemm", "B", b, K)) ||
+      (rc = check_operand("ff_mxfp4_swiglu_gemm", "h", h, F)))
+    return rc;
+  Epi ep{};
+  ep.M = M;
+  ep.N = 2 * F;
+  ep.F = F;
+  ep.hq = hq;
+  ep.hs = hs;
+  ep.ldh = ldh;
+  ep.hchunks = ff::mx::chunks_of(F);
+  return launch_narrow_mp<2>(a, b, K, ep, 2 * F, ff::as_stream(stream));
+}

@@ -9,6 +9,8 @@
 #include "ff_quant.cuh"
 #include "ff_norm.cuh"
 #include "ff_gemm_i8.cuh"
+#include "ff_mxfp4.cuh"
+#include "ff_gemm_mxfp4.cuh"
 
 #ifndef FF_VERSION_STRING
 #define FF_VERSION_STRING "firefly_b200 0.1.0 sm_100a"

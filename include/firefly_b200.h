@@ -516,6 +516,65 @@ FF_API int ff_ipc_close(void* ptr);
  */
 FF_API int ff_update_int8_weight(int8_t* w, const int32_t* dq, int64_t n, void* stream);
 
+/*
+ * Microscaled 4-bit floating point (MXFP4; the reference has no counterpart).  32 consecutive values
+ * along the contraction share one scale 2^(S - 127), S = max(floor(log2 max|x|) + 125, 0) held in one
+ * byte (E8M0); each value is an E2M1 code (0, .5, 1, 1.5, 2, 3, 4, 6 and the negatives), rounded to
+ * the nearest (ties to even) and saturated at 6; two codes to a byte, the earlier value in the low
+ * nibble.  A block with an infinity or a NaN gets S = 255 (NaN) and codes 0.
+ *
+ * Codes: [rows, ld BYTES], ld a multiple of 16 and at least 16 * ceil(cols / 32), 16-byte aligned.
+ * Scales: ff_mxfp4_scale_bytes(rows, cols) bytes, 16-byte aligned, in 512-byte chunks of 128 rows x
+ * 4 blocks: the scale of (row, block) is byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4 of
+ * chunk (row / 128) * chunks + block / 4, chunks = 2 * ceil(cols / 256).
+ */
+FF_API int64_t ff_mxfp4_scale_bytes(int64_t rows, int64_t cols);
+
+/*
+ * Quantise x [rows, cols] (dtype, leading dimension ldx in elements): row codes (blocks along the
+ * columns) into q_rows/s_rows and, in the same read, the codes of the transposed matrix [cols, rows]
+ * (blocks along the rows) into q_cols_t/s_cols.  Either pair may be NULL.  colsum (fp32 [cols], or
+ * NULL; with the column codes only) receives the column sums, added in a fixed order;
+ * colsum_ws then has ff_mxfp4_colsum_ws_elems(rows, cols) floats.
+ */
+FF_API int64_t ff_mxfp4_colsum_ws_elems(int64_t rows, int64_t cols);
+FF_API int ff_mxfp4_quant(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, uint8_t* q_rows,
+                          int64_t ldq, uint8_t* s_rows, uint8_t* q_cols_t, int64_t ldqt, uint8_t* s_cols,
+                          float* colsum, float* colsum_ws, void* stream);
+
+/* The values that codes and scales stand for, as dtype (leading dimension ldo in elements). */
+FF_API int ff_mxfp4_dequant(const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t rows, int64_t cols, void* out,
+                            int dtype, int64_t ldo, void* stream);
+
+/*
+ * The SwiGLU block's activation in the quantiser.  Forward: h = bf16(silu(g) * u) [rows, F] of the bf16
+ * gu = [g | u] (leading dimension ldgu), quantised as ff_mxfp4_quant does; h is not written.
+ * Backward: [dg | du] [rows, 2F], dg = bf16(dh u s (1 + g (1 - s))), du = bf16(dh g s), s = 1/(1+exp(-g)),
+ * quantised likewise.  F a multiple of 32; rows of gu and dh 16-byte aligned.
+ */
+FF_API int ff_mxfp4_swiglu_quant(const void* gu, int64_t ldgu, int64_t rows, int64_t F, uint8_t* q_rows, int64_t ldq,
+                                 uint8_t* s_rows, uint8_t* q_cols_t, int64_t ldqt, uint8_t* s_cols, void* stream);
+FF_API int ff_mxfp4_swiglu_bwd_quant(const void* dh, int64_t lddh, const void* gu, int64_t ldgu, int64_t rows,
+                                     int64_t F, uint8_t* q_rows, int64_t ldq, uint8_t* s_rows, uint8_t* q_cols_t,
+                                     int64_t ldqt, uint8_t* s_cols, void* stream);
+
+/*
+ * D[m, n] = sum_k A[m, k] B[n, k] (+ bias[n]) of two MXFP4 operands with blocks along K, fp32
+ * accumulation; out_kind FF_OUT_F32 or FF_OUT_BF16, ldd in elements, bias fp32 [N] or NULL.
+ */
+FF_API int ff_mxfp4_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, const uint8_t* B, int64_t ldb,
+                         const uint8_t* sB, const float* bias, void* D, int64_t ldd, int out_kind, int64_t M, int64_t N,
+                         int64_t K, void* stream);
+
+/*
+ * The gate/up product of a SwiGLU block with its activation: B [2F, K] holds the gate rows, then the up
+ * rows; g and u are the two products rounded to bf16, and h = bf16(silu(g) * u) [M, F] leaves quantised
+ * (codes hq, leading dimension ldh bytes; scales hs).  F a multiple of 128.
+ */
+FF_API int ff_mxfp4_swiglu_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, const uint8_t* B, int64_t ldb,
+                                const uint8_t* sB, uint8_t* hq, int64_t ldh, uint8_t* hs, int64_t M, int64_t F,
+                                int64_t K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
