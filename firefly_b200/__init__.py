@@ -8,6 +8,7 @@ libfirefly_b200.so (hand-written sm_100a kernels) through a C ABI
 """
 from .fireflykernels import quantize_fp_to_int8
 from .bitLinear import BitLinear, collect_bitlinear_modules
+from .distill import distillation_loss
 from .fireflyoptim import FireFlyOptim, FireFlyOptimSR
 from .mxfp4 import (
     MXFP4Linear,
@@ -28,6 +29,7 @@ __all__ = [
     "MXFP4SwiGLU",
     "MXFP4Tensor",
     "collect_bitlinear_modules",
+    "distillation_loss",
     "mxfp4_linear",
     "mxfp4_matmul",
     "mxfp4_swiglu",

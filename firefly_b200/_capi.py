@@ -83,6 +83,8 @@ SIGNATURES = {
     "ff_mxfp4_swiglu_bwd_quant": (_I, [_P, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P]),
     "ff_mxfp4_gemm": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P]),
     "ff_mxfp4_swiglu_gemm": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P]),
+    "ff_distill_loss": (_I, [_P, _I, _P, _P, _P, _I64, _P, _P, _P]),
+    "ff_distill_grad": (_I, [_P, _I, _P, _P, _I, _P, _P, _I64, _P]),
     "ff_ipc_alloc": (_I, [_I64, ctypes.POINTER(ctypes.c_void_p)]),
     "ff_ipc_free": (_I, [_P]),
     "ff_ipc_get_handle": (_I, [_P, ctypes.c_char_p]),
@@ -99,6 +101,19 @@ class Adamw32Tensor(ctypes.Structure):
     _fields_ = [("param", _P), ("grad", _P), ("exp_avg", _P), ("exp_avg_sq", _P), ("numel", ctypes.c_int64),
                 ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32), ("eps_term", _F),
                 ("step_scale", _F)]
+
+
+class DistillRows(ctypes.Structure):
+    """``FfDistillRows``: the rows of a distillation loss."""
+    _fields_ = [("logits", _P), ("ids", _P), ("teacher_logits", _P), ("labels", _P), ("teacher_lse", _P),
+                ("rows", _I64), ("vocab", _I64), ("top", _I64), ("ld_logits", _I64), ("ld_ids", _I64),
+                ("ld_teacher", _I64), ("ignore_index", _I64), ("dtype", ctypes.c_int32),
+                ("teacher_dtype", ctypes.c_int32), ("ids_64", ctypes.c_int32), ("labels_64", ctypes.c_int32),
+                ("temperature", _F), ("alpha", _F)]
+
+
+FF_REDUCE = {"none": 0, "mean": 1, "sum": 2}
+FF_DISTILL_WS_ELEMS = 128
 
 _lib = None
 
@@ -119,6 +134,7 @@ _KERNELS_PER_CALL = {"ff_quant_rows_i8": 1, "ff_quant_dual_i8": 2, "ff_quant_dua
                      "ff_adamw8_blockwise": 1,
                      "ff_mxfp4_quant": 1, "ff_mxfp4_dequant": 1, "ff_mxfp4_swiglu_quant": 1,
                      "ff_mxfp4_swiglu_bwd_quant": 1, "ff_mxfp4_gemm": 1, "ff_mxfp4_swiglu_gemm": 1,
+                     "ff_distill_loss": 3, "ff_distill_grad": 1,
                      "ff_adamw32_multi": 1}
 
 
@@ -836,6 +852,53 @@ def mxfp4_swiglu_bwd_quant(dh: torch.Tensor, gu: torch.Tensor, rows: bool = True
         _call("ff_mxfp4_swiglu_bwd_quant", _ptr(dh), lddh, _ptr(gu), ld, T, F, _ptr(q), (2 * F + 31) // 32 * 16, _ptr(s),
               _ptr(qt), (T + 31) // 32 * 16, _ptr(st), _stream(dev))
     return (q, s) if rows else None, (qt, st) if cols else None
+
+
+# ---------------------------------------------------------------------------
+# distillation loss
+# ---------------------------------------------------------------------------
+def distill_rows(logits, ids, teacher_logits, labels, teacher_lse, temperature, alpha, ignore_index) -> DistillRows:
+    """The C struct of 2-D operands with unit column stride (the caller keeps them alive)."""
+    return DistillRows(
+        logits.data_ptr(), ids.data_ptr(), teacher_logits.data_ptr(), 0 if labels is None else labels.data_ptr(),
+        0 if teacher_lse is None else teacher_lse.data_ptr(), logits.shape[0], logits.shape[1], ids.shape[1],
+        max(logits.stride(0), logits.shape[1]), max(ids.stride(0), ids.shape[1]),
+        max(teacher_logits.stride(0), teacher_logits.shape[1]), ignore_index, _dtype_code(logits.dtype),
+        _dtype_code(teacher_logits.dtype), int(ids.dtype == torch.int64),
+        int(labels is not None and labels.dtype == torch.int64), temperature, alpha)
+
+
+def distill_loss(rows: DistillRows, logits: torch.Tensor, reduction: str, grad: bool):
+    """``(row losses, scalar loss, gradient, held, counts)`` of ``ff_distill_loss``; parts that the
+    reduction does not have are ``None``."""
+    dev, n = logits.device, logits.shape[0]
+    row = torch.empty((n,), dtype=torch.float32, device=dev)
+    loss = counts = g = held = None
+    if reduction != "none":
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        if reduction == "mean":
+            counts = torch.empty((FF_DISTILL_WS_ELEMS,), dtype=torch.int32, device=dev)
+        if grad:
+            g = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev)
+            held = torch.empty((1,), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _call("ff_distill_loss", ctypes.byref(rows), FF_REDUCE[reduction], _ptr(row), _ptr(loss), _ptr(g),
+              logits.shape[1], _ptr(held), _ptr(counts), _stream(dev))
+    return row, loss, g, held, counts
+
+
+def distill_grad(rows: DistillRows, logits: torch.Tensor, reduction: str, upstream: torch.Tensor,
+                 counts: torch.Tensor | None, grad: torch.Tensor | None = None, held: torch.Tensor | None = None,
+                 keep_held: bool = False) -> torch.Tensor:
+    """The gradient for ``upstream`` (fp32 scalar, or one per row), into ``grad`` when it holds the
+    gradient for ``held`` already."""
+    dev = logits.device
+    if grad is None:
+        grad, held = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev), None
+    with torch.cuda.device(dev):
+        _call("ff_distill_grad", ctypes.byref(rows), FF_REDUCE[reduction], _ptr(upstream), _ptr(held), int(keep_held),
+              _ptr(counts), _ptr(grad), logits.shape[1], _stream(dev))
+    return grad
 
 
 def colsum_bf16(x: torch.Tensor) -> torch.Tensor:

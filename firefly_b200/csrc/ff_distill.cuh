@@ -1,0 +1,682 @@
+// ff_distill.cuh — distillation loss from a teacher's top logits, and its gradient.
+//
+// Row r has student logits s_v (v < V), entries j < K of the teacher (token i_j, logit t_j; an entry
+// with i_j < 0 or t_j = -inf is absent) and possibly a label y.  With temperature T:
+//   p_j = exp(t_j/T) / sum over the row's entries,     or, given the teacher's own log-sum-exp,
+//   p_j = exp(t_j/T - lse) with p_rest = 1 - sum p for the tokens outside the entries;
+//   q_v = softmax(s/T)_v,  q_rest = sum of q_v over the tokens outside the entries
+//   KD  = T^2 [ sum_j p_j (log p_j - log q_{i_j}) + p_rest (log p_rest - log q_rest) ]
+//   L   = alpha KD + (1 - alpha) (logsumexp(s) - s_y)
+//   dL/ds_v = alpha T (q_v - sum_{j: i_j = v} p_j)   on the entries' tokens,
+//             alpha T q_v (1 - p_rest / q_rest)       elsewhere (without lse: alpha T q_v),
+//             + (1 - alpha) (softmax(s)_v - [v = y]).
+// A row whose label is ignore_index, or without labels a row without entries, counts nothing.
+//
+// One cluster of 1 to 8 CTAs per row, each holding its slice of the row in shared memory (bulk
+// copies), so the logits are read once and the gradient is written once: the bound is HBM.  On a
+// slice: the maximum; the entries' logits are gathered and their places overwritten by -inf (which
+// makes the sum of the rest exact instead of 1 - sum q, and leaves each token's first entry as its
+// owner, so a token that occurs twice is summed once); the sum of exp; one exchange of partial
+// results between the CTAs; the gradient of all tokens, then the entries' own.
+// Maxima, sums and probabilities are fp32; the gradient is rounded once.
+#pragma once
+
+#include "ff_gemm_i8.cuh"
+#include "ff_mxfp4.cuh"
+
+namespace ff {
+namespace distill {
+
+constexpr int THREADS = 256;
+constexpr int WARPS = THREADS / 32;
+constexpr int MAX_TOP = 4096;
+constexpr int MAX_SMEM = 227 * 1024;
+constexpr int COUNT_CTAS = FF_DISTILL_WS_ELEMS;
+
+struct Args {
+  const void* logits;
+  int64_t rows, V, ldl;
+  const void* ids;
+  const void* tlogits;
+  const void* labels;
+  const float* lse;
+  int64_t ldi, ldt;
+  int64_t ignore;
+  int K, ids64, tdtype, labels64;
+  float T, alpha;
+  int mean;               // divide by the number of counted rows (`counts`)
+  const int32_t* counts;  // COUNT_CTAS partial counts
+  float* row_loss;        // [rows], or null
+  void* grad;             // [rows, ldg], or null
+  int64_t ldg;
+  const float* upstream;  // null: 1; else a scalar, or one value per row
+  int up_stride;
+  const float* held;      // the scalar upstream whose gradient `grad` holds already, or null
+  int slice;              // elements of a CTA's slice (a multiple of 128)
+};
+
+__device__ __forceinline__ int64_t load_index(const void* p, int64_t i, int is64) {
+  return is64 ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
+}
+__device__ __forceinline__ float load_float(const void* p, int64_t i, int dt) {
+  if (dt == FF_DTYPE_F32) return __ldg(static_cast<const float*>(p) + i);
+  if (dt == FF_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ float neg_inf() { return __uint_as_float(0xFF800000u); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+template <int DT>
+struct Vec {  // 16 bytes of logits
+  static constexpr int N = DT == FF_DTYPE_F32 ? 4 : 8;
+  static __device__ __forceinline__ void get(uint4 w, float (&v)[N]) {
+    if constexpr (DT == FF_DTYPE_F32) {
+      v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
+    } else if constexpr (DT == FF_DTYPE_BF16) {
+      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        v[2 * k] = __uint_as_float(q[k] << 16);
+        v[2 * k + 1] = __uint_as_float(q[k] & 0xFFFF0000u);
+      }
+    } else {
+      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[k]));
+        v[2 * k] = f.x;
+        v[2 * k + 1] = f.y;
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 put(const float (&v)[N]) {
+    if constexpr (DT == FF_DTYPE_F32) {
+      return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    } else {
+      uint32_t q[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (DT == FF_DTYPE_BF16) {
+          q[k] = pack_bf16x2(mk2(v[2 * k], v[2 * k + 1]));
+        } else {
+          const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
+          q[k] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      return make_uint4(q[0], q[1], q[2], q[3]);
+    }
+  }
+};
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::T from_f32(float v) {
+  if constexpr (DT == FF_DTYPE_F32) return v;
+  else if constexpr (DT == FF_DTYPE_BF16) return __float2bfloat16_rn(v);
+  else return __float2half_rn(v);
+}
+
+// what a CTA tells the others about its slice
+struct Part {
+  float m;        // largest logit
+  float sum;      // sum of exp((s - m)/T)
+  float sum1;     // sum of exp(s - m)
+  float rest;     // sum over the tokens outside the entries of exp((s - m)/T)
+  float dot;      // sum over its entries of p (log p - (s - m)/T)
+  float psum;     // sum of p over its entries
+  float label;    // the label's logit where the label lies in the slice, else -inf
+  float pad;
+};
+
+// shared memory: control, then K entries of 12 bytes, then the slice
+struct Ctrl {
+  uint64_t bar;
+  float red[6][WARPS];
+  Part parts[2][8];
+  float t_stats[2];   // of the teacher's entries: the sum of p, whether there is any
+  float label_logit;
+  int dup;
+  int label_in_top;
+};
+__host__ __device__ constexpr int ctrl_bytes() { return (int)((sizeof(Ctrl) + 127) / 128 * 128); }
+__host__ __device__ inline int entry_bytes(int K) { return (K * 12 + 127) / 128 * 128; }
+
+template <int DT>
+__global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
+  using T = typename Elem<DT>::T;
+  constexpr int N = Vec<DT>::N, ES = (int)sizeof(T);
+  extern __shared__ __align__(128) uint8_t smem[];
+  Ctrl& c = *reinterpret_cast<Ctrl*>(smem);
+  int* e_pos = reinterpret_cast<int*>(smem + ctrl_bytes());  // place in this slice, or -1
+  float* e_p = reinterpret_cast<float*>(e_pos + a.K);         // p_j
+  float* e_s = e_p + a.K;                                     // the student's logit (entries of this slice)
+  uint8_t* data = smem + ctrl_bytes() + entry_bytes(a.K);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int csize = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster spans grid x
+  const uint32_t bar = gemm::smem_u32(&c.bar);
+
+  if (a.held && __ldg(a.upstream) == __ldg(a.held)) return;  // every CTA of the grid alike
+
+  if (tid == 0) {
+    gemm::mbar_init(bar, 1);
+    c.label_in_top = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  float inv_count = 1.f;
+  if (a.mean) {
+    int n = 0;
+    for (int i = lane; i < COUNT_CTAS; i += 32) n += __ldg(a.counts + i);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    inv_count = 1.f / (float)max(n, 1);
+  }
+  __syncthreads();
+  if (csize > 1) gemm::cluster_sync_all();  // every CTA of the cluster runs before its memory is written to
+
+  const float inv_t = 1.f / a.T, kT = 1.4426950408889634f * inv_t, k1 = 1.4426950408889634f;
+  const bool two = a.labels != nullptr && a.T != 1.f && a.alpha != 1.f;  // a second softmax at T = 1
+  const int64_t v0 = (int64_t)rank * a.slice;
+  const int len = (int)max64(0, min64(a.slice, a.V - v0));
+  uint32_t phase = 0, par = 0;
+
+  for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+    // ---- does the row count?  (the same answer in every thread of the cluster)
+    int64_t label = -1;
+    bool live = true, bad = false;
+    if (a.labels) {
+      const int64_t y = load_index(a.labels, r, a.labels64);
+      live = y >= 0 && y < a.V && y != a.ignore;
+      bad = !live && y != a.ignore;
+      label = live ? y : -1;
+    }
+    T* grow = a.grad ? static_cast<T*>(a.grad) + r * a.ldg + v0 : nullptr;
+    const T* lrow = static_cast<const T*>(a.logits) + r * a.ldl + v0;
+    const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(lrow) & 15u);  // bytes into a 16-byte word
+    const int bytes = len * ES;
+    const int head = min(bytes, (int)((16u - mis) & 15u)), body = (bytes - head) & ~15;
+    T* s = reinterpret_cast<T*>(data + mis);  // the slice: element i is token v0 + i
+    const int words = (int)(mis + bytes + 15) / 16;
+
+    if (live) {
+      // ---- the slice: whole 16-byte words by bulk copies, the ragged ends by plain loads, and -inf
+      // around them up to whole words
+      if (tid == 0) {
+        gemm::mbar_arrive_expect_tx(bar, (uint32_t)body);
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(lrow) + head;
+        const uint32_t dst = gemm::smem_u32(data) + mis + head;
+        for (int o = 0; o < body; o += 16384) {
+          const uint32_t n = (uint32_t)min(16384, body - o);
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                           dst + o),
+                       "l"(src + o), "r"(n), "r"(bar)
+                       : "memory");
+        }
+      }
+      if (warp == 1) {
+        const int nh = head / ES, nt = (bytes - head - body) / ES;
+        if (lane < nh) s[lane] = lrow[lane];
+        if (lane < nt) s[(head + body) / ES + lane] = lrow[(head + body) / ES + lane];
+        if (lane < (int)mis / ES) reinterpret_cast<T*>(data)[lane] = from_f32<DT>(neg_inf());
+        const int past = words * 16 / ES - ((int)mis + bytes) / ES;
+        if (lane < past) s[len + lane] = from_f32<DT>(neg_inf());
+      }
+      // ---- the teacher's entries, by warp 0 while the copies run
+      if (warp == 0) {
+        float tm = neg_inf();
+        for (int j = lane; j < a.K; j += 32) {
+          const int64_t id = load_index(a.ids, r * a.ldi + j, a.ids64);
+          const float t = load_float(a.tlogits, r * a.ldt + j, a.tdtype);
+          const bool on = id >= 0 && id < a.V && t != neg_inf();
+          bad |= id >= a.V;
+          if (on) tm = t > tm || t != t ? t : tm;
+          e_p[j] = on ? t : neg_inf();
+          // absent: -1; in another CTA's slice: -2
+          e_pos[j] = !on ? -1 : (id >= v0 && id < v0 + len) ? (int)(id - v0) : -2;
+          if (on && id == label) c.label_in_top = (int)(r + 1);
+        }
+        tm = warp_max(tm);
+        const bool any = __any_sync(0xffffffffu, tm != neg_inf());
+        float shift = 0.f, zsum = 0.f;
+        __syncwarp();
+        if (a.lse) {
+          shift = __ldg(a.lse + r);
+        } else {
+          for (int j = lane; j < a.K; j += 32)
+            if (e_pos[j] != -1) zsum += expf((e_p[j] - tm) * inv_t);
+          zsum = warp_sum(zsum);
+        }
+        const float lz = a.lse ? 0.f : logf(zsum);
+        float ps = 0.f;
+        for (int j = lane; j < a.K; j += 32) {
+          if (e_pos[j] == -1) {
+            e_p[j] = neg_inf();
+          } else {  // log p_j
+            e_p[j] = a.lse ? e_p[j] * inv_t - shift : (e_p[j] - tm) * inv_t - lz;
+            ps += expf(e_p[j]);
+          }
+        }
+        ps = warp_sum(ps);
+        if (lane == 0) {
+          c.t_stats[0] = ps;
+          c.t_stats[1] = any ? 1.f : 0.f;
+          c.label_logit = neg_inf();
+          c.dup = 0;
+        }
+      }
+      if (bad) raise_status(FF_DEVICE_BADARG);
+      // wait for the copies: past the limit the error is recorded, and the copies in flight are
+      // waited for once more (bounded) so that none lands after the CTA
+      if (!gemm::mbar_try_wait(bar, phase)) {
+        const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns();
+        while (!gemm::mbar_try_wait(bar, phase)) {
+          if (globaltimer_ns() - t0 > limit) {
+            raise_status(FF_DEVICE_TIMEOUT);
+            gemm::drain_bar(bar, phase);
+            break;
+          }
+        }
+      }
+      phase ^= 1u;
+      __syncthreads();
+
+      // ---- largest logit; the entries' logits
+      const uint4* w = reinterpret_cast<const uint4*>(data);
+      float m = neg_inf();
+      for (int k = tid; k < words; k += THREADS) {
+        float v[N];
+        Vec<DT>::get(w[k], v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, v[e]);
+      }
+      for (int j = tid; j < a.K; j += THREADS)
+        if (e_pos[j] >= 0) e_s[j] = Elem<DT>::to_f32(s[e_pos[j]]);
+      if (tid == 0 && label >= v0 && label < v0 + len) c.label_logit = Elem<DT>::to_f32(s[label - v0]);
+      m = warp_max(m);
+      if (lane == 0) c.red[0][warp] = m;
+      __syncthreads();
+      m = c.red[0][0];
+#pragma unroll
+      for (int k = 1; k < WARPS; ++k) m = fmaxf(m, c.red[0][k]);
+      // ---- every token's place takes the index of one of its entries, which owns it
+      for (int j = tid; j < a.K; j += THREADS)
+        if (e_pos[j] >= 0) {
+          if constexpr (ES == 2) reinterpret_cast<uint16_t*>(s)[e_pos[j]] = (uint16_t)j;
+          else reinterpret_cast<uint32_t*>(s)[e_pos[j]] = (uint32_t)j;
+        }
+      __syncthreads();
+      const float ms = m == neg_inf() ? 0.f : m;  // a slice of -inf sums to 0
+      float sum = 0.f, sum1 = 0.f, rest = 0.f, dot = 0.f, psum = 0.f;
+      for (int j = tid; j < a.K; j += THREADS) {
+        const int pos = e_pos[j];
+        if (pos < 0) continue;
+        uint32_t owner;
+        if constexpr (ES == 2) owner = reinterpret_cast<volatile uint16_t*>(s)[pos];
+        else owner = reinterpret_cast<volatile uint32_t*>(s)[pos];
+        const float d = e_s[j] - ms, p = expf(e_p[j]);
+        if (p > 0.f) dot += p * (e_p[j] - d * inv_t);
+        else if (p != p) dot = p;
+        psum += p;
+        if (owner == (uint32_t)j) {
+          sum += ex2(d * kT);
+          if (two) sum1 += ex2(d * k1);
+          s[pos] = from_f32<DT>(neg_inf());  // never the index of an entry: MAX_TOP is below its bits
+        } else {
+          c.dup = 1;
+          e_pos[j] = -3 - pos;  // in this slice, but not its owner
+        }
+      }
+      __syncthreads();
+      // ---- sums of exp over the tokens outside the entries
+      for (int k = tid; k < words; k += THREADS) {
+        float v[N];
+        Vec<DT>::get(w[k], v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          const float d = v[e] - ms;
+          rest += ex2(d * kT);
+          if (two) sum1 += ex2(d * k1);
+        }
+      }
+      sum += rest;
+      float vals[5] = {sum, sum1, rest, dot, psum};
+#pragma unroll
+      for (int k = 0; k < 5; ++k) vals[k] = warp_sum(vals[k]);
+      if (lane == 0) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) c.red[k + 1][warp] = vals[k];
+      }
+      __syncthreads();
+      Part mine;
+      {
+        float t[5];
+#pragma unroll
+        for (int k = 0; k < 5; ++k) {
+          t[k] = c.red[k + 1][0];
+#pragma unroll
+          for (int x = 1; x < WARPS; ++x) t[k] += c.red[k + 1][x];
+        }
+        mine = Part{m, t[0], t[1], t[2], t[3], t[4], c.label_logit, 0.f};
+      }
+      Part all = mine;
+      if (csize > 1) {
+        if (tid < csize * 8) {  // word tid % 8 of this CTA's part to CTA tid / 8
+          const uint32_t dst = gemm::mapa_shared(gemm::smem_u32(&c.parts[par][rank]) + (tid & 7) * 4, (uint32_t)(tid >> 3));
+          const float word = (tid & 7) == 0 ? mine.m : (tid & 7) == 1 ? mine.sum : (tid & 7) == 2 ? mine.sum1
+                             : (tid & 7) == 3 ? mine.rest : (tid & 7) == 4 ? mine.dot : (tid & 7) == 5 ? mine.psum
+                             : (tid & 7) == 6 ? mine.label : 0.f;
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(word) : "memory");
+        }
+        gemm::cluster_sync_all();
+        all = c.parts[par][0];
+        for (int k = 1; k < csize; ++k) all.m = fmaxf(all.m, c.parts[par][k].m);
+        const float Ms = all.m == neg_inf() ? 0.f : all.m;
+        all.sum = all.sum1 = all.rest = all.dot = all.psum = 0.f;
+        all.label = neg_inf();
+        for (int k = 0; k < csize; ++k) {
+          const Part q = c.parts[par][k];
+          const float d = (q.m == neg_inf() ? 0.f : q.m) - Ms;
+          const float f = q.m == neg_inf() ? 1.f : ex2(d * kT), f1 = q.m == neg_inf() ? 1.f : ex2(d * k1);
+          all.sum += q.sum * f;
+          all.sum1 += q.sum1 * f1;
+          all.rest += q.rest * f;
+          all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot - q.psum * d * inv_t : 0.f;
+          all.psum += q.psum;
+          all.label = fmaxf(all.label, q.label);
+        }
+        par ^= 1u;
+      }
+      const float Ms = all.m == neg_inf() ? 0.f : all.m;
+      const float sum1_all = two ? all.sum1 : all.sum;
+      const bool has = c.t_stats[1] != 0.f;
+      if (!a.labels) live = has;
+      const float q_rest = all.rest / all.sum;
+      float p_rest = a.lse && has ? fmaxf(1.f - c.t_stats[0], 0.f) : 0.f;
+      if (q_rest == 0.f && p_rest < 1e-5f) p_rest = 0.f;  // nothing outside the entries: 1 - sum p is rounding
+      // ---- the loss
+      if (a.row_loss && rank == 0 && tid == 0) {
+        float kd = 0.f, ce = 0.f;
+        if (has) {
+          kd = all.dot + all.psum * logf(all.sum);
+          if (p_rest > 0.f) kd += p_rest * (logf(p_rest) - logf(q_rest));
+          kd *= a.T * a.T;
+        }
+        if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - (all.label - Ms);
+        a.row_loss[r] = live ? (a.alpha != 0.f ? a.alpha * kd : 0.f) + (a.alpha != 1.f ? (1.f - a.alpha) * ce : 0.f) : 0.f;
+      }
+      // ---- the gradient
+      if (grow && live) {
+        const float up = a.upstream ? __ldg(a.upstream + r * a.up_stride) * inv_count : inv_count;
+        const float fk = has ? up * a.alpha * a.T : 0.f, f1 = label >= 0 ? up * (1.f - a.alpha) : 0.f;
+        const float gq = fk / all.sum, g1 = f1 / sum1_all;       // factors of exp(..) for q and softmax at 1
+        const float gr = p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;  // q outside the entries
+        const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == mis;
+        for (int k = tid; k < words; k += THREADS) {
+          float v[N], g[N];
+          Vec<DT>::get(w[k], v);
+#pragma unroll
+          for (int e = 0; e < N; ++e) {
+            const float d = v[e] - Ms, x = ex2(d * kT);
+            g[e] = two ? gr * x + g1 * ex2(d * k1) : (gr + g1) * x;
+          }
+          const int i0 = k * N - (int)mis / ES;  // element of the slice
+          if (vec && i0 >= 0 && i0 + N <= len) {
+            __stcs(reinterpret_cast<uint4*>(grow + i0), Vec<DT>::put(g));
+          } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+              if (i0 + e >= 0 && i0 + e < len) grow[i0 + e] = from_f32<DT>(g[e]);
+          }
+        }
+        __syncthreads();  // the entries' and the label's own values come after the tokens'
+        for (int j = tid; j < a.K; j += THREADS) {
+          const int pos = e_pos[j];
+          if (pos < 0) continue;
+          float p = expf(e_p[j]);
+          if (c.dup) {  // the token's entries in order
+            p = 0.f;
+            for (int x = 0; x < a.K; ++x)
+              if (e_pos[x] == pos || e_pos[x] == -3 - pos) p += expf(e_p[x]);
+          }
+          const float d = e_s[j] - Ms;
+          float g = gq * ex2(d * kT) - fk * p;
+          if (f1 != 0.f) g += g1 * ex2(d * (two ? k1 : kT)) - (v0 + pos == label ? f1 : 0.f);
+          grow[pos] = from_f32<DT>(g);
+        }
+        if (tid == 0 && label >= v0 && label < v0 + len && c.label_in_top != (int)(r + 1)) {
+          const float d = c.label_logit - Ms;
+          const float x = ex2(d * kT);
+          grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(d * k1) : (gr + g1) * x) - f1);
+        }
+      }
+      gemm::fence_proxy_async_smem();
+      __syncthreads();  // the next row's copies overwrite the slice
+    } else if (bad) {
+      raise_status(FF_DEVICE_BADARG);
+    }
+    if (!live) {
+      if (a.row_loss && rank == 0 && tid == 0) a.row_loss[r] = 0.f;
+      if (grow)
+        for (int i = tid; i < len; i += THREADS) grow[i] = from_f32<DT>(0.f);
+    }
+  }
+}
+
+// rows that count, one partial count per CTA
+__global__ void __launch_bounds__(256) distill_count_kernel(Args a, int32_t* counts) {
+  __shared__ int tot;
+  if (threadIdx.x == 0) tot = 0;
+  __syncthreads();
+  int n = 0;
+  if (a.labels) {
+    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * 256) {
+      const int64_t y = load_index(a.labels, r, a.labels64);
+      n += y >= 0 && y < a.V && y != a.ignore;
+    }
+  } else {  // a warp per row, until an entry is found
+    const int lane = threadIdx.x & 31;
+    for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < a.rows; r += (int64_t)gridDim.x * 8) {
+      bool any = false;
+      for (int j = lane; j - lane < a.K && !any; j += 32) {
+        bool on = false;
+        if (j < a.K) {
+          const int64_t id = load_index(a.ids, r * a.ldi + j, a.ids64);
+          on = id >= 0 && id < a.V && load_float(a.tlogits, r * a.ldt + j, a.tdtype) != neg_inf();
+        }
+        any = __any_sync(0xffffffffu, on);
+      }
+      n += any && lane == 0;
+    }
+  }
+  if (n) atomicAdd(&tot, n);  // whole numbers: any order
+  __syncthreads();
+  if (threadIdx.x == 0) counts[blockIdx.x] = tot;
+}
+
+// the rows' losses added in a fixed order (fp64), divided by the number that count
+__global__ void __launch_bounds__(1024) distill_finish_kernel(const float* row_loss, int64_t rows, const int32_t* counts,
+                                                              float* loss, float* held) {
+  __shared__ double part[32];
+  double s = 0.0;
+  for (int64_t r = threadIdx.x; r < rows; r += 1024) s += (double)row_loss[r];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int k = 0; k < 32; ++k) t += part[k];
+    if (counts) {
+      int n = 0;
+      for (int i = 0; i < COUNT_CTAS; ++i) n += counts[i];
+      t /= (double)max(n, 1);
+    }
+    loss[0] = (float)t;
+    if (held) held[0] = 1.f;
+  }
+}
+__global__ void distill_held_kernel(const float* upstream, float* held) { held[0] = upstream[0]; }
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// CTAs per row and elements of a slice: slices of at most 72 KB leave three CTAs on an SM, whose
+// copies and arithmetic overlap; with few rows the row is cut further, so that every SM has work.
+inline bool plan(int64_t rows, int64_t V, int K, int es, int nsm, int* csize, int* slice, int* smem) {
+  auto cut = [&](int c) { return ((V + c - 1) / c + 127) / 128 * 128; };
+  const int fixed = ctrl_bytes() + entry_bytes(K) + 32;
+  int c = 1;
+  while (c < 8 && cut(c) * es > 72 * 1024 - fixed) c *= 2;
+  while (c < 8 && rows * c * 2 <= 2 * nsm && cut(2 * c) * es >= 4096) c *= 2;
+  const int64_t bytes = cut(c) * es + fixed;
+  if (bytes > MAX_SMEM) return false;
+  *csize = c;
+  *slice = (int)cut(c);
+  *smem = (int)bytes;
+  return true;
+}
+
+template <int DT>
+inline int launch(Args& a, cudaStream_t st, const char* name) {
+  int c, smem;
+  FF_REQUIRE(plan(a.rows, a.V, a.K, dtype_size(DT), gemm::num_sms_current(), &c, &a.slice, &smem), FF_ERR_UNSUPPORTED,
+             "%s: a row of %lld logits with %d entries does not fit", name, (long long)a.V, a.K);
+  static bool done[64] = {false};
+  int rc = mx::allow_smem(distill_kernel<DT>, MAX_SMEM, done, name);
+  if (rc) return rc;
+  const int per_sm = smem <= 75 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;
+  const int64_t groups = max64(1, min64(a.rows, (int64_t)gemm::num_sms_current() * per_sm / c));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)c, (unsigned)groups);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)c;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, distill_kernel<DT>, a), name);
+  return check_launch(name);
+}
+
+inline int launch_dt(Args& a, int dtype, cudaStream_t st, const char* name) {
+  return dtype == FF_DTYPE_F32    ? launch<FF_DTYPE_F32>(a, st, name)
+         : dtype == FF_DTYPE_BF16 ? launch<FF_DTYPE_BF16>(a, st, name)
+                                  : launch<FF_DTYPE_F16>(a, st, name);
+}
+
+inline int fill(const char* name, const FfDistillRows* in, Args* a) {
+  FF_REQUIRE(in, FF_ERR_INVALID_ARG, "%s: null pointer", name);
+  FF_REQUIRE(in->rows >= 0 && in->vocab >= 1 && in->top >= 1, FF_ERR_INVALID_ARG, "%s: rows=%lld vocab=%lld top=%lld", name,
+             (long long)in->rows, (long long)in->vocab, (long long)in->top);
+  FF_REQUIRE(in->top <= MAX_TOP, FF_ERR_UNSUPPORTED, "%s: %lld entries per row (at most %d)", name, (long long)in->top, MAX_TOP);
+  FF_REQUIRE(in->rows < ((int64_t)1 << 31) && in->vocab < ((int64_t)1 << 30), FF_ERR_UNSUPPORTED, "%s: rows=%lld vocab=%lld too large",
+             name, (long long)in->rows, (long long)in->vocab);
+  FF_REQUIRE(in->dtype >= FF_DTYPE_F32 && in->dtype <= FF_DTYPE_F16 && in->teacher_dtype >= FF_DTYPE_F32 &&
+                 in->teacher_dtype <= FF_DTYPE_F16,
+             FF_ERR_INVALID_ARG, "%s: bad dtype %d or teacher dtype %d", name, in->dtype, in->teacher_dtype);
+  FF_REQUIRE(in->ld_logits >= in->vocab && in->ld_ids >= in->top && in->ld_teacher >= in->top, FF_ERR_INVALID_ARG,
+             "%s: bad leading dims", name);
+  FF_REQUIRE(in->temperature > 0.f && in->temperature < 1e30f && in->alpha >= 0.f && in->alpha <= 1.f, FF_ERR_INVALID_ARG,
+             "%s: temperature=%g (positive), alpha=%g (0 to 1)", name, in->temperature, in->alpha);
+  if (in->rows > 0)
+    FF_REQUIRE(in->logits && in->ids && in->teacher_logits && aligned(in->logits, dtype_size(in->dtype)), FF_ERR_INVALID_ARG,
+               "%s: null or unaligned pointer", name);
+  *a = Args{};
+  a->logits = in->logits;
+  a->rows = in->rows;
+  a->V = in->vocab;
+  a->ldl = in->ld_logits;
+  a->ids = in->ids;
+  a->tlogits = in->teacher_logits;
+  a->labels = in->labels;
+  a->lse = in->teacher_lse;
+  a->ldi = in->ld_ids;
+  a->ldt = in->ld_teacher;
+  a->ignore = in->ignore_index;
+  a->K = (int)in->top;
+  a->ids64 = in->ids_64;
+  a->tdtype = in->teacher_dtype;
+  a->labels64 = in->labels_64;
+  a->T = in->temperature;
+  a->alpha = in->alpha;
+  return FF_OK;
+}
+
+}  // namespace distill
+}  // namespace ff
+
+extern "C" int ff_distill_loss(const FfDistillRows* in, int reduction, float* row_loss, float* loss, void* grad, int64_t ldg,
+                               float* held, int32_t* counts, void* stream) {
+  using namespace ff::distill;
+  Args a;
+  int rc = fill("ff_distill_loss", in, &a);
+  if (rc) return rc;
+  FF_REQUIRE(reduction >= FF_REDUCE_NONE && reduction <= FF_REDUCE_SUM, FF_ERR_INVALID_ARG, "ff_distill_loss: bad reduction %d",
+             reduction);
+  FF_REQUIRE(!grad || (ldg >= a.V && reduction != FF_REDUCE_NONE), FF_ERR_INVALID_ARG,
+             "ff_distill_loss: a gradient comes with a reduction, ldg=%lld", (long long)ldg);
+  FF_REQUIRE(reduction == FF_REDUCE_NONE || loss, FF_ERR_INVALID_ARG, "ff_distill_loss: null loss");
+  FF_REQUIRE(reduction != FF_REDUCE_MEAN || counts, FF_ERR_INVALID_ARG, "ff_distill_loss: the mean needs counts");
+  cudaStream_t st = ff::as_stream(stream);
+  if (a.rows == 0) {
+    if (reduction == FF_REDUCE_MEAN) FF_CUDA_TRY(cudaMemsetAsync(counts, 0, COUNT_CTAS * 4, st), "ff_distill_loss");
+    if (reduction != FF_REDUCE_NONE) FF_CUDA_TRY(cudaMemsetAsync(loss, 0, 4, st), "ff_distill_loss");
+    return FF_OK;
+  }
+  FF_REQUIRE(row_loss, FF_ERR_INVALID_ARG, "ff_distill_loss: null row_loss");
+  if (reduction == FF_REDUCE_MEAN) {
+    distill_count_kernel<<<COUNT_CTAS, 256, 0, st>>>(a, counts);
+    rc = ff::check_launch("ff_distill_loss count");
+    if (rc) return rc;
+    a.mean = 1;
+    a.counts = counts;
+  }
+  a.row_loss = row_loss;
+  a.grad = grad;
+  a.ldg = ldg;
+  rc = launch_dt(a, in->dtype, st, "ff_distill_loss");
+  if (rc || reduction == FF_REDUCE_NONE) return rc;
+  distill_finish_kernel<<<1, 1024, 0, st>>>(row_loss, a.rows, reduction == FF_REDUCE_MEAN ? counts : nullptr, loss,
+                                          grad ? held : nullptr);
+  return ff::check_launch("ff_distill_loss finish");
+}
+
+extern "C" int ff_distill_grad(const FfDistillRows* in, int reduction, const float* upstream, float* held,
+                               int keep_held, const int32_t* counts, void* grad, int64_t ldg, void* stream) {
+  using namespace ff::distill;
+  Args a;
+  int rc = fill("ff_distill_grad", in, &a);
+  if (rc) return rc;
+  FF_REQUIRE(reduction >= FF_REDUCE_NONE && reduction <= FF_REDUCE_SUM, FF_ERR_INVALID_ARG, "ff_distill_grad: bad reduction %d",
+             reduction);
+  FF_REQUIRE(ldg >= a.V && (reduction != FF_REDUCE_MEAN || counts) && !(held && reduction == FF_REDUCE_NONE),
+             FF_ERR_INVALID_ARG, "ff_distill_grad: ldg=%lld, counts with the mean, held with a scalar", (long long)ldg);
+  if (a.rows == 0) return FF_OK;
+  FF_REQUIRE(grad && upstream, FF_ERR_INVALID_ARG, "ff_distill_grad: null pointer");
+  a.mean = reduction == FF_REDUCE_MEAN;
+  a.counts = counts;
+  a.grad = grad;
+  a.ldg = ldg;
+  a.upstream = upstream;
+  a.up_stride = reduction == FF_REDUCE_NONE ? 1 : 0;
+  a.held = held;
+  rc = launch_dt(a, in->dtype, ff::as_stream(stream), "ff_distill_grad");
+  if (rc || !held || !keep_held) return rc;
+  distill_held_kernel<<<1, 1, 0, ff::as_stream(stream)>>>(upstream, held);
+  return ff::check_launch("ff_distill_grad held");
+}

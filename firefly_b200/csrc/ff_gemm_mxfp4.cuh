@@ -326,6 +326,287 @@ __global__ void __launch_bounds__(NUM_THREADS)
 }
 
 // ---------------------------------------------------------------------------
+// Large products: a CTA pair per 256 x 256 tile (M = 256, cta_group::2).  Each CTA stages its own 128
+// rows of A and of B and the scales of its rows of A; the scales of all 256 rows of B are needed in
+// both CTAs' TMEM (each multiplies its 128 rows of A with all of them), so each CTA loads them.
+//
+// TMEM: the scales take 24 columns per k-block, which two 256-column accumulators leave no room for.
+// The two accumulators overlap by 64 columns instead ([0, 256) and [192, 448)); a tile's epilogue
+// reads the shared columns first and then lets the next tile's products start, so the tensor core
+// waits for a quarter of the tile's TMEM reads only.  The scales alternate between two slots at 448
+// and 480; before a slot is written again the products of two k-blocks ago have finished (their
+// stage's barrier), while the last k-block's are still running.
+// ---------------------------------------------------------------------------
+constexpr int PR_STAGES = 5;
+constexpr int PR_CODES = 2 * ROWS_BYTES;                 // 128 rows of A and of B
+constexpr int PR_STAGE = PR_CODES + 3 * SF_BYTES;        // and the scales of A (128 rows) and B (256 rows)
+constexpr int PR_EPI_WARPS = 8;
+constexpr int PR_THREADS = 64 + 32 * PR_EPI_WARPS;
+constexpr int PR_ACC1 = 192, PR_SF = 448;
+constexpr int PR_STAGING = PR_EPI_WARPS * 2 * 2048;      // two 32 x 32 bf16 boxes per epilogue warp
+constexpr int PR_SMEM = PR_STAGES * PR_STAGE + 1024 + 512 + PR_STAGING;
+static_assert(PR_SMEM <= 232448, "pair kernel exceeds the shared memory of a CTA");
+
+template <bool GATED>
+__global__ void __launch_bounds__(PR_THREADS, 1)
+    mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmSA,
+                        const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSB,
+                        const __grid_constant__ CUtensorMap tmD, int num_kb, int tiles_m, int tiles_n, Epi ep) {
+  constexpr int ST = PR_STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
+  uint8_t* smem = smem_raw + pad;
+  const uint32_t sbase = raw + pad;
+  auto sA = [&](int s) { return sbase + s * PR_STAGE; };
+  auto sB = [&](int s) { return sbase + s * PR_STAGE + ROWS_BYTES; };
+  auto sSA = [&](int s) { return sbase + s * PR_STAGE + PR_CODES; };
+  auto sSB = [&](int s, int half) { return sbase + s * PR_STAGE + PR_CODES + (1 + half) * SF_BYTES; };
+  uint8_t* ctrl = smem + ST * PR_STAGE;
+  const uint32_t cbase = sbase + ST * PR_STAGE;
+  auto full_bar = [&](int s) { return cbase + 8u * s; };
+  auto empty_bar = [&](int s) { return cbase + 8u * (ST + s); };
+  auto tfull_bar = [&](int a) { return cbase + 8u * (2 * ST + a); };
+  const uint32_t shared_bar = cbase + 8u * (2 * ST + 2);  // leader: the shared columns have been read (16 warps)
+  const uint32_t drain = cbase + 8u * (2 * ST + 3);
+  const uint32_t done_bar = cbase + 8u * (2 * ST + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (2 * ST + 5));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * ST + 5) + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
+  const int total = tiles_m * tiles_n, pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(tfull_bar(0), 1);
+    mbar_init(tfull_bar(1), 1);
+    mbar_init(shared_bar, 2 * PR_EPI_WARPS);
+    mbar_init(drain, 1);
+    mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmSA);
+    tma_prefetch_desc(&tmB);
+    tma_prefetch_desc(&tmSB);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = pair; ok && t < total; t += num_pairs) {
+        int tm, tn;
+        tile_coords(t, tiles_m, tiles_n, tm, tn);
+        const int ra = tm * 2 + (int)rank;  // this CTA's 128 rows of A, in units of 128
+        const int rb0 = GATED ? tn : tn * 2, rb1 = GATED ? (int)(ep.F / 128) + tn : tn * 2 + 1;
+        const int rb = rank ? rb1 : rb0;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!wait_bar(empty_bar(s), phase ^ 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t lbar = mapa_shared(full_bar(s), 0);
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * PR_STAGE);
+          tma_load_2d_pair(sA(s), &tmA, kb * 128, ra * 128, lbar);
+          tma_load_2d_pair(sB(s), &tmB, kb * 128, rb * 128, lbar);
+          tma_load_2d_pair(sSA(s), &tmSA, kb * 256, ra, lbar);
+          tma_load_2d_pair(sSB(s, 0), &tmSB, kb * 256, rb0, lbar);
+          tma_load_2d_pair(sSB(s, 1), &tmSB, kb * 256, rb1, lbar);
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (leader only)
+    if (rank == 0 && lane == 0) {
+      constexpr uint32_t idesc = idesc_mx(256, 256);
+      int s = 0, acc = 0, tile = 0;
+      uint32_t phase = 0, g = 0;  // g: k-blocks issued so far
+      bool ok = true;
+      for (int t = pair; ok && t < total; t += num_pairs, ++tile) {
+        if (tile > 0 && !wait_bar(shared_bar, (uint32_t)(tile - 1) & 1u, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (uint32_t)(acc * PR_ACC1);
+        for (int kb = 0; kb < num_kb; ++kb, ++g) {
+          if (!wait_bar(full_bar(s), phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (g >= 2) {  // the products that read this scale slot: two k-blocks ago
+            const uint32_t u = g - 2;
+            if (!wait_bar(empty_bar((int)(u % ST)), (u / ST) & 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+          }
+          tc_fence_after();
+          const uint32_t sf = tmem + PR_SF + (g & 1u) * 32;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            sf_copy<2>(sf + c * 4, sSA(s) + c * 512);
+            sf_copy<2>(sf + 8 + c * 8, sSB(s, 0) + c * 512);
+            sf_copy<2>(sf + 8 + c * 8 + 4, sSB(s, 1) + c * 512);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_mx<2>(d, smem_desc_k_sw128(sA(s) + k * 32), smem_desc_k_sw128(sB(s) + k * 32), idesc | idesc_sf((k & 1) * 2),
+                      sf + (k >> 1) * 4, sf + 8 + (k >> 1) * 8, (kb | k) != 0);
+          tc_commit_pair(empty_bar(s));
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        tc_commit_pair(tfull_bar(acc));
+        acc ^= 1;
+      }
+      tc_commit(drain);
+      drain_bar(drain, 0);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int lg = warp & 3, eh = (warp - 2) >> 2;  // TMEM lane quarter; which of the quarter's two warps
+    uint8_t* stage = ctrl + 512 + (warp - 2) * 4096;
+    const uint32_t stage_addr = cbase + 512 + (uint32_t)(warp - 2) * 4096;
+    uint32_t nst = 0;
+    int tile = 0;
+    const uint32_t sbar = mapa_shared(shared_bar, 0);
+    for (int t = pair; t < total; t += num_pairs, ++tile) {
+      int tm, tn;
+      tile_coords(t, tiles_m, tiles_n, tm, tn);
+      const int acc = tile & 1;
+      if (!__all_sync(0xffffffffu, wait_bar(tfull_bar(acc), (uint32_t)(tile >> 1) & 1u, abort_flag))) break;
+      tc_fence_after();
+      const int64_t row0 = (int64_t)(tm * 2 + (int)rank) * 128 + lg * 32, row = row0 + lane;
+      const uint32_t tb = tmem + ((uint32_t)(lg * 32) << 16) + (uint32_t)(acc * PR_ACC1);
+      if constexpr (!GATED) {
+        // 32-column chunks: the shared ones (6, 7 of accumulator 0; 0, 1 of accumulator 1) first
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+          const int c = i == 0 ? (acc ? eh : 6 + eh) : (acc ? 2 : 0) + eh * 3 + (i - 1);
+          const int64_t col0 = (int64_t)tn * 256 + c * 32;
+          uint32_t r[32];
+          tmem_ld32(tb + c * 32, r);
+          tmem_wait_ld();
+          if (i == 0) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(sbar);
+          }
+          if (col0 >= ep.N) continue;
+          if (ep.bias) {
+            const float bl = col0 + lane < ep.N ? __ldg(ep.bias + col0 + lane) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __shfl_sync(0xffffffffu, bl, j));
+          }
+          if (ep.tma_store) {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(mk2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+            staged_store<true>(w, &tmD, (int32_t)col0, (int32_t)row0, lane, stage, stage_addr, nst);
+          } else if (row < ep.M) {
+            if (ep.out_f32) {
+              float* o = static_cast<float*>(ep.D) + row * ep.ldd + col0;
+              if (ep.vec && col0 + 32 <= ep.N) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  reinterpret_cast<uint4*>(o)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (col0 + j < ep.N) o[j] = __uint_as_float(r[j]);
+              }
+            } else {
+              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(ep.D) + row * ep.ldd + col0;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col0 + j < ep.N) o[j] = __float2bfloat16_rn(__uint_as_float(r[j]));
+            }
+          }
+        }
+      } else {
+        // 32 features: gate columns c * 32, up columns 128 + c * 32; the pairs that hold shared columns first
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          const int c = (i == 0) == (acc == 0) ? 2 + eh : eh;
+          uint32_t rg[32], ru[32];
+          tmem_ld32(tb + c * 32, rg);
+          tmem_ld32(tb + 128 + c * 32, ru);
+          tmem_wait_ld();
+          if (i == 0) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(sbar);
+          }
+          // one block of h per thread
+          float h[32];
+          uint32_t m = 0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            h[j] = swiglu_h(__uint_as_float(rg[j]), __uint_as_float(ru[j]));
+            m = max(m, __float_as_uint(h[j]) & 0x7FFFFFFFu);
+          }
+          const uint32_t S = mx::scale_code(m);
+          const float inv = mx::inv_scale(S);
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = h[8 * k + e] * inv;
+            w[k] = S == mx::kScaleNan ? 0u : mx::codes8(v);
+          }
+          const int64_t blk = (int64_t)tn * 4 + c;
+          if (row < ep.M) {
+            *reinterpret_cast<uint4*>(ep.hq + row * ep.ldh + blk * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            ep.hs[mx::scale_at(row, blk, ep.hchunks)] = (uint8_t)S;
+          }
+          // the padding chunk of h's scales: by the last tile column
+          if (i == 0 && eh == 0 && tn == tiles_n - 1 && ep.hchunks * 128 > ep.F && row < ((ep.M + 127) & ~(int64_t)127))
+            *reinterpret_cast<uint32_t*>(ep.hs + mx::scale_at(row, ep.F / 32, ep.hchunks)) = 0u;
+        }
+      }
+    }
+    if (nst && lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) spin_ns(20000);  // let any TMA load still in flight land before the CTA exits
+  if (threadIdx.x == 32) {  // neither CTA frees TMEM before the other is done with the pair's allocation
+    mbar_arrive_remote(mapa_shared(done_bar, peer));
+    drain_bar(done_bar, 0);
+  }
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
 // scales as a matrix of 32-bit words, one row per 128 rows of the operand: boxes of 256 words
@@ -382,6 +663,48 @@ inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Ep
   return check_launch("ff_mxfp4_gemm");
 }
 
+template <bool GATED>
+inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, int64_t brows, int max_pairs, cudaStream_t st) {
+  static bool done[64] = {false};
+  int rc = mx::allow_smem(mx_gemm_pair_kernel<GATED>, PR_SMEM, done, "ff_mxfp4_gemm");
+  if (rc) return rc;
+  CUtensorMap ta, tsa, tb, tsb, td;
+  memset(&td, 0, sizeof(td));
+  if ((rc = make_map_codes(&ta, a.q, ep.M, K, a.ld, 128))) return rc;
+  if ((rc = make_map_sf(&tsa, a.s, ep.M, K))) return rc;
+  if ((rc = make_map_codes(&tb, b.q, brows, K, b.ld, 128))) return rc;
+  if ((rc = make_map_sf(&tsb, b.s, brows, K))) return rc;
+  ep.tma_store = !GATED && !ep.out_f32 && ep.vec;
+  if (ep.tma_store && (rc = make_map_out_bf16(&td, ep.D, ep.M, ep.N, ep.ldd, true))) return rc;
+  const int tiles_m = (int)((ep.M + 255) / 256), tiles_n = (int)(GATED ? ep.F / 128 : (ep.N + 255) / 256);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * min64((int64_t)tiles_m * tiles_n, max_pairs)));
+  cfg.blockDim = dim3(PR_THREADS);
+  cfg.dynamicSmemBytes = PR_SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel<GATED>, ta, tsa, tb, tsb, td, (int)((K + KB - 1) / KB), tiles_m,
+                                 tiles_n, ep),
+              "ff_mxfp4_gemm pair launch");
+  return check_launch("ff_mxfp4_gemm (pair)");
+}
+
+// Pair tiles or narrow items?  Times in units of a pair's tile per k-block, measured where noted.
+template <bool GATED>
+inline bool use_pair(const Epi& ep, int64_t K, int max_pairs) {
+  (void)K;
+  if (max_pairs < 1 || ep.M <= 128) return false;
+  const int64_t tiles = (ep.M + 255) / 256 * (GATED ? ep.F / 128 : (ep.N + 255) / 256);
+  if (tiles >= ((int64_t)1 << 31)) return false;
+  return tiles * 2 >= max_pairs;
+}
+
 template <int NW>
 inline int launch_narrow_mp(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, cudaStream_t st) {
   const int64_t num_kb = (K + KB - 1) / KB;
@@ -432,6 +755,8 @@ extern "C" int ff_mxfp4_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, c
   ep.bias = bias;
   ep.out_f32 = out_kind == FF_OUT_F32;
   ep.vec = ff::aligned(D, 16) && (ldd * (ep.out_f32 ? 4 : 2)) % 16 == 0;
+  const int pairs = max_pairs_current();
+  if (use_pair<false>(ep, K, pairs)) return launch_pair<false>(a, b, K, ep, N, pairs, ff::as_stream(stream));
   return launch_narrow_mp<1>(a, b, K, ep, N, ff::as_stream(stream));
 }
 
@@ -458,5 +783,7 @@ extern "C" int ff_mxfp4_swiglu_gemm(const uint8_t* A, int64_t lda, const uint8_t
   ep.hs = hs;
   ep.ldh = ldh;
   ep.hchunks = ff::mx::chunks_of(F);
+  const int pairs = max_pairs_current();
+  if (use_pair<true>(ep, K, pairs)) return launch_pair<true>(a, b, K, ep, 2 * F, pairs, ff::as_stream(stream));
   return launch_narrow_mp<2>(a, b, K, ep, 2 * F, ff::as_stream(stream));
 }

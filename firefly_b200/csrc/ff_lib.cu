@@ -11,6 +11,7 @@
 #include "ff_gemm_i8.cuh"
 #include "ff_mxfp4.cuh"
 #include "ff_gemm_mxfp4.cuh"
+#include "ff_distill.cuh"
 
 #ifndef FF_VERSION_STRING
 #define FF_VERSION_STRING "firefly_b200 0.1.0 sm_100a"

@@ -33,6 +33,7 @@ from torch.nn import functional as F
 
 from . import _capi
 from .bitLinear import BitLinear, collect_bitlinear_modules
+from .distill import distillation_loss
 from .fireflykernels import (
     _ACT_CACHE,
     _accumulate_weight_grad,
@@ -254,6 +255,14 @@ class BitDecoder(nn.Module):
     def loss(self, ids: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
         logits = self(ids)
         return F.cross_entropy(logits.view(-1, logits.shape[-1]), targets.reshape(-1))
+
+    def distill_loss(self, ids: torch.Tensor, targets: torch.Tensor | None, teacher_ids: torch.Tensor,
+                     teacher_logits: torch.Tensor, *, teacher_lse: torch.Tensor | None = None,
+                     temperature: float = 1.0, alpha: float = 0.5) -> torch.Tensor:
+        """``distillation_loss`` of the model's logits against a teacher's top logits [B, S, k] (and the
+        target tokens, unless ``None``)."""
+        return distillation_loss(self(ids), teacher_ids, teacher_logits, targets, teacher_lse=teacher_lse,
+                                 temperature=temperature, alpha=alpha)
 
     def bit_modules(self) -> list[BitLinear]:
         return collect_bitlinear_modules(self)

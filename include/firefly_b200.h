@@ -575,6 +575,49 @@ FF_API int ff_mxfp4_swiglu_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA
                                 const uint8_t* sB, uint8_t* hq, int64_t ldh, uint8_t* hs, int64_t M, int64_t F,
                                 int64_t K, void* stream);
 
+/*
+ * Distillation loss from a teacher's top logits (the reference has no counterpart).  Row r: student
+ * logits s [vocab]; `top` entries (token id, teacher logit t), an entry with a negative id or t = -inf
+ * being absent; optionally a label and the teacher's log-sum-exp of its logits / T.
+ *   p = softmax(t/T) over the entries, or exp(t/T - lse) with the rest of the mass in one bucket for
+ *   all other tokens;  q = softmax(s/T);
+ *   KD = T^2 [sum p (log p - log q) + rest],  L = alpha KD + (1 - alpha) cross-entropy(s, label).
+ * A row whose label is ignore_index (without labels: a row without entries) has loss and gradient 0 and
+ * is not counted by the mean; the mean of no rows is 0.  A token id or label beyond the vocabulary
+ * raises FF_DEVICE_BADARG and is treated as absent / ignored.  A token may occur in several entries.
+ */
+#define FF_REDUCE_NONE 0
+#define FF_REDUCE_MEAN 1
+#define FF_REDUCE_SUM 2
+#define FF_DISTILL_WS_ELEMS 128
+typedef struct FfDistillRows {
+  const void* logits; /* [rows, vocab], leading dimension ld_logits */
+  const void* ids;    /* int32 or int64 [rows, top], leading dimension ld_ids */
+  const void* teacher_logits;
+  const void* labels;       /* int32 or int64 [rows], or NULL */
+  const float* teacher_lse; /* [rows], or NULL */
+  int64_t rows, vocab, top, ld_logits, ld_ids, ld_teacher, ignore_index;
+  int32_t dtype, teacher_dtype, ids_64, labels_64;
+  float temperature, alpha;
+} FfDistillRows;
+
+/*
+ * row_loss: fp32 [rows].  With a reduction also loss (fp32 scalar; row losses added in a fixed order)
+ * and, when grad is given (the logits' dtype, leading dimension ldg), the gradient of that scalar;
+ * held (or NULL) is set to 1, the upstream gradient that grad holds.  counts: int32
+ * [FF_DISTILL_WS_ELEMS] with the mean, which ff_distill_grad reads.
+ */
+FF_API int ff_distill_loss(const FfDistillRows* in, int reduction, float* row_loss, float* loss, void* grad,
+                           int64_t ldg, float* held, int32_t* counts, void* stream);
+
+/*
+ * The gradient for an upstream gradient on the device: a scalar, or one value per row for
+ * FF_REDUCE_NONE.  held (or NULL): grad already holds the gradient for that scalar, and an equal
+ * upstream leaves it as it is; keep_held updates held, for a call that is replayed.
+ */
+FF_API int ff_distill_grad(const FfDistillRows* in, int reduction, const float* upstream, float* held, int keep_held,
+                           const int32_t* counts, void* grad, int64_t ldg, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,368 @@
+"""The distillation loss and its gradient against fp64, over vocabularies, masks, reductions and upstreams."""
+import math
+
+import pytest
+import torch
+
+from firefly_b200 import _capi, distillation_loss
+from firefly_b200.decoder import DecoderConfig, build_decoder
+from oracle import distill_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda")
+DTYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _case(n, V, k, seed, dtype=torch.bfloat16, labels=False, tail=False, T=1.0, pad=True, spread=2.5):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    s = torch.randn(n, V, device=DEV, generator=g) * spread
+    z = s + torch.randn(n, V, device=DEV, generator=g) * 0.7
+    top = torch.topk(z, min(k, V), dim=1)
+    ids, t = top.indices, top.values
+    lse = torch.logsumexp(z / T, 1) if tail else None
+    if pad and n > 2:
+        keep = torch.randint(0, k + 1, (n, 1), device=DEV, generator=g)
+        keep[::3] = k
+        ids = torch.where(torch.arange(ids.shape[1], device=DEV)[None] < keep, ids, torch.full_like(ids, -1))
+    lab = None
+    if labels:
+        lab = torch.randint(0, V, (n,), device=DEV, generator=g)
+        lab[1::4] = -100
+        lab[::5] = ids[::5, 0].clamp(min=0)  # the teacher's first choice is the label
+    return s.to(dtype), ids, t, lab, lse
+
+
+def _check(s, ids, t, lab, lse, T, alpha, reduction="mean", up=1.0, grad_of=None):
+    """Loss and gradient against the oracle.  The loss: log p, log q and their products carry the errors of
+    fp32 exponentials, logarithms and sums (below 2^-19 of the magnitudes that are added).  A gradient element
+    is factor * (q - p): 2^-18 of q + p (the exponential's argument, up to 2^6, is rounded to 2^-24 of itself),
+    then one rounding to the logits' type."""
+    x = s.detach().clone().requires_grad_(True) if grad_of is None else grad_of
+    got = distillation_loss(x, ids, t, lab, teacher_lse=lse, temperature=T, alpha=alpha, reduction=reduction)
+    s64 = s.detach().double().requires_grad_(True)
+    rows, counted, scale = O.losses(s64, ids, t, lab, lse, T, alpha)
+    cnt = max(1, sum(counted))
+    tol = 2.0 ** -19 * (T * T * (4 + scale) + 16)
+    if reduction == "none":
+        assert got.shape == rows.shape
+        assert bool(((got.double() - rows).abs() <= tol).all())
+        u = torch.linspace(0.5, 2.0, s.shape[0], device=DEV) * up
+        got.backward(u)
+        (rows * u.double()).sum().backward()
+        f = u.double()[:, None]
+    else:
+        want = rows.sum() / (cnt if reduction == "mean" else 1)
+        tol = tol.sum() / (cnt if reduction == "mean" else 1) + 2.0 ** -24 * float(want.detach().abs())
+        assert abs(float(got.detach()) - float(want.detach())) <= float(tol)
+        (got * up).backward() if up != 1.0 else got.backward()
+        (want * up).backward()
+        f = up / (cnt if reduction == "mean" else 1)
+    assert x.grad.dtype == s.dtype and x.grad.shape == s.shape
+    want = s64.grad
+    q = torch.softmax(s.double() / T, 1) + torch.softmax(s.double(), 1)
+    p = torch.zeros_like(q)
+    on = (ids >= 0) & (ids < s.shape[1])
+    p.scatter_add_(1, torch.where(on, ids, 0).long(), on.double())
+    if lab is not None:
+        # the label's own term is factor * 1, and the factor (upstream * (1 - alpha) / count, each step rounded)
+        # and the subtraction are off by up to four halves of 2^-23 of it
+        y = torch.zeros_like(q).scatter_(1, lab.clamp(min=0)[:, None], 1.0) * (lab >= 0)[:, None]
+        p = p + y * 2.0 ** -4  # 2^-18 * 2 * 2^-4 = 4 * 2^-23
+    tiny = torch.finfo(s.dtype).smallest_normal * torch.finfo(s.dtype).eps
+    tol = 2.0 ** -18 * f * max(T, 1) * 2 * (q + p) + torch.finfo(s.dtype).eps / 2 * want.abs() + tiny
+    if lse is not None:  # off the entries: q (1 - p_rest / q_rest), with 1 - sum p off by k 2^-24
+        tol = tol + 2.0 ** -18 * f * T
+    off = (x.grad.double() - want).abs()
+    worst = int((off / tol).argmax())
+    assert bool((off <= tol).all()), (float((off / tol).max()), divmod(worst, s.shape[1]))
+    live = torch.tensor(counted, device=DEV)
+    assert not x.grad[~live].any()
+    assert _capi.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,k", [(1, 1, 1), (1, 7, 3), (5, 100, 100), (3, 1000, 1), (9, 4099, 33), (4, 32000, 64),
+                                   (2, 70001, 100), (500, 257, 20)])
+def test_loss_and_gradient(n, V, k, dtype):
+    s, ids, t, _, _ = _case(n, V, k, n + V)
+    _check(s.to(dtype), ids, t, None, None, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("V", [131071, 131072, 250007])
+@pytest.mark.parametrize("n", [1, 3])
+def test_long_vocabularies(V, n):
+    s, ids, t, lab, lse = _case(n, V, 100, V, labels=True, tail=True, pad=False)
+    _check(s, ids, t, lab, lse, 1.0, 0.5)
+    _check(s.float(), ids, t, None, lse, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("T", [1.0, 2.0, 0.7, 4.0])
+@pytest.mark.parametrize("labels,alpha", [(False, 1.0), (True, 0.5), (True, 1.0), (True, 0.0), (False, 0.3)])
+@pytest.mark.parametrize("tail", [False, True])
+def test_temperature_labels_and_tail(T, labels, alpha, tail):
+    s, ids, t, lab, lse = _case(12, 2001, 30, 3, labels=labels, tail=tail, T=T)
+    for dtype in (torch.bfloat16, torch.float32):
+        _check(s.to(dtype), ids, t, lab, lse, T, alpha)
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("up", [1.0, 0.25, 3.0])
+def test_reductions_and_upstream_gradients(reduction, up):
+    s, ids, t, lab, lse = _case(20, 999, 16, 5, labels=True, tail=True, T=2.0)
+    _check(s, ids, t, lab, lse, 2.0, 0.6, reduction, up)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+def test_a_token_in_several_entries(tail):
+    s, ids, t, lab, lse = _case(8, 500, 24, 6, labels=True, tail=False, pad=False)
+    ids[:, 5] = ids[:, 0]
+    ids[:, 9] = ids[:, 0]
+    ids[3:, 11] = ids[3:, 2]
+    ids[7] = ids[7, 0]  # all entries the same token
+    if tail:
+        lse = torch.logsumexp(t.double(), 1).float() + 0.5
+    for dtype in DTYPES:
+        _check(s.to(dtype), ids, t, lab, lse, 1.0, 0.5)
+
+
+def test_many_entries():
+    s, ids, t, _, _ = _case(3, 9000, 4096, 7, pad=False)
+    _check(s, ids, t, None, None, 1.0, 1.0)
+    ids[1, 100:200] = ids[1, 0:100]
+    _check(s, ids, t, None, None, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("mask", ["inf", "lowest"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_masked_logits(mask, dtype):
+    """Tokens masked out of the student's vocabulary, the teacher keeping to the others: by -inf, and by the
+    type's lowest value."""
+    s, ids, t, lab, _ = _case(10, 700, 12, 8, labels=True)
+    s = s.to(dtype)
+    off = torch.ones_like(s, dtype=torch.bool)
+    off.scatter_(1, ids.clamp(min=0), False)
+    off[torch.arange(10, device=DEV), lab.clamp(min=0)] = False
+    off[:, ::2] &= True
+    off[:, 1::2] = False
+    s = torch.where(off, torch.full_like(s, -math.inf if mask == "inf" else torch.finfo(dtype).min), s)
+    x = s.clone().requires_grad_(True)
+    distillation_loss(x, ids, t, lab, alpha=0.5).backward()
+    assert torch.isfinite(x.grad).all() and not x.grad[off].any()
+    keep = torch.where(off, torch.full_like(s, -1e4 if dtype != torch.float16 else torch.finfo(dtype).min), s)
+    y = keep.clone().requires_grad_(True)
+    _check(keep, ids, t, lab, None, 1.0, 0.5, grad_of=y)
+    assert torch.equal(x.grad, y.grad)
+
+
+def test_teacher_entries_of_minus_infinity_and_rows_without_entries():
+    s, ids, t, _, _ = _case(9, 300, 8, 9, pad=False)
+    t[2, 3:] = -math.inf
+    t[4] = -math.inf
+    ids[5] = -1
+    ids[6, 1:] = -7
+    _check(s, ids, t, None, None, 1.5, 1.0)
+    lab = torch.arange(9, device=DEV)
+    _check(s, ids, t, lab, None, 1.5, 0.5)
+
+
+def test_ignored_rows_are_not_read():
+    s, ids, t, lab, lse = _case(12, 4000, 10, 10, labels=True)
+    clean = s.clone().requires_grad_(True)
+    a = distillation_loss(clean, ids, t, lab, alpha=0.5)
+    a.backward()
+    dirty = s.clone()
+    dirty[lab == -100] = math.nan
+    t = torch.where((lab == -100)[:, None], torch.full_like(t, math.nan), t)
+    dirty.requires_grad_(True)
+    b = distillation_loss(dirty, ids, t, lab, alpha=0.5)
+    b.backward()
+    assert torch.equal(a, b) and torch.equal(clean.grad, dirty.grad)
+
+
+def test_a_nan_reaches_the_loss():
+    s, ids, t, _, _ = _case(6, 500, 4, 11, pad=False)
+    s[2, 77] = math.nan
+    row = distillation_loss(s, ids, t, reduction="none")
+    assert bool(torch.isnan(row[2])) and int(torch.isnan(row).sum()) == 1
+
+
+def test_strides_and_alignment():
+    big, ids, t, lab, lse = _case(14, 1037, 9, 12, labels=True, tail=True)
+    for s in (big[:, :1001], big[:, 3:1004], big[2:, 1:1002], big[::2, :1001], big.t().contiguous().t()[:, :1001]):
+        n = s.shape[0]
+        _check(s, ids[:n].clamp(max=1000), t[:n], lab[:n].clamp(max=1000), lse[:n], 1.0, 0.5,
+               grad_of=s.detach().requires_grad_(True))
+    s = big[:, :1001]
+    ref = distillation_loss(s, ids, t)
+    wide = torch.full((14, 40), -5, device=DEV)
+    wide[:, :9] = ids
+    assert torch.equal(distillation_loss(s, wide[:, :9], t), ref)
+    assert torch.equal(distillation_loss(s, ids.int(), t), ref)
+    assert torch.equal(distillation_loss(s.reshape(2, 7, 1001), ids.view(2, 7, 9), t.view(2, 7, 9)), ref)
+    # the cut vocabulary leaves some of the teacher's tokens beyond it
+    assert _capi.device_status() == (_capi.FF_DEVICE_BADARG if bool((ids >= 1001).any()) else 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_teacher_logits_of_16_bits(dtype):
+    s, ids, t, _, _ = _case(7, 800, 12, 13)
+    _check(s, ids, t.to(dtype), None, None, 2.0, 1.0)
+
+
+def test_indexes_beyond_the_vocabulary_are_reported():
+    s, ids, t, lab, _ = _case(6, 200, 5, 14, labels=True, pad=False)
+    ids2, lab2 = ids.clone(), lab.clone()
+    ids2[2, 3] = 200
+    lab2[3] = 4000
+    got = distillation_loss(s, ids2, t, lab2, alpha=0.5)
+    assert _capi.device_status() == _capi.FF_DEVICE_BADARG
+    ids[2, 3], lab[3] = -1, -100
+    assert torch.equal(got, distillation_loss(s, ids, t, lab, alpha=0.5))
+    assert _capi.device_status() == 0
+
+
+def test_no_rows_and_no_counted_rows():
+    x = torch.zeros(0, 50, device=DEV, requires_grad=True)
+    e = torch.zeros(0, 3, device=DEV)
+    for red in ("mean", "sum"):
+        l = distillation_loss(x, e.long(), e, reduction=red)
+        assert float(l.detach()) == 0.0
+        l.backward()
+    assert distillation_loss(x, e.long(), e, reduction="none").shape == (0,)
+    s, ids, t, _, _ = _case(4, 50, 3, 15)
+    x = s.requires_grad_(True)
+    l = distillation_loss(x, ids, t, torch.full((4,), -100, device=DEV), alpha=0.5)
+    l.backward()
+    assert float(l) == 0.0 and not x.grad.any()
+
+
+def test_backward_twice_and_without_gradients():
+    s, ids, t, lab, _ = _case(30, 3000, 16, 16, labels=True)
+    x = s.requires_grad_(True)
+    l = distillation_loss(x, ids, t, lab, alpha=0.5)
+    (g1,) = torch.autograd.grad(l, x, retain_graph=True)
+    first = g1.clone()
+    (g2,) = torch.autograd.grad(l * 2, x, retain_graph=True)
+    (g3,) = torch.autograd.grad(l, x)
+    assert torch.equal(g1, first) and torch.equal(g3, first)
+    torch.testing.assert_close(g2.float(), first.float() * 2, rtol=0, atol=0)  # a power of two: no other rounding
+    with torch.no_grad():
+        assert torch.equal(distillation_loss(x, ids, t, lab, alpha=0.5), l)
+
+
+def test_same_result_every_time():
+    s, ids, t, lab, lse = _case(64, 32000, 64, 17, labels=True, tail=True, T=2.0)
+    x = s.requires_grad_(True)
+    ref = None
+    for _ in range(4):
+        l = distillation_loss(x, ids, t, lab, teacher_lse=lse, temperature=2.0, alpha=0.5)
+        (g,) = torch.autograd.grad(l, x)
+        if ref is not None:
+            assert torch.equal(l, ref[0]) and torch.equal(g, ref[1])
+        ref = (l.detach(), g)
+
+
+def test_gradient_against_differences():
+    s, ids, t, lab, lse = _case(3, 60, 6, 18, dtype=torch.float32, labels=True, tail=True, T=2.0)
+    lab[:] = torch.tensor([3, 5, 7], device=DEV)
+    x = s.clone().requires_grad_(True)
+    distillation_loss(x, ids, t, lab, teacher_lse=lse, temperature=2.0, alpha=0.5, reduction="sum").backward()
+    f = lambda z: O.losses(z, ids, t, lab, lse, 2.0, 0.5)[0].sum()
+    h = 1e-4
+    for r, v in ((0, 3), (0, int(ids[0, 0])), (1, 59), (2, int(ids[2, 5])), (2, 7)):
+        a, b = s.double(), s.double()
+        a, b = a.clone(), b.clone()
+        a[r, v] += h
+        b[r, v] -= h
+        diff = float((f(a) - f(b)) / (2 * h))
+        # the third derivative is at most alpha T^2 / T^3 + 1 in size: h^2 / 6 of it; fp32 in the kernel
+        assert abs(diff - float(x.grad[r, v])) <= 2 * h * h + 1e-10 / h + 2.0 ** -18 * 4
+
+
+def test_captured_and_replayed_with_another_upstream():
+    s, ids, t, lab, _ = _case(40, 5000, 16, 19, labels=True)
+    x = s.clone().requires_grad_(True)
+    up = torch.ones((), device=DEV)
+    def step():
+        l = distillation_loss(x, ids, t, lab, alpha=0.5)
+        return l, torch.autograd.grad(l, x, up)[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        l, grad = step()
+    for k, u in enumerate((1.0, 0.5, 1.0, 2.0, 1.0)):
+        with torch.no_grad():
+            x.copy_(s * (1 + 0.125 * k))
+        up.fill_(u)
+        g.replay()
+        got = l.clone(), grad.clone()
+        want = step()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_backward_alone_captured():
+    """Only the backward pass is replayed, with one upstream gradient after another."""
+    s, ids, t, lab, _ = _case(40, 5000, 16, 20, labels=True)
+    x = s.clone().requires_grad_(True)
+    up = torch.ones((), device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    # the leaf's first graph is made on the stream that captures: torch refuses to capture a backward pass
+    # while an eager graph of the same leaf on the default stream is alive
+    with torch.cuda.stream(side):
+        l = distillation_loss(x, ids, t, lab, alpha=0.5)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            grad = torch.autograd.grad(l, x, up)[0]
+    for u in (1.0, 3.0, 1.0, 1.0, 0.5):
+        up.fill_(u)
+        g.replay()
+        got = grad.clone()
+        y = s.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(distillation_loss(y, ids, t, lab, alpha=0.5), y, up.clone())
+        assert torch.equal(got, want)
+
+
+def test_two_streams_at_once():
+    cases = [_case(50, 8000, 16, s, labels=True) for s in (21, 22)]
+    f = lambda c: distillation_loss(c[0], c[1], c[2], c[3], alpha=0.5)
+    wants = [f(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(f(cases[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for v in got[k]:
+            assert torch.equal(v, wants[k])
+
+
+def test_decoder_distils_from_a_teacher():
+    """The decoder's own path: the teacher's top logits, the student's loss, gradients in every parameter."""
+    cfg = DecoderConfig(vocab=512, d_model=128, heads=4, ffn=256, layers=2, max_seq=64)
+    teacher, student = build_decoder(cfg, DEV, seed=1), build_decoder(cfg, DEV, seed=2)
+    ids = torch.randint(0, cfg.vocab, (2, 65), device=DEV)
+    with torch.no_grad():
+        tl = teacher(ids[:, :-1]).float()
+    top = tl.topk(16, dim=-1)
+    loss = student.distill_loss(ids[:, :-1], ids[:, 1:], top.indices, top.values,
+                                teacher_lse=torch.logsumexp(tl / 2, -1), temperature=2.0, alpha=0.5)
+    with torch.no_grad():
+        logits = student(ids[:, :-1]).double().view(-1, cfg.vocab)
+    want, counted, scale = O.losses(logits, top.indices.view(-1, 16), top.values.view(-1, 16), ids[:, 1:].reshape(-1),
+                                    torch.logsumexp(tl / 2, -1).view(-1), 2.0, 0.5)
+    assert abs(float(loss) - float(want.mean())) <= 2.0 ** -19 * (4 * (4 + float(scale.max())) + 16)
+    loss.backward()
+    for lin in student.bit_modules():
+        g = lin.consume_weight_grad()
+        assert g is not None and torch.isfinite(g).all() and bool(g.any())
+    for p in student.dense_parameters():
+        assert p.grad is not None and torch.isfinite(p.grad).all()

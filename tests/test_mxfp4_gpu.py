@@ -131,7 +131,8 @@ def _check_product(got, a, b, bias=None):
 SHAPES = [(1, 1, 1), (1, 128, 256), (1, 4096, 4096), (2, 130, 64), (16, 256, 512), (17, 1000, 100), (32, 96, 4096),
           (33, 300, 777), (64, 128, 2000), (65, 129, 257), (128, 384, 1024), (129, 65, 320), (200, 500, 300),
           (255, 257, 288), (256, 256, 256), (257, 513, 1100), (512, 768, 2048), (700, 1300, 96), (1000, 3000, 640),
-          (4096, 300, 128), (300, 5000, 31)]
+          (4096, 300, 128), (300, 5000, 31),
+          (1500, 3300, 1100), (2500, 1999, 288), (2304, 2560, 4096), (130, 20000, 512)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -145,7 +146,7 @@ def test_product_against_fp64(M, N, K, out):
     assert _capi.device_status() == 0
 
 
-@pytest.mark.parametrize("M,N,K", [(5, 200, 512), (300, 400, 512), (700, 900, 1024)])
+@pytest.mark.parametrize("M,N,K", [(5, 200, 512), (300, 400, 512), (700, 900, 1024), (1500, 3300, 1024)])
 def test_product_of_whole_numbers_is_exact(M, N, K):
     """Codes times powers of two whose sums stay below 2^24: every order of addition is exact."""
     g = _gen(11)
@@ -163,7 +164,7 @@ def test_product_uses_every_scale():
     """One value per block, every block with its own scale on both sides: a scale taken from a
     neighbouring row or block changes the result."""
     g = _gen(12)
-    for M, N, K in ((40, 300, 1024), (400, 600, 1024)):
+    for M, N, K in ((40, 300, 1024), (400, 600, 1024), (1500, 3300, 1792)):
         a = torch.zeros(M, K, device=DEV)
         b = torch.zeros(N, K, device=DEV)
         a[:, ::32] = torch.exp2(torch.randint(-5, 6, (M, K // 32), device=DEV, generator=g).float())
@@ -173,7 +174,7 @@ def test_product_uses_every_scale():
 
 
 def test_product_is_the_same_every_time():
-    for M, N, K in ((1, 4096, 4096), (20, 1000, 11008), (600, 900, 2048)):
+    for M, N, K in ((1, 4096, 4096), (20, 1000, 11008), (600, 900, 2048), (2000, 4100, 2048)):
         a, b = quantize_fp_to_mxfp4(_randn(M, K, 1)), quantize_fp_to_mxfp4(_randn(N, K, 2))
         first = mxfp4_matmul(a, b, out_dtype=torch.float32)
         for _ in range(4):
@@ -279,7 +280,7 @@ def _flip_tolerance(v, mag, K, dtype, left, right):
 
 
 @pytest.mark.parametrize("T,K,F,N", [(1, 64, 128, 96), (3, 256, 32, 40), (16, 512, 384, 512), (40, 100, 160, 77),
-                                     (130, 256, 256, 300), (300, 320, 640, 256), (513, 512, 128, 260)])
+                                     (130, 256, 256, 300), (300, 320, 640, 256), (513, 512, 128, 260), (1300, 512, 1152, 640), (2200, 256, 640, 300)])
 def test_gated_block_forward_and_gradients(T, K, F, N):
     x = _randn(T, K, 1).requires_grad_(True)
     wgu = _randn(2 * F, K, 2, scale=0.05).requires_grad_(True)
