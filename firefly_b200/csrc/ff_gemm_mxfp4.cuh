@@ -7,8 +7,8 @@
 // instruction are 32 bytes, so a 128-byte swizzled row is 256 values of K, and the operand tiles
 // and descriptors are those of the int8 kernels (ff_gemm_i8.cuh).  The scales of a k-block travel in
 // the order that the tensor core wants (512-byte chunks of 128 rows x 4 blocks): TMA brings two
-// chunks per 128 rows, tcgen05.cp spreads them over TMEM (lane = row % 32, word = row / 32,
-// repeated for the four lane quarters), and the instruction descriptor says which two of a word's
+// chunks per 128 rows, they are spread over TMEM (lane = row % 32, word = row / 32, repeated for
+// the four lane quarters), and the instruction descriptor says which two of a word's
 // four bytes the current 64 values use.
 //
 // Two kernels:
@@ -330,22 +330,63 @@ __global__ void __launch_bounds__(NUM_THREADS)
 // rows of A and of B and the scales of its rows of A; the scales of all 256 rows of B are needed in
 // both CTAs' TMEM (each multiplies its 128 rows of A with all of them), so each CTA loads them.
 //
-// TMEM: the scales take 24 columns per k-block, which two 256-column accumulators leave no room for.
-// The two accumulators overlap by 64 columns instead ([0, 256) and [192, 448)); a tile's epilogue
-// reads the shared columns first and then lets the next tile's products start, so the tensor core
-// waits for a quarter of the tile's TMEM reads only.  The scales alternate between two slots at 448
-// and 480; before a slot is written again the products of two k-blocks ago have finished (their
-// stage's barrier), while the last k-block's are still running.
+// TMEM: the scales need columns that two 256-column accumulators do not leave.  The accumulators
+// overlap by half instead ([0, 256) and [128, 384)); a tile's epilogue reads the shared columns into
+// registers first and then lets the next tile's products start.  Every stage has its slot of 24
+// columns (the scales of one k-block: 8 of A, 16 of B) from column 384 on, so a slot is free as soon as
+// its stage is loaded again.
+//
+// The scale copies are issued by a warp of their own.  In one thread's order copies and products do not
+// overlap (8192x4096x11008: 195 us with a k-block's six copies ahead of its products, 8 us for each of the
+// six, and no gain from copying earlier; 268 us with four warps writing the scales by tcgen05.st); issued
+// from two warps, with a commit and a barrier between them, they do: 144 us = 5.1 PFLOP/s, within 2% of
+// the time without any copies.  What is left is the fill of shared memory: 35 KB per k-block and CTA,
+// 10.8 TB/s over all SMs.
 // ---------------------------------------------------------------------------
 constexpr int PR_STAGES = 5;
 constexpr int PR_CODES = 2 * ROWS_BYTES;                 // 128 rows of A and of B
 constexpr int PR_STAGE = PR_CODES + 3 * SF_BYTES;        // and the scales of A (128 rows) and B (256 rows)
 constexpr int PR_EPI_WARPS = 8;
-constexpr int PR_THREADS = 64 + 32 * PR_EPI_WARPS;
-constexpr int PR_ACC1 = 192, PR_SF = 448;
+constexpr int PR_THREADS = 64 + 32 * PR_EPI_WARPS + 32;  // TMA, MMA, epilogue, scale copies
+constexpr int PR_ACC1 = 128, PR_SF = 384, PR_SF_COLS = 24;
+static_assert(PR_SF + PR_STAGES * PR_SF_COLS <= 512, "TMEM columns");
 constexpr int PR_STAGING = PR_EPI_WARPS * 2 * 2048;      // two 32 x 32 bf16 boxes per epilogue warp
 constexpr int PR_SMEM = PR_STAGES * PR_STAGE + 1024 + 512 + PR_STAGING;
 static_assert(PR_SMEM <= 232448, "pair kernel exceeds the shared memory of a CTA");
+
+// 32 columns of one row (a thread) of the output; all lanes take part
+__device__ __forceinline__ void pair_store(uint32_t (&r)[32], int64_t row, int64_t col0, const Epi& ep, const CUtensorMap* tmD,
+                                           int lane, uint8_t* stage, uint32_t stage_addr, uint32_t& nst) {
+  if (col0 >= ep.N) return;
+  if (ep.bias) {
+    const float bl = col0 + lane < ep.N ? __ldg(ep.bias + col0 + lane) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __shfl_sync(0xffffffffu, bl, j));
+  }
+  if (ep.tma_store) {
+    uint32_t w[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(mk2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
+    staged_store<true>(w, tmD, (int32_t)col0, (int32_t)(row - lane), lane, stage, stage_addr, nst);
+  } else if (row < ep.M) {
+    if (ep.out_f32) {
+      float* o = static_cast<float*>(ep.D) + row * ep.ldd + col0;
+      if (ep.vec && col0 + 32 <= ep.N) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reinterpret_cast<uint4*>(o)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (col0 + j < ep.N) o[j] = __uint_as_float(r[j]);
+      }
+    } else {
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(ep.D) + row * ep.ldd + col0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (col0 + j < ep.N) o[j] = __float2bfloat16_rn(__uint_as_float(r[j]));
+    }
+  }
+}
 
 template <bool GATED>
 __global__ void __launch_bounds__(PR_THREADS, 1)
@@ -370,8 +411,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   const uint32_t shared_bar = cbase + 8u * (2 * ST + 2);  // leader: the shared columns have been read (16 warps)
   const uint32_t drain = cbase + 8u * (2 * ST + 3);
   const uint32_t done_bar = cbase + 8u * (2 * ST + 4);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (2 * ST + 5));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * ST + 5) + 4);
+  auto sf_ready = [&](int s) { return cbase + 8u * (2 * ST + 5 + s); };  // leader: the stage's scales are in TMEM
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (3 * ST + 5));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (3 * ST + 5) + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
@@ -381,6 +423,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     for (int s = 0; s < ST; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
+      mbar_init(sf_ready(s), 1);
     }
     mbar_init(tfull_bar(0), 1);
     mbar_init(tfull_bar(1), 1);
@@ -423,11 +466,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
           }
           const uint32_t lbar = mapa_shared(full_bar(s), 0);
           if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * PR_STAGE);
-          tma_load_2d_pair(sA(s), &tmA, kb * 128, ra * 128, lbar);
-          tma_load_2d_pair(sB(s), &tmB, kb * 128, rb * 128, lbar);
           tma_load_2d_pair(sSA(s), &tmSA, kb * 256, ra, lbar);
           tma_load_2d_pair(sSB(s, 0), &tmSB, kb * 256, rb0, lbar);
           tma_load_2d_pair(sSB(s, 1), &tmSB, kb * 256, rb1, lbar);
+          tma_load_2d_pair(sA(s), &tmA, kb * 128, ra * 128, lbar);
+          tma_load_2d_pair(sB(s), &tmB, kb * 128, rb * 128, lbar);
           if (++s == ST) {
             s = 0;
             phase ^= 1u;
@@ -441,32 +484,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     if (rank == 0 && lane == 0) {
       constexpr uint32_t idesc = idesc_mx(256, 256);
       int s = 0, acc = 0, tile = 0;
-      uint32_t phase = 0, g = 0;  // g: k-blocks issued so far
+      uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; ok && t < total; t += num_pairs, ++tile) {
         if (tile > 0 && !wait_bar(shared_bar, (uint32_t)(tile - 1) & 1u, abort_flag)) break;
-        tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * PR_ACC1);
-        for (int kb = 0; kb < num_kb; ++kb, ++g) {
-          if (!wait_bar(full_bar(s), phase, abort_flag)) {
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!wait_bar(sf_ready(s), phase, abort_flag)) {
             ok = false;
             break;
           }
-          if (g >= 2) {  // the products that read this scale slot: two k-blocks ago
-            const uint32_t u = g - 2;
-            if (!wait_bar(empty_bar((int)(u % ST)), (u / ST) & 1u, abort_flag)) {
-              ok = false;
-              break;
-            }
-          }
           tc_fence_after();
-          const uint32_t sf = tmem + PR_SF + (g & 1u) * 32;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            sf_copy<2>(sf + c * 4, sSA(s) + c * 512);
-            sf_copy<2>(sf + 8 + c * 8, sSB(s, 0) + c * 512);
-            sf_copy<2>(sf + 8 + c * 8 + 4, sSB(s, 1) + c * 512);
-          }
+          const uint32_t sf = tmem + PR_SF + (uint32_t)(s * PR_SF_COLS);
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             mma_mx<2>(d, smem_desc_k_sw128(sA(s) + k * 32), smem_desc_k_sw128(sB(s) + k * 32), idesc | idesc_sf((k & 1) * 2),
@@ -485,6 +514,30 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       drain_bar(drain, 0);
     }
     __syncwarp();
+  } else if (warp == 2 + PR_EPI_WARPS) {
+    // ------------------------------------------------------------ scales into TMEM (leader only)
+    if (rank == 0 && lane == 0) {
+      const uint32_t steps = pair < total ? (uint32_t)((total - pair + num_pairs - 1) / num_pairs) * (uint32_t)num_kb : 0u;
+      int s = 0;
+      uint32_t phase = 0, g = 0;
+      for (; g < steps; ++g) {
+        if (!wait_bar(full_bar(s), phase, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t sf = tmem + PR_SF + (uint32_t)(s * PR_SF_COLS);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          sf_copy<2>(sf + c * 4, sSA(s) + c * 512);
+          sf_copy<2>(sf + 8 + c * 8, sSB(s, 0) + c * 512);
+          sf_copy<2>(sf + 8 + c * 8 + 4, sSB(s, 1) + c * 512);
+        }
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sf_ready(s)) : "memory");
+        if (++s == ST) {
+          s = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int lg = warp & 3, eh = (warp - 2) >> 2;  // TMEM lane quarter; which of the quarter's two warps
@@ -501,71 +554,41 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       tc_fence_after();
       const int64_t row0 = (int64_t)(tm * 2 + (int)rank) * 128 + lg * 32, row = row0 + lane;
       const uint32_t tb = tmem + ((uint32_t)(lg * 32) << 16) + (uint32_t)(acc * PR_ACC1);
+      // the columns that the accumulators share (the upper half of accumulator 0, the lower half of
+      // accumulator 1) are read first: two 32-column chunks per warp, then the next tile may start
+      const int sh = acc ? 0 : 4;
+      uint32_t r0[32], r1[32];
+      tmem_ld32(tb + (sh + eh * 2) * 32, r0);
+      tmem_ld32(tb + (sh + eh * 2 + 1) * 32, r1);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(sbar);
       if constexpr (!GATED) {
-        // 32-column chunks: the shared ones (6, 7 of accumulator 0; 0, 1 of accumulator 1) first
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int c = i == 0 ? (acc ? eh : 6 + eh) : (acc ? 2 : 0) + eh * 3 + (i - 1);
-          const int64_t col0 = (int64_t)tn * 256 + c * 32;
-          uint32_t r[32];
-          tmem_ld32(tb + c * 32, r);
-          tmem_wait_ld();
-          if (i == 0) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_remote(sbar);
-          }
-          if (col0 >= ep.N) continue;
-          if (ep.bias) {
-            const float bl = col0 + lane < ep.N ? __ldg(ep.bias + col0 + lane) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) + __shfl_sync(0xffffffffu, bl, j));
-          }
-          if (ep.tma_store) {
-            uint32_t w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = pack_bf16x2(mk2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])));
-            staged_store<true>(w, &tmD, (int32_t)col0, (int32_t)row0, lane, stage, stage_addr, nst);
-          } else if (row < ep.M) {
-            if (ep.out_f32) {
-              float* o = static_cast<float*>(ep.D) + row * ep.ldd + col0;
-              if (ep.vec && col0 + 32 <= ep.N) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                  reinterpret_cast<uint4*>(o)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (col0 + j < ep.N) o[j] = __uint_as_float(r[j]);
-              }
-            } else {
-              __nv_bfloat16* o = static_cast<__nv_bfloat16*>(ep.D) + row * ep.ldd + col0;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (col0 + j < ep.N) o[j] = __float2bfloat16_rn(__uint_as_float(r[j]));
-            }
-          }
-        }
-      } else {
-        // 32 features: gate columns c * 32, up columns 128 + c * 32; the pairs that hold shared columns first
+        const int64_t col0 = (int64_t)tn * 256 + eh * 64;
+        pair_store(r0, row, col0 + sh * 32, ep, &tmD, lane, stage, stage_addr, nst);
+        pair_store(r1, row, col0 + sh * 32 + 32, ep, &tmD, lane, stage, stage_addr, nst);
 #pragma unroll 1
         for (int i = 0; i < 2; ++i) {
-          const int c = (i == 0) == (acc == 0) ? 2 + eh : eh;
-          uint32_t rg[32], ru[32];
-          tmem_ld32(tb + c * 32, rg);
-          tmem_ld32(tb + 128 + c * 32, ru);
+          tmem_ld32(tb + ((4 - sh) + eh * 2 + i) * 32, r0);
           tmem_wait_ld();
-          if (i == 0) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_remote(sbar);
-          }
+          pair_store(r0, row, col0 + (4 - sh) * 32 + i * 32, ep, &tmD, lane, stage, stage_addr, nst);
+        }
+      } else {
+        // gate features in the lower half, up features in the upper half: one half of each block is here
+        uint32_t ro[32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = eh * 2 + i;
+          tmem_ld32(tb + ((4 - sh) + c) * 32, ro);
+          tmem_wait_ld();
           // one block of h per thread
           float h[32];
           uint32_t m = 0;
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            h[j] = swiglu_h(__uint_as_float(rg[j]), __uint_as_float(ru[j]));
+            const float x = __uint_as_float(i ? r1[j] : r0[j]), y = __uint_as_float(ro[j]);
+            h[j] = swiglu_h(acc ? x : y, acc ? y : x);
             m = max(m, __float_as_uint(h[j]) & 0x7FFFFFFFu);
           }
           const uint32_t S = mx::scale_code(m);
@@ -583,10 +606,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             *reinterpret_cast<uint4*>(ep.hq + row * ep.ldh + blk * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             ep.hs[mx::scale_at(row, blk, ep.hchunks)] = (uint8_t)S;
           }
-          // the padding chunk of h's scales: by the last tile column
-          if (i == 0 && eh == 0 && tn == tiles_n - 1 && ep.hchunks * 128 > ep.F && row < ((ep.M + 127) & ~(int64_t)127))
-            *reinterpret_cast<uint32_t*>(ep.hs + mx::scale_at(row, ep.F / 32, ep.hchunks)) = 0u;
         }
+        // the padding chunk of h's scales: by the last tile column
+        if (eh == 0 && tn == tiles_n - 1 && ep.hchunks * 128 > ep.F && row < ((ep.M + 127) & ~(int64_t)127))
+          *reinterpret_cast<uint32_t*>(ep.hs + mx::scale_at(row, ep.F / 32, ep.hchunks)) = 0u;
       }
     }
     if (nst && lane == 0) bulk_wait_all();
