@@ -81,45 +81,66 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 template <int DT>
-struct Vec {  // 16 bytes of logits
-  static constexpr int N = DT == FF_DTYPE_F32 ? 4 : 8;
-  static __device__ __forceinline__ void get(uint4 w, float (&v)[N]) {
-    if constexpr (DT == FF_DTYPE_F32) {
-      v[0] = __uint_as_float(w.x); v[1] = __uint_as_float(w.y); v[2] = __uint_as_float(w.z); v[3] = __uint_as_float(w.w);
-    } else if constexpr (DT == FF_DTYPE_BF16) {
-      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+struct Vec {  // 16 bytes of logits as packed pairs of floats
+  static constexpr int N = DT == FF_DTYPE_F32 ? 4 : 8, P = N / 2;
+  static __device__ __forceinline__ void get(uint4 w, f2 (&v)[P]) {
+    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[2 * k] = __uint_as_float(q[k] << 16);
-        v[2 * k + 1] = __uint_as_float(q[k] & 0xFFFF0000u);
-      }
-    } else {
-      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < P; ++k) {
+      if constexpr (DT == FF_DTYPE_F32) {
+        v[k] = mk2(__uint_as_float(q[2 * k]), __uint_as_float(q[2 * k + 1]));
+      } else if constexpr (DT == FF_DTYPE_BF16) {
+        v[k] = unpack_bf16x2(q[k]);
+      } else {
         const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q[k]));
-        v[2 * k] = f.x;
-        v[2 * k + 1] = f.y;
+        v[k] = mk2(f.x, f.y);
       }
     }
   }
-  static __device__ __forceinline__ uint4 put(const float (&v)[N]) {
-    if constexpr (DT == FF_DTYPE_F32) {
-      return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-    } else {
-      uint32_t q[4];
+  static __device__ __forceinline__ uint4 put(const f2 (&v)[P]) {
+    uint32_t q[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (DT == FF_DTYPE_BF16) {
-          q[k] = pack_bf16x2(mk2(v[2 * k], v[2 * k + 1]));
-        } else {
-          const __half2 h = __floats2half2_rn(v[2 * k], v[2 * k + 1]);
-          q[k] = *reinterpret_cast<const uint32_t*>(&h);
-        }
+    for (int k = 0; k < P; ++k) {
+      if constexpr (DT == FF_DTYPE_F32) {
+        words2(v[k], q[2 * k], q[2 * k + 1]);
+      } else if constexpr (DT == FF_DTYPE_BF16) {
+        q[k] = pack_bf16x2(v[k]);
+      } else {
+        float a, b;
+        un2(v[k], a, b);
+        const __half2 h = __floats2half2_rn(a, b);
+        q[k] = *reinterpret_cast<const uint32_t*>(&h);
       }
-      return make_uint4(q[0], q[1], q[2], q[3]);
     }
+    return make_uint4(q[0], q[1], q[2], q[3]);
   }
+  // running maximum of a 16-byte word, two values at a time in the type itself where it has 16 bits
+  struct Max {
+    float f;
+    __nv_bfloat162 b;
+    __half2 h;
+    __device__ __forceinline__ Max() {
+      f = __uint_as_float(0xFF800000u);
+      b.x = b.y = __ushort_as_bfloat16(0xFF80);
+      h.x = h.y = __ushort_as_half(0xFC00);
+    }
+    __device__ __forceinline__ void add(uint4 w) {
+      if constexpr (DT == FF_DTYPE_F32) {
+        f = fmaxf(f, fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w))));
+      } else if constexpr (DT == FF_DTYPE_BF16) {
+        const __nv_bfloat162* p = reinterpret_cast<const __nv_bfloat162*>(&w);
+        b = __hmax2(b, __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])));
+      } else {
+        const __half2* p = reinterpret_cast<const __half2*>(&w);
+        h = __hmax2(h, __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3])));
+      }
+    }
+    __device__ __forceinline__ float value() const {
+      if constexpr (DT == FF_DTYPE_F32) return f;
+      else if constexpr (DT == FF_DTYPE_BF16) return fmaxf(__bfloat162float(b.x), __bfloat162float(b.y));
+      else return fmaxf(__half2float(h.x), __half2float(h.y));
+    }
+  };
 };
 template <int DT>
 __device__ __forceinline__ typename Elem<DT>::T from_f32(float v) {
@@ -153,10 +174,34 @@ struct Ctrl {
 __host__ __device__ constexpr int ctrl_bytes() { return (int)((sizeof(Ctrl) + 127) / 128 * 128); }
 __host__ __device__ inline int entry_bytes(int K) { return (K * 12 + 127) / 128 * 128; }
 
-template <int DT>
+// How the softmax at temperature 1 is had beside the one at T (PW): 1: it is the same, or not needed;
+// 2, 4: T is that, and exp(x) = exp(x / T)^T by squaring; 0: an exponential of its own.  The
+// exponentials are what the kernel computes most of (the special-function unit takes 16 a cycle and SM:
+// two per logit are 230 us of a 16384 x 32000 batch, four 460 us, its bytes 320 us).
+template <int PW>
+__device__ __forceinline__ f2 at_one(f2 x, f2 v, f2 k1, f2 nm1) {
+  if constexpr (PW == 2) {
+    return mul2(x, x);
+  } else if constexpr (PW == 4) {
+    x = mul2(x, x);
+    return mul2(x, x);
+  } else {
+    float a, b;
+    un2(fma2(v, k1, nm1), a, b);
+    return mk2(ex2(a), ex2(b));
+  }
+}
+__device__ __forceinline__ f2 ex2_2(f2 y) {
+  float a, b;
+  un2(y, a, b);
+  return mk2(ex2(a), ex2(b));
+}
+
+template <int DT, int PW>
 __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
   using T = typename Elem<DT>::T;
-  constexpr int N = Vec<DT>::N, ES = (int)sizeof(T);
+  constexpr int N = Vec<DT>::N, P = Vec<DT>::P, ES = (int)sizeof(T);
+  constexpr bool two = PW != 1;  // a second softmax at T = 1
   extern __shared__ __align__(128) uint8_t smem[];
   Ctrl& c = *reinterpret_cast<Ctrl*>(smem);
   int* e_pos = reinterpret_cast<int*>(smem + ctrl_bytes());  // place in this slice, or -1
@@ -185,8 +230,7 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
   __syncthreads();
   if (csize > 1) gemm::cluster_sync_all();  // every CTA of the cluster runs before its memory is written to
 
-  const float inv_t = 1.f / a.T, kT = 1.4426950408889634f * inv_t, k1 = 1.4426950408889634f;
-  const bool two = a.labels != nullptr && a.T != 1.f && a.alpha != 1.f;  // a second softmax at T = 1
+  const float inv_t = 1.f / a.T, kT = 1.4426950408889634f * inv_t, k1 = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
   const int64_t v0 = (int64_t)rank * a.slice;
   const int len = (int)max64(0, min64(a.slice, a.V - v0));
   uint32_t phase = 0, par = 0;
@@ -293,13 +337,10 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
 
       // ---- largest logit; the entries' logits
       const uint4* w = reinterpret_cast<const uint4*>(data);
-      float m = neg_inf();
-      for (int k = tid; k < words; k += THREADS) {
-        float v[N];
-        Vec<DT>::get(w[k], v);
-#pragma unroll
-        for (int e = 0; e < N; ++e) m = fmaxf(m, v[e]);
-      }
+      typename Vec<DT>::Max mx;
+#pragma unroll 4
+      for (int k = tid; k < words; k += THREADS) mx.add(w[k]);
+      float m = mx.value();
       for (int j = tid; j < a.K; j += THREADS)
         if (e_pos[j] >= 0) e_s[j] = Elem<DT>::to_f32(s[e_pos[j]]);
       if (tid == 0 && label >= v0 && label < v0 + len) c.label_logit = Elem<DT>::to_f32(s[label - v0]);
@@ -317,6 +358,9 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
         }
       __syncthreads();
       const float ms = m == neg_inf() ? 0.f : m;  // a slice of -inf sums to 0
+      // exp((s - m)/T) = 2^(s k - m k): one fused multiply-add with the rounded m k, the same for the
+      // entries, so that its rounding cancels between q's numerator and denominator and in log q
+      const float nmT = -ms * kT, nm1 = -ms * k1;
       float sum = 0.f, sum1 = 0.f, rest = 0.f, dot = 0.f, psum = 0.f;
       for (int j = tid; j < a.K; j += THREADS) {
         const int pos = e_pos[j];
@@ -324,13 +368,13 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
         uint32_t owner;
         if constexpr (ES == 2) owner = reinterpret_cast<volatile uint16_t*>(s)[pos];
         else owner = reinterpret_cast<volatile uint32_t*>(s)[pos];
-        const float d = e_s[j] - ms, p = expf(e_p[j]);
-        if (p > 0.f) dot += p * (e_p[j] - d * inv_t);
+        const float y = fmaf(e_s[j], kT, nmT), p = expf(e_p[j]);
+        if (p > 0.f) dot += p * (e_p[j] - y * kLn2);
         else if (p != p) dot = p;
         psum += p;
         if (owner == (uint32_t)j) {
-          sum += ex2(d * kT);
-          if (two) sum1 += ex2(d * k1);
+          sum += ex2(y);
+          if (two) sum1 += ex2(fmaf(e_s[j], k1, nm1));
           s[pos] = from_f32<DT>(neg_inf());  // never the index of an entry: MAX_TOP is below its bits
         } else {
           c.dup = 1;
@@ -339,15 +383,25 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
       }
       __syncthreads();
       // ---- sums of exp over the tokens outside the entries
-      for (int k = tid; k < words; k += THREADS) {
-        float v[N];
-        Vec<DT>::get(w[k], v);
+      f2 acc = splat(0.f), acc1 = splat(0.f);
+      {
+        const f2 kT2 = splat(kT), nT2 = splat(nmT), k12 = splat(k1), n12 = splat(nm1);
+#pragma unroll 2
+        for (int k = tid; k < words; k += THREADS) {
+          f2 v[P];
+          Vec<DT>::get(w[k], v);
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-          const float d = v[e] - ms;
-          rest += ex2(d * kT);
-          if (two) sum1 += ex2(d * k1);
+          for (int e = 0; e < P; ++e) {
+            const f2 x = ex2_2(fma2(v[e], kT2, nT2));
+            acc = add2(acc, x);
+            if (two) acc1 = add2(acc1, at_one<PW>(x, v[e], k12, n12));
+          }
         }
+        float p, q;
+        un2(acc, p, q);
+        rest = p + q;
+        un2(acc1, p, q);
+        sum1 += p + q;
       }
       sum += rest;
       float vals[5] = {sum, sum1, rest, dot, psum};
@@ -386,18 +440,19 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
         all.label = neg_inf();
         for (int k = 0; k < csize; ++k) {
           const Part q = c.parts[par][k];
-          const float d = (q.m == neg_inf() ? 0.f : q.m) - Ms;
-          const float f = q.m == neg_inf() ? 1.f : ex2(d * kT), f1 = q.m == neg_inf() ? 1.f : ex2(d * k1);
+          // from 2^(s k - m k) to 2^(s k - M k): the difference of the two rounded products
+          const float d = q.m == neg_inf() ? 0.f : Ms * kT - q.m * kT;
+          const float f = ex2(-d), f1 = q.m == neg_inf() ? 1.f : ex2(q.m * k1 - Ms * k1);
           all.sum += q.sum * f;
           all.sum1 += q.sum1 * f1;
           all.rest += q.rest * f;
-          all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot - q.psum * d * inv_t : 0.f;
+          all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot + q.psum * d * kLn2 : 0.f;
           all.psum += q.psum;
           all.label = fmaxf(all.label, q.label);
         }
         par ^= 1u;
       }
-      const float Ms = all.m == neg_inf() ? 0.f : all.m;
+      const float Ms = all.m == neg_inf() ? 0.f : all.m, nMT = -Ms * kT, nM1 = -Ms * k1;
       const float sum1_all = two ? all.sum1 : all.sum;
       const bool has = c.t_stats[1] != 0.f;
       if (!a.labels) live = has;
@@ -412,7 +467,7 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
           if (p_rest > 0.f) kd += p_rest * (logf(p_rest) - logf(q_rest));
           kd *= a.T * a.T;
         }
-        if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - (all.label - Ms);
+        if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - fmaf(all.label, two ? k1 : kT, two ? nM1 : nMT) * kLn2;
         a.row_loss[r] = live ? (a.alpha != 0.f ? a.alpha * kd : 0.f) + (a.alpha != 1.f ? (1.f - a.alpha) * ce : 0.f) : 0.f;
       }
       // ---- the gradient
@@ -422,21 +477,30 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
         const float gq = fk / all.sum, g1 = f1 / sum1_all;       // factors of exp(..) for q and softmax at 1
         const float gr = p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;  // q outside the entries
         const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == mis;
+        const f2 kT2 = splat(kT), nT2 = splat(nMT), k12 = splat(k1), n12 = splat(nM1), gr2 = splat(two ? gr : gr + g1),
+                 g12 = splat(g1);
+#pragma unroll 2
         for (int k = tid; k < words; k += THREADS) {
-          float v[N], g[N];
+          f2 v[P], g[P];
           Vec<DT>::get(w[k], v);
 #pragma unroll
-          for (int e = 0; e < N; ++e) {
-            const float d = v[e] - Ms, x = ex2(d * kT);
-            g[e] = two ? gr * x + g1 * ex2(d * k1) : (gr + g1) * x;
+          for (int e = 0; e < P; ++e) {
+            const f2 x = ex2_2(fma2(v[e], kT2, nT2));
+            g[e] = mul2(gr2, x);
+            if (two) g[e] = fma2(g12, at_one<PW>(x, v[e], k12, n12), g[e]);
           }
           const int i0 = k * N - (int)mis / ES;  // element of the slice
           if (vec && i0 >= 0 && i0 + N <= len) {
             __stcs(reinterpret_cast<uint4*>(grow + i0), Vec<DT>::put(g));
           } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-              if (i0 + e >= 0 && i0 + e < len) grow[i0 + e] = from_f32<DT>(g[e]);
+            for (int e = 0; e < P; ++e) {
+              float x, y;
+              un2(g[e], x, y);
+              const int i = i0 + 2 * e;
+              if (i >= 0 && i < len) grow[i] = from_f32<DT>(x);
+              if (i + 1 >= 0 && i + 1 < len) grow[i + 1] = from_f32<DT>(y);
+            }
           }
         }
         __syncthreads();  // the entries' and the label's own values come after the tokens'
@@ -449,15 +513,13 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
             for (int x = 0; x < a.K; ++x)
               if (e_pos[x] == pos || e_pos[x] == -3 - pos) p += expf(e_p[x]);
           }
-          const float d = e_s[j] - Ms;
-          float g = gq * ex2(d * kT) - fk * p;
-          if (f1 != 0.f) g += g1 * ex2(d * (two ? k1 : kT)) - (v0 + pos == label ? f1 : 0.f);
+          float g = gq * ex2(fmaf(e_s[j], kT, nMT)) - fk * p;
+          if (f1 != 0.f) g += g1 * ex2(fmaf(e_s[j], two ? k1 : kT, two ? nM1 : nMT)) - (v0 + pos == label ? f1 : 0.f);
           grow[pos] = from_f32<DT>(g);
         }
         if (tid == 0 && label >= v0 && label < v0 + len && c.label_in_top != (int)(r + 1)) {
-          const float d = c.label_logit - Ms;
-          const float x = ex2(d * kT);
-          grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(d * k1) : (gr + g1) * x) - f1);
+          const float x = ex2(fmaf(c.label_logit, kT, nMT));
+          grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(fmaf(c.label_logit, k1, nM1)) : (gr + g1) * x) - f1);
         }
       }
       gemm::fence_proxy_async_smem();
@@ -547,20 +609,22 @@ inline bool plan(int64_t rows, int64_t V, int K, int es, int nsm, int* csize, in
   return true;
 }
 
-template <int DT>
+template <int DT, int PW>
 inline int launch(Args& a, cudaStream_t st, const char* name) {
   int c, smem;
   FF_REQUIRE(plan(a.rows, a.V, a.K, dtype_size(DT), gemm::num_sms_current(), &c, &a.slice, &smem), FF_ERR_UNSUPPORTED,
              "%s: a row of %lld logits with %d entries does not fit", name, (long long)a.V, a.K);
   static bool done[64] = {false};
-  int rc = mx::allow_smem(distill_kernel<DT>, MAX_SMEM, done, name);
+  int rc = mx::allow_smem(distill_kernel<DT, PW>, MAX_SMEM, done, name);
   if (rc) return rc;
-  const int per_sm = smem <= 75 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;
-  const int64_t groups = max64(1, min64(a.rows, (int64_t)gemm::num_sms_current() * per_sm / c));
+  // shared memory in three sizes (three, two or one CTA per SM), so that the number of clusters that
+  // run at once is known: a persistent grid larger than that would take a second turn
+  const int size = smem <= 75 * 1024 ? 0 : smem <= 113 * 1024 ? 1 : 2, lc = c == 1 ? 0 : c == 2 ? 1 : c == 4 ? 2 : 3;
+  static const int bytes[3] = {75 * 1024, 113 * 1024, MAX_SMEM};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)c, (unsigned)groups);
+  cfg.gridDim = dim3((unsigned)c, 1);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.dynamicSmemBytes = (size_t)bytes[size];
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -569,14 +633,31 @@ inline int launch(Args& a, cudaStream_t st, const char* name) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, distill_kernel<DT>, a), name);
+  static int resident[64][3][4] = {};
+  int dev = 0;
+  FF_CUDA_TRY(cudaGetDevice(&dev), name);
+  int n = dev < 64 ? resident[dev][size][lc] : 0;
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveClusters(&n, distill_kernel<DT, PW>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = max(1, gemm::num_sms_current() / c);
+    }
+    if (dev < 64) resident[dev][size][lc] = n;
+  }
+  cfg.gridDim = dim3((unsigned)c, (unsigned)min64(a.rows, n));
+  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, distill_kernel<DT, PW>, a), name);
   return check_launch(name);
 }
 
+template <int DT>
+inline int launch_pw(Args& a, cudaStream_t st, const char* name) {
+  if (a.labels == nullptr || a.T == 1.f || a.alpha == 1.f) return launch<DT, 1>(a, st, name);
+  return a.T == 2.f ? launch<DT, 2>(a, st, name) : a.T == 4.f ? launch<DT, 4>(a, st, name) : launch<DT, 0>(a, st, name);
+}
 inline int launch_dt(Args& a, int dtype, cudaStream_t st, const char* name) {
-  return dtype == FF_DTYPE_F32    ? launch<FF_DTYPE_F32>(a, st, name)
-         : dtype == FF_DTYPE_BF16 ? launch<FF_DTYPE_BF16>(a, st, name)
-                                  : launch<FF_DTYPE_F16>(a, st, name);
+  return dtype == FF_DTYPE_F32    ? launch_pw<FF_DTYPE_F32>(a, st, name)
+         : dtype == FF_DTYPE_BF16 ? launch_pw<FF_DTYPE_BF16>(a, st, name)
+                                  : launch_pw<FF_DTYPE_F16>(a, st, name);
 }
 
 inline int fill(const char* name, const FfDistillRows* in, Args* a) {
