@@ -17,7 +17,9 @@
 // slice: the maximum; the entries' logits are gathered and their places overwritten by -inf (which
 // makes the sum of the rest exact instead of 1 - sum q, and leaves each token's first entry as its
 // owner, so a token that occurs twice is summed once); the sum of exp; one exchange of partial
-// results between the CTAs; the gradient of all tokens, then the entries' own.
+// results between the CTAs; the gradient of all tokens, then the entries' own.  While the gradient is
+// formed the next row's copies move into the parts of the slice that have been read, and a ninth warp
+// works out the next row's entries.
 // Maxima, sums and probabilities are fp32; the gradient is rounded once.
 #pragma once
 
@@ -27,8 +29,9 @@
 namespace ff {
 namespace distill {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 256;  // and a warp for the teacher's entries
 constexpr int WARPS = THREADS / 32;
+static_assert(THREADS == 256, "bar_compute counts them");
 constexpr int MAX_TOP = 4096;
 constexpr int MAX_SMEM = 227 * 1024;
 constexpr int COUNT_CTAS = FF_DISTILL_WS_ELEMS;
@@ -66,7 +69,7 @@ __device__ __forceinline__ float load_float(const void* p, int64_t i, int dt) {
 __device__ __forceinline__ float neg_inf() { return __uint_as_float(0xFF800000u); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));  // below 2^-126: 0
   return y;
 }
 __device__ __forceinline__ float warp_max(float v) {
@@ -161,18 +164,19 @@ struct Part {
   float pad;
 };
 
-// shared memory: control, then K entries of 12 bytes, then the slice
+// shared memory: control, then K entries of 20 bytes, then the slice
 struct Ctrl {
   uint64_t bar;
   float red[6][WARPS];
   Part parts[2][8];
-  float t_stats[2];   // of the teacher's entries: the sum of p, whether there is any
+  float t_sum[2];        // of the teacher's entries (two rows in turn): the sum of p,
+  int t_any[2];          // whether there is any,
+  int label_in_top[2];   // whether the label's token is among them
   float label_logit;
   int dup;
-  int label_in_top;
 };
 __host__ __device__ constexpr int ctrl_bytes() { return (int)((sizeof(Ctrl) + 127) / 128 * 128); }
-__host__ __device__ inline int entry_bytes(int K) { return (K * 12 + 127) / 128 * 128; }
+__host__ __device__ inline int entry_bytes(int K) { return (K * 20 + 127) / 128 * 128; }
 
 // How the softmax at temperature 1 is had beside the one at T (PW): 1: it is the same, or not needed;
 // 2, 4: T is that, and exp(x) = exp(x / T)^T by squaring; 0: an exponential of its own.  The
@@ -197,26 +201,29 @@ __device__ __forceinline__ f2 ex2_2(f2 y) {
   return mk2(ex2(a), ex2(b));
 }
 
+// barrier of the compute warps (the teacher's warp takes no part)
+__device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
 template <int DT, int PW>
-__global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
   using T = typename Elem<DT>::T;
   constexpr int N = Vec<DT>::N, P = Vec<DT>::P, ES = (int)sizeof(T);
   constexpr bool two = PW != 1;  // a second softmax at T = 1
   extern __shared__ __align__(128) uint8_t smem[];
   Ctrl& c = *reinterpret_cast<Ctrl*>(smem);
-  int* e_pos = reinterpret_cast<int*>(smem + ctrl_bytes());  // place in this slice, or -1
-  float* e_p = reinterpret_cast<float*>(e_pos + a.K);         // p_j
-  float* e_s = e_p + a.K;                                     // the student's logit (entries of this slice)
+  // the entries, of two rows in turn: log p_j; place in this slice, -1: absent, -2: in another CTA's slice
+  auto pos_of = [&](uint32_t b) { return reinterpret_cast<int*>(smem + ctrl_bytes()) + b * (uint32_t)a.K; };
+  auto logp_of = [&](uint32_t b) { return reinterpret_cast<float*>(smem + ctrl_bytes()) + (2 + b) * (uint32_t)a.K; };
+  float* e_s = reinterpret_cast<float*>(smem + ctrl_bytes()) + 4 * a.K;  // the student's logits of this slice's entries
   uint8_t* data = smem + ctrl_bytes() + entry_bytes(a.K);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int csize = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster spans grid x
+  const int csize = (int)gridDim.x, rank = (int)blockIdx.x;  // the cluster spans grid x
   const uint32_t bar = gemm::smem_u32(&c.bar);
 
   if (a.held && __ldg(a.upstream) == __ldg(a.held)) return;  // every CTA of the grid alike
 
   if (tid == 0) {
     gemm::mbar_init(bar, 1);
-    c.label_in_top = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   float inv_count = 1.f;
@@ -227,311 +234,380 @@ __global__ void __launch_bounds__(THREADS) distill_kernel(Args a) {
     for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     inv_count = 1.f / (float)max(n, 1);
   }
-  __syncthreads();
-  if (csize > 1) gemm::cluster_sync_all();  // every CTA of the cluster runs before its memory is written to
 
   const float inv_t = 1.f / a.T, kT = 1.4426950408889634f * inv_t, k1 = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
   const int64_t v0 = (int64_t)rank * a.slice;
-  const int len = (int)max64(0, min64(a.slice, a.V - v0));
-  uint32_t phase = 0, par = 0;
+  const int len = (int)max64(0, min64(a.slice, a.V - v0)), bytes = len * ES;
+  const uint4* w = reinterpret_cast<const uint4*>(data);
 
-  for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-    // ---- does the row count?  (the same answer in every thread of the cluster)
-    int64_t label = -1;
-    bool live = true, bad = false;
-    if (a.labels) {
-      const int64_t y = load_index(a.labels, r, a.labels64);
-      live = y >= 0 && y < a.V && y != a.ignore;
-      bad = !live && y != a.ignore;
-      label = live ? y : -1;
-    }
-    T* grow = a.grad ? static_cast<T*>(a.grad) + r * a.ldg + v0 : nullptr;
-    const T* lrow = static_cast<const T*>(a.logits) + r * a.ldl + v0;
-    const uint32_t mis = (uint32_t)(reinterpret_cast<uintptr_t>(lrow) & 15u);  // bytes into a 16-byte word
-    const int bytes = len * ES;
-    const int head = min(bytes, (int)((16u - mis) & 15u)), body = (bytes - head) & ~15;
-    T* s = reinterpret_cast<T*>(data + mis);  // the slice: element i is token v0 + i
-    const int words = (int)(mis + bytes + 15) / 16;
+  // ---- where a row's slice lies: `mis` bytes into its first 16-byte word; the words [wb, we) are whole
+  struct Geo {
+    const T* src;
+    int mis, head, wb, we, words;
+  };
+  auto geo = [&](int64_t r) {
+    Geo g;
+    g.src = static_cast<const T*>(a.logits) + r * a.ldl + v0;
+    g.mis = (int)(reinterpret_cast<uintptr_t>(g.src) & 15u);
+    g.head = min(bytes, (16 - g.mis) & 15);
+    g.wb = (g.mis + g.head) / 16;
+    g.we = g.wb + (bytes - g.head) / 16;
+    g.words = (g.mis + bytes + 15) / 16;
+    return g;
+  };
+  // thread 0: the copies of the words [from, to) of a row; the first call of a row (from 0) announces all
+  auto issue = [&](const Geo& g, int from, int to) {
+    if (from == 0) gemm::mbar_arrive_expect_tx(bar, (uint32_t)(g.we - g.wb) * 16u);
+    const int b = max(from, g.wb), e = min(to, g.we);
+    const uint8_t* src = reinterpret_cast<const uint8_t*>(g.src) - g.mis;
+    for (int o = b; o < e; o += 1024)
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       gemm::smem_u32(data) + o * 16),
+                   "l"(src + (int64_t)o * 16), "r"(min(1024, e - o) * 16), "r"(bar)
+                   : "memory");
+  };
+  // one warp: the ragged ends by plain loads, and -inf around them up to whole words
+  auto edges = [&](const Geo& g) {
+    T* d = reinterpret_cast<T*>(data + g.mis);
+    const int nh = g.head / ES, t0 = ((g.we * 16) - g.mis) / ES;  // first element after the whole words
+    if (lane < nh) d[lane] = g.src[lane];
+    if (bytes > g.head && lane < len - t0) d[t0 + lane] = g.src[t0 + lane];
+    if (lane < g.mis / ES) reinterpret_cast<T*>(data)[lane] = from_f32<DT>(neg_inf());
+    if (lane < (g.words * 16 - g.mis - bytes) / ES) d[len + lane] = from_f32<DT>(neg_inf());
+  };
+  auto label_ok = [&](int64_t y) { return y >= 0 && y < a.V && y != a.ignore; };
 
-    if (live) {
-      // ---- the slice: whole 16-byte words by bulk copies, the ragged ends by plain loads, and -inf
-      // around them up to whole words
-      if (tid == 0) {
-        gemm::mbar_arrive_expect_tx(bar, (uint32_t)body);
-        const uint8_t* src = reinterpret_cast<const uint8_t*>(lrow) + head;
-        const uint32_t dst = gemm::smem_u32(data) + mis + head;
-        for (int o = 0; o < body; o += 16384) {
-          const uint32_t n = (uint32_t)min(16384, body - o);
-          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                           dst + o),
-                       "l"(src + o), "r"(n), "r"(bar)
-                       : "memory");
-        }
-      }
-      if (warp == 1) {
-        const int nh = head / ES, nt = (bytes - head - body) / ES;
-        if (lane < nh) s[lane] = lrow[lane];
-        if (lane < nt) s[(head + body) / ES + lane] = lrow[(head + body) / ES + lane];
-        if (lane < (int)mis / ES) reinterpret_cast<T*>(data)[lane] = from_f32<DT>(neg_inf());
-        const int past = words * 16 / ES - ((int)mis + bytes) / ES;
-        if (lane < past) s[len + lane] = from_f32<DT>(neg_inf());
-      }
-      // ---- the teacher's entries, by warp 0 while the copies run
-      if (warp == 0) {
-        float tm = neg_inf();
-        for (int j = lane; j < a.K; j += 32) {
-          const int64_t id = load_index(a.ids, r * a.ldi + j, a.ids64);
-          const float t = load_float(a.tlogits, r * a.ldt + j, a.tdtype);
-          const bool on = id >= 0 && id < a.V && t != neg_inf();
-          bad |= id >= a.V;
-          if (on) tm = t > tm || t != t ? t : tm;
-          e_p[j] = on ? t : neg_inf();
-          // absent: -1; in another CTA's slice: -2
-          e_pos[j] = !on ? -1 : (id >= v0 && id < v0 + len) ? (int)(id - v0) : -2;
-          if (on && id == label) c.label_in_top = (int)(r + 1);
-        }
-        tm = warp_max(tm);
-        const bool any = __any_sync(0xffffffffu, tm != neg_inf());
-        float shift = 0.f, zsum = 0.f;
-        __syncwarp();
-        if (a.lse) {
-          shift = __ldg(a.lse + r);
-        } else {
-          for (int j = lane; j < a.K; j += 32)
-            if (e_pos[j] != -1) zsum += expf((e_p[j] - tm) * inv_t);
-          zsum = warp_sum(zsum);
-        }
-        const float lz = a.lse ? 0.f : logf(zsum);
-        float ps = 0.f;
-        for (int j = lane; j < a.K; j += 32) {
-          if (e_pos[j] == -1) {
-            e_p[j] = neg_inf();
-          } else {  // log p_j
-            e_p[j] = a.lse ? e_p[j] * inv_t - shift : (e_p[j] - tm) * inv_t - lz;
-            ps += expf(e_p[j]);
-          }
-        }
-        ps = warp_sum(ps);
-        if (lane == 0) {
-          c.t_stats[0] = ps;
-          c.t_stats[1] = any ? 1.f : 0.f;
-          c.label_logit = neg_inf();
-          c.dup = 0;
-        }
-      }
-      if (bad) raise_status(FF_DEVICE_BADARG);
-      // wait for the copies: past the limit the error is recorded, and the copies in flight are
-      // waited for once more (bounded) so that none lands after the CTA
-      if (!gemm::mbar_try_wait(bar, phase)) {
-        const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns();
-        while (!gemm::mbar_try_wait(bar, phase)) {
-          if (globaltimer_ns() - t0 > limit) {
-            raise_status(FF_DEVICE_TIMEOUT);
-            gemm::drain_bar(bar, phase);
-            break;
-          }
-        }
-      }
-      phase ^= 1u;
-      __syncthreads();
-
-      // ---- largest logit; the entries' logits
-      const uint4* w = reinterpret_cast<const uint4*>(data);
-      typename Vec<DT>::Max mx;
+  // ---- the teacher's warp: log p of a row's entries, their places, sum p
+  auto teacher = [&](int64_t r, int64_t label, uint32_t b) {
+    int* e_pos = pos_of(b);
+    float* e_p = logp_of(b);
+    float tm = neg_inf();
+    bool bad = false, in_top = false;
 #pragma unroll 4
-      for (int k = tid; k < words; k += THREADS) mx.add(w[k]);
-      float m = mx.value();
-      for (int j = tid; j < a.K; j += THREADS)
-        if (e_pos[j] >= 0) e_s[j] = Elem<DT>::to_f32(s[e_pos[j]]);
-      if (tid == 0 && label >= v0 && label < v0 + len) c.label_logit = Elem<DT>::to_f32(s[label - v0]);
-      m = warp_max(m);
-      if (lane == 0) c.red[0][warp] = m;
-      __syncthreads();
-      m = c.red[0][0];
-#pragma unroll
-      for (int k = 1; k < WARPS; ++k) m = fmaxf(m, c.red[0][k]);
-      // ---- every token's place takes the index of one of its entries, which owns it
-      for (int j = tid; j < a.K; j += THREADS)
-        if (e_pos[j] >= 0) {
-          if constexpr (ES == 2) reinterpret_cast<uint16_t*>(s)[e_pos[j]] = (uint16_t)j;
-          else reinterpret_cast<uint32_t*>(s)[e_pos[j]] = (uint32_t)j;
-        }
-      __syncthreads();
-      const float ms = m == neg_inf() ? 0.f : m;  // a slice of -inf sums to 0
-      // exp((s - m)/T) = 2^(s k - m k): one fused multiply-add with the rounded m k, the same for the
-      // entries, so that its rounding cancels between q's numerator and denominator and in log q
-      const float nmT = -ms * kT, nm1 = -ms * k1;
-      float sum = 0.f, sum1 = 0.f, rest = 0.f, dot = 0.f, psum = 0.f;
-      for (int j = tid; j < a.K; j += THREADS) {
-        const int pos = e_pos[j];
-        if (pos < 0) continue;
-        uint32_t owner;
-        if constexpr (ES == 2) owner = reinterpret_cast<volatile uint16_t*>(s)[pos];
-        else owner = reinterpret_cast<volatile uint32_t*>(s)[pos];
-        const float y = fmaf(e_s[j], kT, nmT), p = expf(e_p[j]);
-        if (p > 0.f) dot += p * (e_p[j] - y * kLn2);
-        else if (p != p) dot = p;
-        psum += p;
-        if (owner == (uint32_t)j) {
-          sum += ex2(y);
-          if (two) sum1 += ex2(fmaf(e_s[j], k1, nm1));
-          s[pos] = from_f32<DT>(neg_inf());  // never the index of an entry: MAX_TOP is below its bits
-        } else {
-          c.dup = 1;
-          e_pos[j] = -3 - pos;  // in this slice, but not its owner
-        }
-      }
-      __syncthreads();
-      // ---- sums of exp over the tokens outside the entries
-      f2 acc = splat(0.f), acc1 = splat(0.f);
-      {
-        const f2 kT2 = splat(kT), nT2 = splat(nmT), k12 = splat(k1), n12 = splat(nm1);
+    for (int j = lane; j < a.K; j += 32) {
+      const int64_t id = load_index(a.ids, r * a.ldi + j, a.ids64);
+      const float t = load_float(a.tlogits, r * a.ldt + j, a.tdtype);
+      const bool on = id >= 0 && id < a.V && t != neg_inf();
+      bad |= id >= a.V;
+      if (on) tm = t > tm || t != t ? t : tm;
+      e_p[j] = on ? t : neg_inf();
+      e_pos[j] = !on ? -1 : (id >= v0 && id < v0 + len) ? (int)(id - v0) : -2;
+      in_top |= on && id == label;
+    }
+    const bool any = __any_sync(0xffffffffu, tm != neg_inf());
+    tm = warp_max(tm);
+    __syncwarp();
+    float lz;
+    if (a.lse) {
+      tm = 0.f;
+      lz = __ldg(a.lse + r);
+    } else {
+      float z = 0.f;
 #pragma unroll 2
-        for (int k = tid; k < words; k += THREADS) {
-          f2 v[P];
-          Vec<DT>::get(w[k], v);
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const f2 x = ex2_2(fma2(v[e], kT2, nT2));
-            acc = add2(acc, x);
-            if (two) acc1 = add2(acc1, at_one<PW>(x, v[e], k12, n12));
-          }
-        }
-        float p, q;
-        un2(acc, p, q);
-        rest = p + q;
-        un2(acc1, p, q);
-        sum1 += p + q;
-      }
-      sum += rest;
-      float vals[5] = {sum, sum1, rest, dot, psum};
-#pragma unroll
-      for (int k = 0; k < 5; ++k) vals[k] = warp_sum(vals[k]);
-      if (lane == 0) {
-#pragma unroll
-        for (int k = 0; k < 5; ++k) c.red[k + 1][warp] = vals[k];
-      }
-      __syncthreads();
-      Part mine;
-      {
-        float t[5];
-#pragma unroll
-        for (int k = 0; k < 5; ++k) {
-          t[k] = c.red[k + 1][0];
-#pragma unroll
-          for (int x = 1; x < WARPS; ++x) t[k] += c.red[k + 1][x];
-        }
-        mine = Part{m, t[0], t[1], t[2], t[3], t[4], c.label_logit, 0.f};
-      }
-      Part all = mine;
-      if (csize > 1) {
-        if (tid < csize * 8) {  // word tid % 8 of this CTA's part to CTA tid / 8
-          const uint32_t dst = gemm::mapa_shared(gemm::smem_u32(&c.parts[par][rank]) + (tid & 7) * 4, (uint32_t)(tid >> 3));
-          const float word = (tid & 7) == 0 ? mine.m : (tid & 7) == 1 ? mine.sum : (tid & 7) == 2 ? mine.sum1
-                             : (tid & 7) == 3 ? mine.rest : (tid & 7) == 4 ? mine.dot : (tid & 7) == 5 ? mine.psum
-                             : (tid & 7) == 6 ? mine.label : 0.f;
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(word) : "memory");
-        }
-        gemm::cluster_sync_all();
-        all = c.parts[par][0];
-        for (int k = 1; k < csize; ++k) all.m = fmaxf(all.m, c.parts[par][k].m);
-        const float Ms = all.m == neg_inf() ? 0.f : all.m;
-        all.sum = all.sum1 = all.rest = all.dot = all.psum = 0.f;
-        all.label = neg_inf();
-        for (int k = 0; k < csize; ++k) {
-          const Part q = c.parts[par][k];
-          // from 2^(s k - m k) to 2^(s k - M k): the difference of the two rounded products
-          const float d = q.m == neg_inf() ? 0.f : Ms * kT - q.m * kT;
-          const float f = ex2(-d), f1 = q.m == neg_inf() ? 1.f : ex2(q.m * k1 - Ms * k1);
-          all.sum += q.sum * f;
-          all.sum1 += q.sum1 * f1;
-          all.rest += q.rest * f;
-          all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot + q.psum * d * kLn2 : 0.f;
-          all.psum += q.psum;
-          all.label = fmaxf(all.label, q.label);
-        }
-        par ^= 1u;
-      }
-      const float Ms = all.m == neg_inf() ? 0.f : all.m, nMT = -Ms * kT, nM1 = -Ms * k1;
-      const float sum1_all = two ? all.sum1 : all.sum;
-      const bool has = c.t_stats[1] != 0.f;
-      if (!a.labels) live = has;
-      const float q_rest = all.rest / all.sum;
-      float p_rest = a.lse && has ? fmaxf(1.f - c.t_stats[0], 0.f) : 0.f;
-      if (q_rest == 0.f && p_rest < 1e-5f) p_rest = 0.f;  // nothing outside the entries: 1 - sum p is rounding
-      // ---- the loss
-      if (a.row_loss && rank == 0 && tid == 0) {
-        float kd = 0.f, ce = 0.f;
-        if (has) {
-          kd = all.dot + all.psum * logf(all.sum);
-          if (p_rest > 0.f) kd += p_rest * (logf(p_rest) - logf(q_rest));
-          kd *= a.T * a.T;
-        }
-        if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - fmaf(all.label, two ? k1 : kT, two ? nM1 : nMT) * kLn2;
-        a.row_loss[r] = live ? (a.alpha != 0.f ? a.alpha * kd : 0.f) + (a.alpha != 1.f ? (1.f - a.alpha) * ce : 0.f) : 0.f;
-      }
-      // ---- the gradient
-      if (grow && live) {
-        const float up = a.upstream ? __ldg(a.upstream + r * a.up_stride) * inv_count : inv_count;
-        const float fk = has ? up * a.alpha * a.T : 0.f, f1 = label >= 0 ? up * (1.f - a.alpha) : 0.f;
-        const float gq = fk / all.sum, g1 = f1 / sum1_all;       // factors of exp(..) for q and softmax at 1
-        const float gr = p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;  // q outside the entries
-        const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == mis;
-        const f2 kT2 = splat(kT), nT2 = splat(nMT), k12 = splat(k1), n12 = splat(nM1), gr2 = splat(two ? gr : gr + g1),
-                 g12 = splat(g1);
+      for (int j = lane; j < a.K; j += 32)
+        if (e_pos[j] != -1) z += expf((e_p[j] - tm) * inv_t);
+      lz = logf(warp_sum(z));
+    }
+    float ps = 0.f;
 #pragma unroll 2
-        for (int k = tid; k < words; k += THREADS) {
-          f2 v[P], g[P];
-          Vec<DT>::get(w[k], v);
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const f2 x = ex2_2(fma2(v[e], kT2, nT2));
-            g[e] = mul2(gr2, x);
-            if (two) g[e] = fma2(g12, at_one<PW>(x, v[e], k12, n12), g[e]);
-          }
-          const int i0 = k * N - (int)mis / ES;  // element of the slice
-          if (vec && i0 >= 0 && i0 + N <= len) {
-            __stcs(reinterpret_cast<uint4*>(grow + i0), Vec<DT>::put(g));
-          } else {
-#pragma unroll
-            for (int e = 0; e < P; ++e) {
-              float x, y;
-              un2(g[e], x, y);
-              const int i = i0 + 2 * e;
-              if (i >= 0 && i < len) grow[i] = from_f32<DT>(x);
-              if (i + 1 >= 0 && i + 1 < len) grow[i + 1] = from_f32<DT>(y);
+    for (int j = lane; j < a.K; j += 32) {
+      if (e_pos[j] == -1) continue;
+      const float lp = (e_p[j] - tm) * inv_t - lz;
+      e_p[j] = lp;
+      ps += expf(lp);
+    }
+    ps = warp_sum(ps);
+    in_top = __any_sync(0xffffffffu, in_top);
+    if (bad) raise_status(FF_DEVICE_BADARG);
+    if (lane == 0) {
+      c.t_sum[b] = ps;
+      c.t_any[b] = any;
+      c.label_in_top[b] = in_top;
+    }
+  };
+
+  int64_t r = blockIdx.y;
+  int64_t y = a.labels && r < a.rows ? load_index(a.labels, r, a.labels64) : 0;
+  __syncthreads();
+  if (csize > 1) gemm::cluster_sync_all();  // every CTA of the cluster runs before its memory is written to
+  if (r < a.rows && (!a.labels || label_ok(y))) {
+    if (warp == WARPS) {
+      teacher(r, a.labels ? y : -1, 0);
+    } else {
+      const Geo g = geo(r);
+      if (tid == 0) issue(g, 0, g.words);
+      if (warp == 1) edges(g);
+    }
+  }
+  __syncthreads();
+
+  uint32_t phase = 0, par = 0, buf = 0;
+  for (; r < a.rows; buf ^= 1u) {
+    // does the row count, and the next one of this cluster?  (the same answer in every thread of the cluster)
+    const int64_t rn = r + gridDim.y;
+    const int64_t yn = a.labels && rn < a.rows ? load_index(a.labels, rn, a.labels64) : 0;
+    const bool counted = !a.labels || label_ok(y);
+    const bool ahead = rn < a.rows && (!a.labels || label_ok(yn));
+    const int64_t label = a.labels && counted ? y : -1;
+    bool live = counted;
+
+    if (warp == WARPS) {
+      if (!counted && y != a.ignore && lane == 0) raise_status(FF_DEVICE_BADARG);
+      if (ahead) teacher(rn, a.labels ? yn : -1, buf ^ 1u);
+      __syncwarp();
+      if (counted && csize > 1) gemm::cluster_sync_all();  // the compute warps' exchange
+    } else {
+      const Geo g = geo(r);
+      Geo gn = geo(ahead ? rn : r);
+      T* grow = a.grad ? static_cast<T*>(a.grad) + r * a.ldg + v0 : nullptr;
+      T* s = reinterpret_cast<T*>(data + g.mis);  // the slice: element i is token v0 + i
+      int given = 0;  // words of the next row whose copies have been issued
+      bool under_way = false;
+      if (counted) {
+        int* e_pos = pos_of(buf);
+        const float* e_p = logp_of(buf);
+        // wait for the copies: past the limit the error is recorded, and the copies in flight are
+        // waited for once more (bounded) so that none lands after the CTA
+        if (!gemm::mbar_try_wait(bar, phase)) {
+          const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns();
+          while (!gemm::mbar_try_wait(bar, phase)) {
+            if (globaltimer_ns() - t0 > limit) {
+              raise_status(FF_DEVICE_TIMEOUT);
+              gemm::drain_bar(bar, phase);
+              break;
             }
           }
         }
-        __syncthreads();  // the entries' and the label's own values come after the tokens'
+        phase ^= 1u;
+
+        // ---- largest logit; the entries' logits
+        typename Vec<DT>::Max mx;
+#pragma unroll 4
+        for (int k = tid; k < g.words; k += THREADS) mx.add(w[k]);
+        float m = mx.value();
+        for (int j = tid; j < a.K; j += THREADS)
+          if (e_pos[j] >= 0) e_s[j] = Elem<DT>::to_f32(s[e_pos[j]]);
+        if (tid == 0) {
+          c.label_logit = label >= v0 && label < v0 + len ? Elem<DT>::to_f32(s[label - v0]) : neg_inf();
+          c.dup = 0;
+        }
+        m = warp_max(m);
+        if (lane == 0) c.red[0][warp] = m;
+        bar_compute();
+        m = c.red[0][0];
+#pragma unroll
+        for (int k = 1; k < WARPS; ++k) m = fmaxf(m, c.red[0][k]);
+        // ---- every token's place takes the index of one of its entries, which owns it
+        for (int j = tid; j < a.K; j += THREADS)
+          if (e_pos[j] >= 0) {
+            if constexpr (ES == 2) reinterpret_cast<uint16_t*>(s)[e_pos[j]] = (uint16_t)j;
+            else reinterpret_cast<uint32_t*>(s)[e_pos[j]] = (uint32_t)j;
+          }
+        bar_compute();
+        const float ms = m == neg_inf() ? 0.f : m;  // a slice of -inf sums to 0
+        // exp((s - m)/T) = 2^(s k - m k): one fused multiply-add with the rounded m k, the same for the
+        // entries, so that its rounding cancels between q's numerator and denominator and in log q
+        const float nmT = -ms * kT, nm1 = -ms * k1;
+        float sum = 0.f, sum1 = 0.f, rest = 0.f, dot = 0.f, psum = 0.f;
         for (int j = tid; j < a.K; j += THREADS) {
           const int pos = e_pos[j];
           if (pos < 0) continue;
-          float p = expf(e_p[j]);
-          if (c.dup) {  // the token's entries in order
-            p = 0.f;
-            for (int x = 0; x < a.K; ++x)
-              if (e_pos[x] == pos || e_pos[x] == -3 - pos) p += expf(e_p[x]);
+          uint32_t owner;
+          if constexpr (ES == 2) owner = reinterpret_cast<volatile uint16_t*>(s)[pos];
+          else owner = reinterpret_cast<volatile uint32_t*>(s)[pos];
+          const float z = fmaf(e_s[j], kT, nmT), p = expf(e_p[j]);
+          if (p > 0.f) dot += p * (e_p[j] - z * kLn2);
+          else if (p != p) dot = p;
+          psum += p;
+          if (owner == (uint32_t)j) {
+            sum += ex2(z);
+            if (two) sum1 += ex2(fmaf(e_s[j], k1, nm1));
+            s[pos] = from_f32<DT>(neg_inf());  // never the index of an entry: MAX_TOP is below its bits
+          } else {
+            c.dup = 1;
+            e_pos[j] = -3 - pos;  // in this slice, but not its owner
           }
-          float g = gq * ex2(fmaf(e_s[j], kT, nMT)) - fk * p;
-          if (f1 != 0.f) g += g1 * ex2(fmaf(e_s[j], two ? k1 : kT, two ? nM1 : nMT)) - (v0 + pos == label ? f1 : 0.f);
-          grow[pos] = from_f32<DT>(g);
         }
-        if (tid == 0 && label >= v0 && label < v0 + len && c.label_in_top != (int)(r + 1)) {
-          const float x = ex2(fmaf(c.label_logit, kT, nMT));
-          grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(fmaf(c.label_logit, k1, nM1)) : (gr + g1) * x) - f1);
+        bar_compute();
+        // ---- sums of exp over the tokens outside the entries
+        f2 acc = splat(0.f), acc1 = splat(0.f);
+        {
+          const f2 kT2 = splat(kT), nT2 = splat(nmT), k12 = splat(k1), n12 = splat(nm1);
+#pragma unroll 2
+          for (int k = tid; k < g.words; k += THREADS) {
+            f2 v[P];
+            Vec<DT>::get(w[k], v);
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+              const f2 x = ex2_2(fma2(v[e], kT2, nT2));
+              acc = add2(acc, x);
+              if (two) acc1 = add2(acc1, at_one<PW>(x, v[e], k12, n12));
+            }
+          }
+          float p, q;
+          un2(acc, p, q);
+          rest = p + q;
+          un2(acc1, p, q);
+          sum1 += p + q;
+        }
+        sum += rest;
+        float vals[5] = {sum, sum1, rest, dot, psum};
+#pragma unroll
+        for (int k = 0; k < 5; ++k) vals[k] = warp_sum(vals[k]);
+        if (lane == 0) {
+#pragma unroll
+          for (int k = 0; k < 5; ++k) c.red[k + 1][warp] = vals[k];
+        }
+        if (!grow) gemm::fence_proxy_async_smem();
+        bar_compute();
+        if (!grow && ahead) {  // the slice has been read for the last time
+          if (tid == 0) issue(gn, 0, gn.words);
+          under_way = true;
+        }
+        Part mine;
+        {
+          float t[5];
+#pragma unroll
+          for (int k = 0; k < 5; ++k) {
+            t[k] = c.red[k + 1][0];
+#pragma unroll
+            for (int x = 1; x < WARPS; ++x) t[k] += c.red[k + 1][x];
+          }
+          mine = Part{m, t[0], t[1], t[2], t[3], t[4], c.label_logit, 0.f};
+        }
+        Part all = mine;
+        if (csize > 1) {
+          if (tid < csize * 8) {  // word tid % 8 of this CTA's part to CTA tid / 8
+            const uint32_t dst = gemm::mapa_shared(gemm::smem_u32(&c.parts[par][rank]) + (tid & 7) * 4, (uint32_t)(tid >> 3));
+            const float word = (tid & 7) == 0 ? mine.m : (tid & 7) == 1 ? mine.sum : (tid & 7) == 2 ? mine.sum1
+                               : (tid & 7) == 3 ? mine.rest : (tid & 7) == 4 ? mine.dot : (tid & 7) == 5 ? mine.psum
+                               : (tid & 7) == 6 ? mine.label : 0.f;
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(word) : "memory");
+          }
+          __syncwarp();
+          gemm::cluster_sync_all();
+          all = c.parts[par][0];
+          for (int k = 1; k < csize; ++k) all.m = fmaxf(all.m, c.parts[par][k].m);
+          const float Ms = all.m == neg_inf() ? 0.f : all.m;
+          all.sum = all.sum1 = all.rest = all.dot = all.psum = 0.f;
+          all.label = neg_inf();
+          for (int k = 0; k < csize; ++k) {
+            const Part q = c.parts[par][k];
+            // from 2^(s k - m k) to 2^(s k - M k): the difference of the two rounded products
+            const float d = q.m == neg_inf() ? 0.f : Ms * kT - q.m * kT;
+            const float f = ex2(-d), f1 = q.m == neg_inf() ? 1.f : ex2(q.m * k1 - Ms * k1);
+            all.sum += q.sum * f;
+            all.sum1 += q.sum1 * f1;
+            all.rest += q.rest * f;
+            all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot + q.psum * d * kLn2 : 0.f;
+            all.psum += q.psum;
+            all.label = fmaxf(all.label, q.label);
+          }
+          par ^= 1u;
+        }
+        const float Ms = all.m == neg_inf() ? 0.f : all.m, nMT = -Ms * kT, nM1 = -Ms * k1;
+        const float sum1_all = two ? all.sum1 : all.sum;
+        const bool has = c.t_any[buf] != 0;
+        if (!a.labels) live = has;
+        const float q_rest = all.rest / all.sum;
+        float p_rest = a.lse && has ? fmaxf(1.f - c.t_sum[buf], 0.f) : 0.f;
+        if (q_rest == 0.f && p_rest < 1e-5f) p_rest = 0.f;  // nothing outside the entries: 1 - sum p is rounding
+        // ---- the loss
+        if (a.row_loss && rank == 0 && tid == 0) {
+          float kd = 0.f, ce = 0.f;
+          if (has) {
+            kd = all.dot + all.psum * logf(all.sum);
+            if (p_rest > 0.f) kd += p_rest * (logf(p_rest) - logf(q_rest));
+            kd *= a.T * a.T;
+          }
+          if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - fmaf(all.label, two ? k1 : kT, two ? nM1 : nMT) * kLn2;
+          a.row_loss[r] = live ? (a.alpha != 0.f ? a.alpha * kd : 0.f) + (a.alpha != 1.f ? (1.f - a.alpha) * ce : 0.f) : 0.f;
+        }
+        // ---- the gradient, a quarter of the slice at a time; the next row's copies follow into each
+        // quarter as it has been read
+        if (grow && live) {
+          const float up = a.upstream ? __ldg(a.upstream + r * a.up_stride) * inv_count : inv_count;
+          const float fk = has ? up * a.alpha * a.T : 0.f, f1 = label >= 0 ? up * (1.f - a.alpha) : 0.f;
+          const float gq = fk / all.sum, g1 = f1 / sum1_all;  // factors of exp(..) for q and the softmax at 1
+          const float gr = p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;  // q outside the entries
+          const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == (uint32_t)g.mis;
+          const f2 kT2 = splat(kT), nT2 = splat(nMT), k12 = splat(k1), n12 = splat(nM1), gr2 = splat(two ? gr : gr + g1),
+                   g12 = splat(g1);
+          const int step = (max(g.words, gn.words) + 4 * THREADS - 1) / (4 * THREADS) * THREADS;
+#pragma unroll 1
+          for (int w0 = 0; w0 < g.words; w0 += step) {
+            const int w1 = min(g.words, w0 + step);
+#pragma unroll 2
+            for (int k = w0 + tid; k < w1; k += THREADS) {
+              f2 v[P], gv[P];
+              Vec<DT>::get(w[k], v);
+#pragma unroll
+              for (int e = 0; e < P; ++e) {
+                const f2 x = ex2_2(fma2(v[e], kT2, nT2));
+                gv[e] = mul2(gr2, x);
+                if (two) gv[e] = fma2(g12, at_one<PW>(x, v[e], k12, n12), gv[e]);
+              }
+              const int i0 = k * N - g.mis / ES;  // element of the slice
+              if (vec && i0 >= 0 && i0 + N <= len) {
+                __stcs(reinterpret_cast<uint4*>(grow + i0), Vec<DT>::put(gv));
+              } else {
+#pragma unroll
+                for (int e = 0; e < P; ++e) {
+                  float x0, x1;
+                  un2(gv[e], x0, x1);
+                  const int i = i0 + 2 * e;
+                  if (i >= 0 && i < len) grow[i] = from_f32<DT>(x0);
+                  if (i + 1 >= 0 && i + 1 < len) grow[i + 1] = from_f32<DT>(x1);
+                }
+              }
+            }
+            gemm::fence_proxy_async_smem();
+            bar_compute();
+            if (ahead) {
+              const int to = w0 + step < g.words ? w0 + step : gn.words;
+              if (tid == 0) issue(gn, given, to);
+              given = to;
+              under_way = true;
+            }
+          }
+          if (g.words == 0) bar_compute();
+          // the entries' and the label's own values come after the tokens' (the barrier above)
+          for (int j = tid; j < a.K; j += THREADS) {
+            const int pos = e_pos[j];
+            if (pos < 0) continue;
+            float p = expf(e_p[j]);
+            if (c.dup) {  // the token's entries in order
+              p = 0.f;
+              for (int x = 0; x < a.K; ++x)
+                if (e_pos[x] == pos || e_pos[x] == -3 - pos) p += expf(e_p[x]);
+            }
+            float gv = gq * ex2(fmaf(e_s[j], kT, nMT)) - fk * p;
+            if (f1 != 0.f) gv += g1 * ex2(fmaf(e_s[j], two ? k1 : kT, two ? nM1 : nMT)) - (v0 + pos == label ? f1 : 0.f);
+            grow[pos] = from_f32<DT>(gv);
+          }
+          if (tid == 0 && label >= v0 && label < v0 + len && !c.label_in_top[buf]) {
+            const float x = ex2(fmaf(c.label_logit, kT, nMT));
+            grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(fmaf(c.label_logit, k1, nM1)) : (gr + g1) * x) - f1);
+          }
         }
       }
-      gemm::fence_proxy_async_smem();
-      __syncthreads();  // the next row's copies overwrite the slice
-    } else if (bad) {
-      raise_status(FF_DEVICE_BADARG);
+      if (!live) {
+        if (a.row_loss && rank == 0 && tid == 0) a.row_loss[r] = 0.f;
+        if (grow)
+          for (int i = tid; i < len; i += THREADS) grow[i] = from_f32<DT>(0.f);
+      }
+      if (ahead) {
+        if (!under_way) {  // this row's slice is not needed any more
+          gemm::fence_proxy_async_smem();
+          bar_compute();
+          if (tid == 0) issue(gn, 0, gn.words);
+        }
+        if (warp == 1) edges(gn);
+      }
     }
-    if (!live) {
-      if (a.row_loss && rank == 0 && tid == 0) a.row_loss[r] = 0.f;
-      if (grow)
-        for (int i = tid; i < len; i += THREADS) grow[i] = from_f32<DT>(0.f);
-    }
+    r = rn;
+    y = yn;
+    __syncthreads();  // the next row's entries and edges are there
   }
 }
 
@@ -623,7 +699,7 @@ inline int launch(Args& a, cudaStream_t st, const char* name) {
   static const int bytes[3] = {75 * 1024, 113 * 1024, MAX_SMEM};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)c, 1);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(THREADS + 32);
   cfg.dynamicSmemBytes = (size_t)bytes[size];
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
