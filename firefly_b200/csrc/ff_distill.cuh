@@ -167,16 +167,17 @@ struct Part {
 // shared memory: control, then K entries of 20 bytes, then the slice
 struct Ctrl {
   uint64_t bar;
-  float red[6][WARPS];
+  alignas(16) float red[6][WARPS];
   Part parts[2][8];
   float t_sum[2];        // of the teacher's entries (two rows in turn): the sum of p,
   int t_any[2];          // whether there is any,
-  int label_in_top[2];   // whether the label's token is among them
+  int label_in_top[2];   // whether the label's token is among them,
+  int twice[2];          // whether a token of the slice occurs twice
   float label_logit;
-  int dup;
 };
 __host__ __device__ constexpr int ctrl_bytes() { return (int)((sizeof(Ctrl) + 127) / 128 * 128); }
 __host__ __device__ inline int entry_bytes(int K) { return (K * 20 + 127) / 128 * 128; }
+__host__ __device__ inline int seen_bytes(int64_t slice) { return (int)(slice / 8 + 127) / 128 * 128; }
 
 // How the softmax at temperature 1 is had beside the one at T (PW): 1: it is the same, or not needed;
 // 2, 4: T is that, and exp(x) = exp(x / T)^T by squaring; 0: an exponential of its own.  The
@@ -201,11 +202,21 @@ __device__ __forceinline__ f2 ex2_2(f2 y) {
   return mk2(ex2(a), ex2(b));
 }
 
+// eight warps' values, in warp order
+__device__ __forceinline__ float sum8(const float (&v)[WARPS]) {
+  const float4 x = *reinterpret_cast<const float4*>(v), y = *reinterpret_cast<const float4*>(v + 4);
+  return ((((((x.x + x.y) + x.z) + x.w) + y.x) + y.y) + y.z) + y.w;
+}
+__device__ __forceinline__ float max8(const float (&v)[WARPS]) {
+  const float4 x = *reinterpret_cast<const float4*>(v), y = *reinterpret_cast<const float4*>(v + 4);
+  return fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+}
+
 // barrier of the compute warps (the teacher's warp takes no part)
 __device__ __forceinline__ void bar_compute() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <int DT, int PW>
-__global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
+__global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
   using T = typename Elem<DT>::T;
   constexpr int N = Vec<DT>::N, P = Vec<DT>::P, ES = (int)sizeof(T);
   constexpr bool two = PW != 1;  // a second softmax at T = 1
@@ -215,7 +226,9 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
   auto pos_of = [&](uint32_t b) { return reinterpret_cast<int*>(smem + ctrl_bytes()) + b * (uint32_t)a.K; };
   auto logp_of = [&](uint32_t b) { return reinterpret_cast<float*>(smem + ctrl_bytes()) + (2 + b) * (uint32_t)a.K; };
   float* e_s = reinterpret_cast<float*>(smem + ctrl_bytes()) + 4 * a.K;  // the student's logits of this slice's entries
-  uint8_t* data = smem + ctrl_bytes() + entry_bytes(a.K);
+  // a bit per token of the slice, all zero between rows: the teacher's warp finds repeated tokens with it
+  uint32_t* seen = reinterpret_cast<uint32_t*>(smem + ctrl_bytes() + entry_bytes(a.K));
+  uint8_t* data = smem + ctrl_bytes() + entry_bytes(a.K) + seen_bytes(a.slice);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int csize = (int)gridDim.x, rank = (int)blockIdx.x;  // the cluster spans grid x
   const uint32_t bar = gemm::smem_u32(&c.bar);
@@ -226,6 +239,7 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
     gemm::mbar_init(bar, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  for (int i = tid; i < a.slice / 32; i += THREADS + 32) seen[i] = 0u;
   float inv_count = 1.f;
   if (a.mean) {
     int n = 0;
@@ -282,7 +296,7 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
     int* e_pos = pos_of(b);
     float* e_p = logp_of(b);
     float tm = neg_inf();
-    bool bad = false, in_top = false;
+    bool bad = false, in_top = false, twice = false;
 #pragma unroll 4
     for (int j = lane; j < a.K; j += 32) {
       const int64_t id = load_index(a.ids, r * a.ldi + j, a.ids64);
@@ -296,6 +310,18 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
     }
     const bool any = __any_sync(0xffffffffu, tm != neg_inf());
     tm = warp_max(tm);
+    // a token's first entry in the slice owns it, later ones are marked; then the bits are taken back
+    for (int j0 = 0; j0 < a.K; j0 += 32) {
+      const int j = j0 + lane, pos = j < a.K ? e_pos[j] : -1;
+      const bool first = __ffs(__match_any_sync(0xffffffffu, pos)) - 1 == lane;
+      if (pos >= 0 && (!first || (atomicOr(seen + (pos >> 5), 1u << (pos & 31)) >> (pos & 31) & 1u))) {
+        e_pos[j] = -3 - pos;
+        twice = true;
+      }
+    }
+    __syncwarp();
+    for (int j = lane; j < a.K; j += 32)
+      if (e_pos[j] >= 0) seen[e_pos[j] >> 5] = 0u;
     __syncwarp();
     float lz;
     if (a.lse) {
@@ -318,11 +344,13 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
     }
     ps = warp_sum(ps);
     in_top = __any_sync(0xffffffffu, in_top);
+    twice = __any_sync(0xffffffffu, twice);
     if (bad) raise_status(FF_DEVICE_BADARG);
     if (lane == 0) {
       c.t_sum[b] = ps;
       c.t_any[b] = any;
       c.label_in_top[b] = in_top;
+      c.twice[b] = twice;
     }
   };
 
@@ -342,10 +370,22 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
   __syncthreads();
 
   uint32_t phase = 0, par = 0, buf = 0;
+  // small operands are asked for early, the loaded memory answers late: labels two rows ahead, entries
+  // into L2 two rows ahead
+  int64_t yn = a.labels && r + gridDim.y < a.rows ? load_index(a.labels, r + gridDim.y, a.labels64) : 0;
+  auto entries_to_l2 = [&](int64_t row) {
+    const int isz = a.ids64 ? 8 : 4, tsz = a.tdtype == FF_DTYPE_F32 ? 4 : 2;
+    for (int j = lane * 32; j < a.K * isz; j += 1024)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.ids) + row * a.ldi * isz + j));
+    for (int j = lane * 32; j < a.K * tsz; j += 1024)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(static_cast<const uint8_t*>(a.tlogits) + row * a.ldt * tsz + j));
+    if (a.lse && lane == 0) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.lse + row));
+  };
+  if (warp == WARPS && r + gridDim.y < a.rows) entries_to_l2(r + gridDim.y);
   for (; r < a.rows; buf ^= 1u) {
     // does the row count, and the next one of this cluster?  (the same answer in every thread of the cluster)
     const int64_t rn = r + gridDim.y;
-    const int64_t yn = a.labels && rn < a.rows ? load_index(a.labels, rn, a.labels64) : 0;
+    yn = a.labels && rn < a.rows ? load_index(a.labels, rn, a.labels64) : 0;
     const bool counted = !a.labels || label_ok(y);
     const bool ahead = rn < a.rows && (!a.labels || label_ok(yn));
     const int64_t label = a.labels && counted ? y : -1;
@@ -353,6 +393,7 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
 
     if (warp == WARPS) {
       if (!counted && y != a.ignore && lane == 0) raise_status(FF_DEVICE_BADARG);
+      if (rn + gridDim.y < a.rows) entries_to_l2(rn + gridDim.y);
       if (ahead) teacher(rn, a.labels ? yn : -1, buf ^ 1u);
       __syncwarp();
       if (counted && csize > 1) gemm::cluster_sync_all();  // the compute warps' exchange
@@ -380,30 +421,34 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
         }
         phase ^= 1u;
 
-        // ---- largest logit; the entries' logits
+        // ---- largest logit; the entries' logits, whose places become -inf (their own values go into the
+        // maximum, so it does not matter when another thread comes past)
         typename Vec<DT>::Max mx;
 #pragma unroll 4
         for (int k = tid; k < g.words; k += THREADS) mx.add(w[k]);
         float m = mx.value();
-        for (int j = tid; j < a.K; j += THREADS)
-          if (e_pos[j] >= 0) e_s[j] = Elem<DT>::to_f32(s[e_pos[j]]);
-        if (tid == 0) {
-          c.label_logit = label >= v0 && label < v0 + len ? Elem<DT>::to_f32(s[label - v0]) : neg_inf();
-          c.dup = 0;
+        const bool twice = c.twice[buf] != 0;
+        const bool here = label >= v0 && label < v0 + len;  // the label lies in this slice
+        if (tid == 0 && !(here && c.label_in_top[buf])) c.label_logit = here ? Elem<DT>::to_f32(s[label - v0]) : neg_inf();
+        if (twice) bar_compute();  // a place is read more than once: every read before it changes
+        for (int j = tid; j < a.K; j += THREADS) {
+          const int pos = e_pos[j];
+          if (pos == -1 || pos == -2) continue;
+          const float v = Elem<DT>::to_f32(s[pos >= 0 ? pos : -3 - pos]);
+          e_s[j] = v;
+          m = fmaxf(m, v);
+          if (here && pos == (int)(label - v0)) c.label_logit = v;
+          if (pos >= 0 && !twice) s[pos] = from_f32<DT>(neg_inf());
+        }
+        if (twice) {
+          bar_compute();
+          for (int j = tid; j < a.K; j += THREADS)
+            if (e_pos[j] >= 0) s[e_pos[j]] = from_f32<DT>(neg_inf());
         }
         m = warp_max(m);
         if (lane == 0) c.red[0][warp] = m;
         bar_compute();
-        m = c.red[0][0];
-#pragma unroll
-        for (int k = 1; k < WARPS; ++k) m = fmaxf(m, c.red[0][k]);
-        // ---- every token's place takes the index of one of its entries, which owns it
-        for (int j = tid; j < a.K; j += THREADS)
-          if (e_pos[j] >= 0) {
-            if constexpr (ES == 2) reinterpret_cast<uint16_t*>(s)[e_pos[j]] = (uint16_t)j;
-            else reinterpret_cast<uint32_t*>(s)[e_pos[j]] = (uint32_t)j;
-          }
-        bar_compute();
+        m = max8(c.red[0]);
         const float ms = m == neg_inf() ? 0.f : m;  // a slice of -inf sums to 0
         // exp((s - m)/T) = 2^(s k - m k): one fused multiply-add with the rounded m k, the same for the
         // entries, so that its rounding cancels between q's numerator and denominator and in log q
@@ -411,24 +456,16 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
         float sum = 0.f, sum1 = 0.f, rest = 0.f, dot = 0.f, psum = 0.f;
         for (int j = tid; j < a.K; j += THREADS) {
           const int pos = e_pos[j];
-          if (pos < 0) continue;
-          uint32_t owner;
-          if constexpr (ES == 2) owner = reinterpret_cast<volatile uint16_t*>(s)[pos];
-          else owner = reinterpret_cast<volatile uint32_t*>(s)[pos];
+          if (pos == -1 || pos == -2) continue;
           const float z = fmaf(e_s[j], kT, nmT), p = expf(e_p[j]);
           if (p > 0.f) dot += p * (e_p[j] - z * kLn2);
           else if (p != p) dot = p;
           psum += p;
-          if (owner == (uint32_t)j) {
+          if (pos >= 0) {
             sum += ex2(z);
             if (two) sum1 += ex2(fmaf(e_s[j], k1, nm1));
-            s[pos] = from_f32<DT>(neg_inf());  // never the index of an entry: MAX_TOP is below its bits
-          } else {
-            c.dup = 1;
-            e_pos[j] = -3 - pos;  // in this slice, but not its owner
           }
         }
-        bar_compute();
         // ---- sums of exp over the tokens outside the entries
         f2 acc = splat(0.f), acc1 = splat(0.f);
         {
@@ -451,12 +488,21 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
           sum1 += p + q;
         }
         sum += rest;
-        float vals[5] = {sum, sum1, rest, dot, psum};
-#pragma unroll
-        for (int k = 0; k < 5; ++k) vals[k] = warp_sum(vals[k]);
+        // sums over the CTA: only those that are not zero throughout
+        const bool more = warp * 32 < a.K;  // this warp has entries
+        sum = warp_sum(sum);
+        if (two) sum1 = warp_sum(sum1);
+        if (a.lse) rest = warp_sum(rest);
+        if (more) {
+          dot = warp_sum(dot);
+          psum = warp_sum(psum);
+        }
         if (lane == 0) {
-#pragma unroll
-          for (int k = 0; k < 5; ++k) c.red[k + 1][warp] = vals[k];
+          c.red[1][warp] = sum;
+          c.red[2][warp] = sum1;
+          c.red[3][warp] = rest;
+          c.red[4][warp] = dot;
+          c.red[5][warp] = psum;
         }
         if (!grow) gemm::fence_proxy_async_smem();
         bar_compute();
@@ -464,17 +510,8 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
           if (tid == 0) issue(gn, 0, gn.words);
           under_way = true;
         }
-        Part mine;
-        {
-          float t[5];
-#pragma unroll
-          for (int k = 0; k < 5; ++k) {
-            t[k] = c.red[k + 1][0];
-#pragma unroll
-            for (int x = 1; x < WARPS; ++x) t[k] += c.red[k + 1][x];
-          }
-          mine = Part{m, t[0], t[1], t[2], t[3], t[4], c.label_logit, 0.f};
-        }
+        const Part mine = Part{m, sum8(c.red[1]), two ? sum8(c.red[2]) : 0.f, a.lse ? sum8(c.red[3]) : 0.f, sum8(c.red[4]),
+                               sum8(c.red[5]), c.label_logit, 0.f};
         Part all = mine;
         if (csize > 1) {
           if (tid < csize * 8) {  // word tid % 8 of this CTA's part to CTA tid / 8
@@ -523,8 +560,8 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
           if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - fmaf(all.label, two ? k1 : kT, two ? nM1 : nMT) * kLn2;
           a.row_loss[r] = live ? (a.alpha != 0.f ? a.alpha * kd : 0.f) + (a.alpha != 1.f ? (1.f - a.alpha) * ce : 0.f) : 0.f;
         }
-        // ---- the gradient, a quarter of the slice at a time; the next row's copies follow into each
-        // quarter as it has been read
+        // ---- the gradient, half the slice at a time; the next row's copies follow into each
+        // half as it has been read
         if (grow && live) {
           const float up = a.upstream ? __ldg(a.upstream + r * a.up_stride) * inv_count : inv_count;
           const float fk = has ? up * a.alpha * a.T : 0.f, f1 = label >= 0 ? up * (1.f - a.alpha) : 0.f;
@@ -533,33 +570,38 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
           const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == (uint32_t)g.mis;
           const f2 kT2 = splat(kT), nT2 = splat(nMT), k12 = splat(k1), n12 = splat(nM1), gr2 = splat(two ? gr : gr + g1),
                    g12 = splat(g1);
-          const int step = (max(g.words, gn.words) + 4 * THREADS - 1) / (4 * THREADS) * THREADS;
+          const int step = (max(g.words, gn.words) + 2 * THREADS - 1) / (2 * THREADS) * THREADS;
+          uint4* gw = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(grow) - g.mis);  // word k of the slice
+          auto grad_word = [&](int k) {
+            f2 v[P], gv[P];
+            Vec<DT>::get(w[k], v);
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+              const f2 x = ex2_2(fma2(v[e], kT2, nT2));
+              gv[e] = mul2(gr2, x);
+              if (two) gv[e] = fma2(g12, at_one<PW>(x, v[e], k12, n12), gv[e]);
+            }
+            return Vec<DT>::put(gv);
+          };
+          auto edge_word = [&](int k) {  // element by element: a word that the slice does not fill, or another alignment
+            const uint4 q = grad_word(k);
+            const T* e = reinterpret_cast<const T*>(&q);
+            const int i0 = k * N - g.mis / ES;
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+              if (i0 + x >= 0 && i0 + x < len) grow[i0 + x] = e[x];
+          };
 #pragma unroll 1
           for (int w0 = 0; w0 < g.words; w0 += step) {
             const int w1 = min(g.words, w0 + step);
+            if (vec) {
 #pragma unroll 2
-            for (int k = w0 + tid; k < w1; k += THREADS) {
-              f2 v[P], gv[P];
-              Vec<DT>::get(w[k], v);
-#pragma unroll
-              for (int e = 0; e < P; ++e) {
-                const f2 x = ex2_2(fma2(v[e], kT2, nT2));
-                gv[e] = mul2(gr2, x);
-                if (two) gv[e] = fma2(g12, at_one<PW>(x, v[e], k12, n12), gv[e]);
-              }
-              const int i0 = k * N - g.mis / ES;  // element of the slice
-              if (vec && i0 >= 0 && i0 + N <= len) {
-                __stcs(reinterpret_cast<uint4*>(grow + i0), Vec<DT>::put(gv));
-              } else {
-#pragma unroll
-                for (int e = 0; e < P; ++e) {
-                  float x0, x1;
-                  un2(gv[e], x0, x1);
-                  const int i = i0 + 2 * e;
-                  if (i >= 0 && i < len) grow[i] = from_f32<DT>(x0);
-                  if (i + 1 >= 0 && i + 1 < len) grow[i + 1] = from_f32<DT>(x1);
-                }
-              }
+              for (int k = max(w0, g.wb) + tid; k < min(w1, g.we); k += THREADS) __stcs(gw + k, grad_word(k));
+              if (tid == 0 && w0 == 0 && g.wb > 0) edge_word(0);
+              if (tid == 32 && w1 == g.words && g.words > g.we && (g.words > 1 || g.wb == 0)) edge_word(g.words - 1);
+            } else {
+#pragma unroll 1
+              for (int k = w0 + tid; k < w1; k += THREADS) edge_word(k);
             }
             gemm::fence_proxy_async_smem();
             bar_compute();
@@ -576,7 +618,7 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
             const int pos = e_pos[j];
             if (pos < 0) continue;
             float p = expf(e_p[j]);
-            if (c.dup) {  // the token's entries in order
+            if (twice) {  // the token's entries in order
               p = 0.f;
               for (int x = 0; x < a.K; ++x)
                 if (e_pos[x] == pos || e_pos[x] == -3 - pos) p += expf(e_p[x]);
@@ -593,8 +635,12 @@ __global__ void __launch_bounds__(THREADS + 32) distill_kernel(Args a) {
       }
       if (!live) {
         if (a.row_loss && rank == 0 && tid == 0) a.row_loss[r] = 0.f;
-        if (grow)
-          for (int i = tid; i < len; i += THREADS) grow[i] = from_f32<DT>(0.f);
+        if (grow) {  // zeros: single elements up to a 16-byte boundary, then whole words
+          const int h0 = min(len, (int)((16u - (reinterpret_cast<uintptr_t>(grow) & 15u)) & 15u) / ES), nw = (len - h0) / N;
+          for (int k = tid; k < nw; k += THREADS) __stcs(reinterpret_cast<uint4*>(grow + h0) + k, make_uint4(0, 0, 0, 0));
+          if (tid < h0) grow[tid] = from_f32<DT>(0.f);
+          if (tid < len - h0 - nw * N) grow[h0 + nw * N + tid] = from_f32<DT>(0.f);
+        }
       }
       if (ahead) {
         if (!under_way) {  // this row's slice is not needed any more
@@ -669,15 +715,16 @@ __global__ void distill_held_kernel(const float* upstream, float* held) { held[0
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-// CTAs per row and elements of a slice: slices of at most 72 KB leave three CTAs on an SM, whose
+// CTAs per row and elements of a slice: slices of about 70 KB leave three CTAs on an SM, whose
 // copies and arithmetic overlap; with few rows the row is cut further, so that every SM has work.
 inline bool plan(int64_t rows, int64_t V, int K, int es, int nsm, int* csize, int* slice, int* smem) {
   auto cut = [&](int c) { return ((V + c - 1) / c + 127) / 128 * 128; };
   const int fixed = ctrl_bytes() + entry_bytes(K) + 32;
+  auto all = [&](int c) { return cut(c) * es + fixed + seen_bytes(cut(c)); };
   int c = 1;
-  while (c < 8 && cut(c) * es > 72 * 1024 - fixed) c *= 2;
+  while (c < 8 && all(c) > 75 * 1024) c *= 2;
   while (c < 8 && rows * c * 2 <= 2 * nsm && cut(2 * c) * es >= 4096) c *= 2;
-  const int64_t bytes = cut(c) * es + fixed;
+  const int64_t bytes = all(c);
   if (bytes > MAX_SMEM) return false;
   *csize = c;
   *slice = (int)cut(c);
