@@ -48,9 +48,14 @@ __device__ __forceinline__ float scale_value(uint32_t S) {
   return S == kScaleNan ? __uint_as_float(0x7FC00000u) : (S == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(S << 23));
 }
 
-// eight values (already divided by the scale) -> one word of codes, v[0] in the lowest nibble
-__device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
+// eight values (already divided by the scale) -> one word of codes, the first in the lowest nibble
+__device__ __forceinline__ uint32_t codes8(f2 p, f2 q, f2 r, f2 t) {
   uint32_t w;
+  float v0, v1, v2, v3, v4, v5, v6, v7;
+  un2(p, v0, v1);
+  un2(q, v2, v3);
+  un2(r, v4, v5);
+  un2(t, v6, v7);
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
@@ -58,8 +63,11 @@ __device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
       "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
       "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(w)
-      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+      : "f"(v0), "f"(v1), "f"(v2), "f"(v3), "f"(v4), "f"(v5), "f"(v6), "f"(v7));
   return w;
+}
+__device__ __forceinline__ uint32_t codes8(const float (&v)[8]) {
+  return codes8(mk2(v[0], v[1]), mk2(v[2], v[3]), mk2(v[4], v[5]), mk2(v[6], v[7]));
 }
 // one byte of codes -> two values
 __device__ __forceinline__ float2 values2(uint32_t byte) {
@@ -76,6 +84,7 @@ struct Pair<FF_DTYPE_BF16> {
   static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
   static __device__ __forceinline__ uint32_t f32_bits(uint32_t h) { return h << 16; }
+  static __device__ __forceinline__ f2 both(uint32_t w) { return unpack_bf16x2(w); }
 };
 template <>
 struct Pair<FF_DTYPE_F16> {
@@ -83,6 +92,10 @@ struct Pair<FF_DTYPE_F16> {
   static __device__ __forceinline__ float hi(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
   static __device__ __forceinline__ uint32_t f32_bits(uint32_t h) {
     return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+  }
+  static __device__ __forceinline__ f2 both(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return mk2(f.x, f.y);
   }
 };
 
@@ -112,14 +125,18 @@ __host__ __device__ constexpr int row_bytes() {
 template <int DT>
 __device__ __forceinline__ void quant_rows(const uint8_t* tile, int64_t row0, int64_t col0, int64_t nblk, int64_t sblk,
                                            const Out& o) {
-  const int lane = threadIdx.x & 31;
+  // the tile's own bases in 64 bits, everything per item in 32
   const int64_t blk0 = col0 / BLOCK;
-  const bool words = (blk0 & 3) == 0 && blk0 + 4 <= sblk;
+  const int b = threadIdx.x & 3, r0 = threadIdx.x >> 2;
+  const int live_rows = (int)min64(TILE, o.rows - row0);
+  const bool put = blk0 + b < nblk, word = (blk0 & 3) == 0 && blk0 + 4 <= sblk, byte = !word && blk0 + b < sblk;
+  const uint32_t ldq = (uint32_t)o.ldq;  // below 2^31: cols are
+  uint8_t* q = o.q_rows + row0 * o.ldq + (blk0 + b) * 16;
+  uint8_t* sc = o.s_rows + scale_at(row0, word ? blk0 : blk0 + b, o.chunks_r);
+  if (live_rows <= 0) return;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int item = threadIdx.x + i * THREADS;
-    const int r = item >> 2, b = item & 3;
-    const int64_t row = row0 + r, blk = blk0 + b;
+    const int r = r0 + i * 64;
     const uint8_t* src = tile + r * row_bytes<DT>();
     uint32_t w[4];
     uint32_t S;
@@ -134,13 +151,13 @@ __device__ __forceinline__ void quant_rows(const uint8_t* tile, int64_t row0, in
 #pragma unroll
       for (int j = 0; j < 32; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7FFFFFFFu);
       S = scale_code(amax);
-      const float inv = inv_scale(S);
+      const f2 inv = splat(inv_scale(S));
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float t[8];
+        f2 t[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = S == kScaleNan ? 0.f : v[8 * k + e] * inv;
-        w[k] = codes8(t);
+        for (int e = 0; e < 4; ++e) t[e] = mul2(mk2(v[8 * k + 2 * e], v[8 * k + 2 * e + 1]), inv);
+        w[k] = codes8(t[0], t[1], t[2], t[3]);
       }
     } else {
       const int swap = b & 2;
@@ -153,35 +170,29 @@ __device__ __forceinline__ void quant_rows(const uint8_t* tile, int64_t row0, in
                                  __vmaxu2(p[j].z & 0x7FFF7FFFu, p[j].w & 0x7FFF7FFFu)));
       }
       S = scale_code(Pair<DT>::f32_bits(max(m & 0xFFFFu, m >> 16)));
-      const float inv = inv_scale(S);
+      const f2 inv = splat(inv_scale(S));
       uint32_t c[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t q[4] = {p[j].x, p[j].y, p[j].z, p[j].w};
-        float t[8];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          t[2 * e] = Pair<DT>::lo(q[e]) * inv;
-          t[2 * e + 1] = Pair<DT>::hi(q[e]) * inv;
-        }
-        c[j] = S == kScaleNan ? 0u : codes8(t);
-      }
+      for (int j = 0; j < 4; ++j)
+        c[j] = codes8(mul2(Pair<DT>::both(p[j].x), inv), mul2(Pair<DT>::both(p[j].y), inv),
+                      mul2(Pair<DT>::both(p[j].z), inv), mul2(Pair<DT>::both(p[j].w), inv));
       w[0] = swap ? c[2] : c[0];
       w[1] = swap ? c[3] : c[1];
       w[2] = swap ? c[0] : c[2];
       w[3] = swap ? c[1] : c[3];
     }
-    if (row < o.rows && blk < nblk)
-      *reinterpret_cast<uint4*>(o.q_rows + row * o.ldq + blk * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-    // scales: the four lanes of a row hold one word of a chunk when the tile starts on a chunk
-    if (words) {
-      const uint32_t s1 = __shfl_down_sync(0xffffffffu, S, 1);
-      const uint32_t s2 = __shfl_down_sync(0xffffffffu, S, 2);
-      const uint32_t s3 = __shfl_down_sync(0xffffffffu, S, 3);
-      if ((lane & 3) == 0 && row0 < o.rows)
-        *reinterpret_cast<uint32_t*>(o.s_rows + scale_at(row, blk, o.chunks_r)) = S | (s1 << 8) | (s2 << 16) | (s3 << 24);
-    } else if (row0 < o.rows && blk < sblk) {
-      o.s_rows[scale_at(row, blk, o.chunks_r)] = (uint8_t)S;
+    if (S == kScaleNan) w[0] = w[1] = w[2] = w[3] = 0u;
+    if (put && r < live_rows)
+      *reinterpret_cast<uint4*>(q + (uint64_t)ldq * (uint32_t)r) = make_uint4(w[0], w[1], w[2], w[3]);
+    // scales (row % 32 at 16 bytes, row / 32 at 4): the four lanes of a row hold one word of a chunk
+    // when the tile starts on a chunk
+    const int at = (r & 31) * 16 + (r >> 5) * 4;
+    if (word) {
+      const uint32_t s1 = S | (__shfl_down_sync(0xffffffffu, S, 1) << 8);
+      const uint32_t s2 = s1 | (__shfl_down_sync(0xffffffffu, s1, 2) << 16);
+      if (b == 0) *reinterpret_cast<uint32_t*>(sc + at) = s2;
+    } else if (byte) {
+      sc[at] = (uint8_t)S;
     }
   }
 }
@@ -196,6 +207,9 @@ __device__ __forceinline__ void quant_cols(const uint8_t* tile, int64_t row0, in
                                            const Out& o, uint8_t* s_buf /* 128 x 4 */, float* sum_buf /* 4 x 128 */) {
   constexpr int W = DT == FF_DTYPE_F32 ? 1 : 2;   // columns of an item
   constexpr int ITEMS = 4 * TILE / W / THREADS;
+  const uint32_t ldqt = (uint32_t)o.ldqt;  // below 2^31: rows are
+  uint8_t* q = o.q_cols + col0 * o.ldqt + row0 / 2;
+  const int live_rb = (int)min64(4, (o.rows - row0 + BLOCK - 1) / BLOCK);  // row blocks that exist
 #pragma unroll 1
   for (int i = 0; i < ITEMS; ++i) {
     const int item = threadIdx.x + i * THREADS;
@@ -216,29 +230,31 @@ __device__ __forceinline__ void quant_cols(const uint8_t* tile, int64_t row0, in
       if constexpr (DT == FF_DTYPE_F32) bits = m;
       else bits = Pair<DT>::f32_bits(h ? m >> 16 : m & 0xFFFFu);
       const uint32_t S = scale_code(bits);
-      const float inv = inv_scale(S);
+      const f2 inv = splat(inv_scale(S));
+      auto value = [&](int i) {
+        if constexpr (DT == FF_DTYPE_F32) return __uint_as_float(x[i]);
+        else return h ? Pair<DT>::hi(x[i]) : Pair<DT>::lo(x[i]);
+      };
       uint32_t w[4];
-      float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        float t[8];
+        f2 t[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float v;
-          if constexpr (DT == FF_DTYPE_F32) v = __uint_as_float(x[8 * k + e]);
-          else v = h ? Pair<DT>::hi(x[8 * k + e]) : Pair<DT>::lo(x[8 * k + e]);
-          sum += v;
-          t[e] = v * inv;
-        }
-        w[k] = S == kScaleNan ? 0u : codes8(t);
+        for (int e = 0; e < 4; ++e) t[e] = mul2(mk2(value(8 * k + 2 * e), value(8 * k + 2 * e + 1)), inv);
+        w[k] = codes8(t[0], t[1], t[2], t[3]);
       }
+      if (S == kScaleNan) w[0] = w[1] = w[2] = w[3] = 0u;
       const int c = wc * W + h;
-      // 16 bytes per 32 rows; row blocks past the matrix are not stored (ldqt covers whole blocks)
-      if (c < live && row0 + rb * BLOCK < o.rows)
-        *reinterpret_cast<uint4*>(o.q_cols + (col0 + c) * o.ldqt + (row0 / 2 + rb * 16)) =
-            make_uint4(w[0], w[1], w[2], w[3]);
+      // 16 bytes per 32 rows (ldqt covers whole blocks)
+      if (c < live && rb < live_rb)
+        *reinterpret_cast<uint4*>(q + (uint64_t)ldqt * (uint32_t)c + rb * 16) = make_uint4(w[0], w[1], w[2], w[3]);
       s_buf[c * 4 + rb] = (uint8_t)S;
-      if (o.colsum) sum_buf[rb * TILE + c] = sum;
+      if (o.colsum) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sum += value(i);
+        sum_buf[rb * TILE + c] = sum;
+      }
     }
   }
   __syncthreads();
@@ -264,29 +280,30 @@ __device__ __forceinline__ void stage_tile(uint8_t* tile, const void* x, int64_t
   constexpr int V = 16 / (int)sizeof(T);
   constexpr int PER_ROW = TILE / V;
   constexpr int N = TILE * PER_ROW / THREADS;
-  const T* p = reinterpret_cast<const T*>(x);
+  // a thread's pieces lie below one another, THREADS / PER_ROW rows apart
+  constexpr int DR = THREADS / PER_ROW;
+  const int64_t c = col0 + (threadIdx.x % PER_ROW) * V, r = row0 + threadIdx.x / PER_ROW;
+  const int live = (int)min64(TILE, rows - r), n = (int)min64(V, max64(0, cols - c));
+  const T* p = reinterpret_cast<const T*>(x) + r * ld + c;
   uint4 v[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int k = threadIdx.x + i * THREADS;
-    const int64_t r = row0 + k / PER_ROW, c = col0 + (k % PER_ROW) * V;
     v[i] = make_uint4(0, 0, 0, 0);
-    if (r < rows && c < cols) {
-      if (vec && c + V <= cols) {
-        v[i] = __ldg(reinterpret_cast<const uint4*>(p + r * ld + c));
+    if (i * DR < live && n > 0) {
+      const T* q = p + (int64_t)(i * DR) * ld;
+      if (vec && n == V) {
+        v[i] = __ldg(reinterpret_cast<const uint4*>(q));
       } else {
         T* e = reinterpret_cast<T*>(&v[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (c + j < cols) e[j] = p[r * ld + c + j];
+          if (j < n) e[j] = q[j];
       }
     }
   }
+  uint8_t* d = tile + (threadIdx.x / PER_ROW) * row_bytes<DT>() + (threadIdx.x % PER_ROW) * 16;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int k = threadIdx.x + i * THREADS;
-    *reinterpret_cast<uint4*>(tile + (k / PER_ROW) * row_bytes<DT>() + (k % PER_ROW) * 16) = v[i];
-  }
+  for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(d + i * DR * row_bytes<DT>()) = v[i];
 }
 
 // both orientations of a tile of the matrix o.rows x o.cols
@@ -307,7 +324,7 @@ __host__ __device__ constexpr int quant_smem() {
 // One 128 x 128 tile per CTA: read once, quantised along either axis or both from shared memory.
 // Bound by HBM: 2 bytes read and 17/32 byte written per value and orientation.
 template <int DT>
-__global__ void __launch_bounds__(THREADS) mx_quant_kernel(const void* x, int64_t ldx, int64_t tiles_c, Out o, int vec) {
+__global__ void __launch_bounds__(THREADS, DT == FF_DTYPE_F32 ? 2 : 4) mx_quant_kernel(const void* x, int64_t ldx, int64_t tiles_c, Out o, int vec) {
   extern __shared__ __align__(16) uint8_t smem[];
   uint8_t* s_buf = smem + TILE * row_bytes<DT>();
   float* sum_buf = reinterpret_cast<float*>(s_buf + TILE * 4);
@@ -317,48 +334,119 @@ __global__ void __launch_bounds__(THREADS) mx_quant_kernel(const void* x, int64_
   quant_tile<DT>(smem, row0, col0, o, s_buf, sum_buf);
 }
 
-// silu and its derivative's parts in fp32: sigmoid from the exponential, exact at both ends
-// (exp(-g) = inf gives 0, and 0 gives 1)
-__device__ __forceinline__ float sigmoid_f32(float g) { return __fdividef(1.f, 1.f + __expf(-g)); }
+// The same for 16-bit inputs whose rows are 16-byte aligned: persistent CTAs, three per SM, each with two
+// tile buffers, so that the next tile arrives (cp.async) while one is quantised.
+// 8192 x 4096 bf16, both orientations: ... us (... us with one tile per CTA).
+template <int DT>
+__host__ __device__ constexpr int pipe_smem() {
+  return 2 * TILE * row_bytes<DT>() + TILE * 4 + 4 * TILE * 4;
+}
+// 16-byte pieces of a tile, zeros outside the matrix
+template <int DT>
+__device__ __forceinline__ void stage_async(uint32_t tile, const void* x, int64_t ld, int64_t rows, int64_t cols, int64_t row0,
+                                            int64_t col0) {
+  static_assert(DT != FF_DTYPE_F32, "16-bit types");
+  // a thread's pieces lie below one another, 16 rows apart
+  const int64_t c = col0 + (threadIdx.x % 16) * 8, r = row0 + threadIdx.x / 16;
+  const int n = (int)min64(16, max64(0, (cols - c) * 2));  // bytes of a piece that exist
+  const int live = (int)min64(TILE, rows - r);              // its rows, counted from the first piece's
+  const uint8_t* src = static_cast<const uint8_t*>(x) + (n ? (r * ld + c) * 2 : 0);
+  const int64_t step = n ? ld * 32 : 0;
+  const uint32_t dst = tile + (threadIdx.x / 16) * row_bytes<DT>() + (threadIdx.x % 16) * 16;
+#pragma unroll
+  for (int i = 0; i < TILE * 16 / THREADS; ++i) {
+    const bool on = i * 16 < live;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + i * 16 * row_bytes<DT>()),
+                 "l"(on ? src + i * step : static_cast<const uint8_t*>(x)), "r"(on ? n : 0)
+                 : "memory");
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int DT>
+__global__ void __launch_bounds__(THREADS, 3) mx_quant_pipe_kernel(const void* x, int64_t ldx, int tiles_c, int tiles, Out o) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  constexpr int TB = TILE * row_bytes<DT>();
+  uint8_t* s_buf = smem + 2 * TB;
+  float* sum_buf = reinterpret_cast<float*>(s_buf + TILE * 4);
+  const uint32_t base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+  int t = blockIdx.x, b = 0;
+  if (t < tiles) stage_async<DT>(base, x, ldx, o.rows, o.cols, (int64_t)(t / tiles_c) * TILE, (int64_t)(t % tiles_c) * TILE);
+  for (; t < tiles; t += gridDim.x, b ^= 1) {
+    const int n = t + gridDim.x;
+    if (n < tiles)
+      stage_async<DT>(base + (b ^ 1) * TB, x, ldx, o.rows, o.cols, (int64_t)(n / tiles_c) * TILE, (int64_t)(n % tiles_c) * TILE);
+    else
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncthreads();
+    quant_tile<DT>(smem + b * TB, (int64_t)(t / tiles_c) * TILE, (int64_t)(t % tiles_c) * TILE, o, s_buf, sum_buf);
+    __syncthreads();  // the buffer is filled again
+  }
+}
+
+// sigmoid(g) = 1 / (1 + 2^(-g log2 e)) in fp32, on the special-function unit (relative error below
+// 2^-20 for the |g| where it is not 0 or 1): exact at both ends (2^.. = inf gives 0, and 0 gives 1)
+__device__ __forceinline__ float ex2_rcp(float t) {
+  float e, s;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+  return s;
+}
+__device__ __forceinline__ float sigmoid_f32(float g) { return ex2_rcp(g * -1.4426950408889634f); }
+__device__ __forceinline__ f2 sigmoid2(f2 g) {
+  float a, b;
+  un2(mul2(g, splat(-1.4426950408889634f)), a, b);
+  return mk2(ex2_rcp(a), ex2_rcp(b));
+}
+
+__device__ __forceinline__ uint32_t swiglu_word(uint32_t wg, uint32_t wu) {
+  const f2 g = unpack_bf16x2(wg);
+  return pack_bf16x2(mul2(mul2(g, sigmoid2(g)), unpack_bf16x2(wu)));
+}
 
 // h = bf16(silu(g) * u) of the bf16 gate/up activations gu = [g | u], quantised like mx_quant_kernel;
 // h itself is not written.
-__global__ void __launch_bounds__(THREADS) mx_swiglu_quant_kernel(const __nv_bfloat16* gu, int64_t ld, int64_t F,
+__global__ void __launch_bounds__(THREADS, 3) mx_swiglu_quant_kernel(const __nv_bfloat16* gu, int64_t ld, int64_t F,
                                                                   int64_t tiles_c, Out o) {
   extern __shared__ __align__(16) uint8_t smem[];
   constexpr int DT = FF_DTYPE_BF16;
   uint8_t* s_buf = smem + TILE * row_bytes<DT>();
   float* sum_buf = reinterpret_cast<float*>(s_buf + TILE * 4);
   const int64_t row0 = (blockIdx.x / tiles_c) * TILE, col0 = (blockIdx.x % tiles_c) * TILE;
+  // a thread's pieces lie below one another, 16 rows apart; F is a multiple of 32: whole pieces
   constexpr int N = TILE * 16 / THREADS;
+  const int64_t c = col0 + (threadIdx.x % 16) * 8, r = row0 + threadIdx.x / 16;
+  const int live = c < F ? (int)min64(TILE, o.rows - r) : 0;
+  const __nv_bfloat16* pg = gu + r * ld + c;
+  uint8_t* d = smem + (threadIdx.x / 16) * row_bytes<DT>() + (threadIdx.x % 16) * 16;
+  uint4 wg[N], wu[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int k = threadIdx.x + i * THREADS;
-    const int64_t r = row0 + k / 16, c = col0 + (k % 16) * 8;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (r < o.rows && c < F) {  // F is a multiple of 32: whole pieces
-      float g[8], u[8];
-      load8<DT>(gu + r * ld + c, g);
-      load8<DT>(gu + r * ld + F + c, u);
-      uint32_t q[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = g[2 * e] * sigmoid_f32(g[2 * e]) * u[2 * e];
-        const float b = g[2 * e + 1] * sigmoid_f32(g[2 * e + 1]) * u[2 * e + 1];
-        q[e] = pack_bf16x2(mk2(a, b));
-      }
-      w = make_uint4(q[0], q[1], q[2], q[3]);
+    wg[i] = wu[i] = make_uint4(0, 0, 0, 0);
+    if (i * 16 < live) {
+      wg[i] = __ldg(reinterpret_cast<const uint4*>(pg + i * 16 * ld));
+      wu[i] = __ldg(reinterpret_cast<const uint4*>(pg + i * 16 * ld + F));
     }
-    *reinterpret_cast<uint4*>(smem + (k / 16) * row_bytes<DT>() + (k % 16) * 16) = w;
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i)  // silu(0) * 0 = 0 outside the matrix
+    *reinterpret_cast<uint4*>(d + i * 16 * row_bytes<DT>()) =
+        make_uint4(swiglu_word(wg[i].x, wu[i].x), swiglu_word(wg[i].y, wu[i].y), swiglu_word(wg[i].z, wu[i].z),
+                   swiglu_word(wg[i].w, wu[i].w));
   __syncthreads();
   quant_tile<DT>(smem, row0, col0, o, s_buf, sum_buf);
+}
+
+__device__ __forceinline__ void swiglu_bwd_word(uint32_t wg, uint32_t wu, uint32_t wd, uint32_t& dg, uint32_t& du) {
+  const f2 g = unpack_bf16x2(wg), d = unpack_bf16x2(wd), s = sigmoid2(g), one = splat(1.f);
+  dg = pack_bf16x2(mul2(mul2(d, unpack_bf16x2(wu)), mul2(s, fma2(g, sub2(one, s), one))));
+  du = pack_bf16x2(mul2(d, mul2(g, s)));
 }
 
 // The gradient of gu from dh and gu (all bf16), quantised as the matrix [dg | du] of 2F columns
 // without being written:  dg = bf16(dh * u * sig(g) * (1 + g * (1 - sig(g)))),  du = bf16(dh * g * sig(g)).
 // One CTA takes the same 128 features of dg and of du.
-__global__ void __launch_bounds__(THREADS) mx_swiglu_bwd_quant_kernel(const __nv_bfloat16* dh, int64_t lddh,
+__global__ void __launch_bounds__(THREADS, 3) mx_swiglu_bwd_quant_kernel(const __nv_bfloat16* dh, int64_t lddh,
                                                                       const __nv_bfloat16* gu, int64_t ld, int64_t F,
                                                                       int64_t tiles_c, Out o) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -367,30 +455,26 @@ __global__ void __launch_bounds__(THREADS) mx_swiglu_bwd_quant_kernel(const __nv
   uint8_t* s_buf = smem + 2 * TB;
   const int64_t row0 = (blockIdx.x / tiles_c) * TILE, col0 = (blockIdx.x % tiles_c) * TILE;
   constexpr int N = TILE * 16 / THREADS;
+  {
+    const int64_t c = col0 + (threadIdx.x % 16) * 8, r = row0 + threadIdx.x / 16;
+    const int live = c < F ? (int)min64(TILE, o.rows - r) : 0;
+    const __nv_bfloat16 *pg = gu + r * ld + c, *pd = dh + r * lddh + c;
+    uint8_t* d = smem + (threadIdx.x / 16) * row_bytes<DT>() + (threadIdx.x % 16) * 16;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int k = threadIdx.x + i * THREADS;
-    const int64_t r = row0 + k / 16, c = col0 + (k % 16) * 8;
-    uint4 wg = make_uint4(0, 0, 0, 0), wu = wg;
-    if (r < o.rows && c < F) {
-      float g[8], u[8], d[8], dg[8], du[8];
-      load8<DT>(gu + r * ld + c, g);
-      load8<DT>(gu + r * ld + F + c, u);
-      load8<DT>(dh + r * lddh + c, d);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float s = sigmoid_f32(g[e]);
-        dg[e] = d[e] * u[e] * (s * (1.f + g[e] * (1.f - s)));
-        du[e] = d[e] * (g[e] * s);
+    for (int i = 0; i < N; ++i) {
+      uint4 vg = make_uint4(0, 0, 0, 0), vu = vg, vd = vg, wg, wu;
+      if (i * 16 < live) {
+        vg = __ldg(reinterpret_cast<const uint4*>(pg + i * 16 * ld));
+        vu = __ldg(reinterpret_cast<const uint4*>(pg + i * 16 * ld + F));
+        vd = __ldg(reinterpret_cast<const uint4*>(pd + i * 16 * lddh));
       }
-      wg = make_uint4(pack_bf16x2(mk2(dg[0], dg[1])), pack_bf16x2(mk2(dg[2], dg[3])), pack_bf16x2(mk2(dg[4], dg[5])),
-                      pack_bf16x2(mk2(dg[6], dg[7])));
-      wu = make_uint4(pack_bf16x2(mk2(du[0], du[1])), pack_bf16x2(mk2(du[2], du[3])), pack_bf16x2(mk2(du[4], du[5])),
-                      pack_bf16x2(mk2(du[6], du[7])));
+      swiglu_bwd_word(vg.x, vu.x, vd.x, wg.x, wu.x);
+      swiglu_bwd_word(vg.y, vu.y, vd.y, wg.y, wu.y);
+      swiglu_bwd_word(vg.z, vu.z, vd.z, wg.z, wu.z);
+      swiglu_bwd_word(vg.w, vu.w, vd.w, wg.w, wu.w);
+      *reinterpret_cast<uint4*>(d + i * 16 * row_bytes<DT>()) = wg;
+      *reinterpret_cast<uint4*>(d + TB + i * 16 * row_bytes<DT>()) = wu;
     }
-    const int at = (k / 16) * row_bytes<DT>() + (k % 16) * 16;
-    *reinterpret_cast<uint4*>(smem + at) = wg;
-    *reinterpret_cast<uint4*>(smem + TB + at) = wu;
   }
   __syncthreads();
   const int live = (int)min64(TILE, F - col0);
@@ -432,40 +516,53 @@ __global__ void __launch_bounds__(256) mx_colsum_kernel(const float* part, int64
   }
 }
 
-// eight values per thread: one word of codes -> 16 (or 32) bytes
+// Eight values per thread and row: one word of codes -> 16 (or 32) bytes.  blockDim.x threads side by side
+// in a row, four rows per thread in flight.
 template <int DT>
-__global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* q, int64_t ldq, const uint8_t* s, int64_t chunks,
-                                                         int64_t rows, int64_t cols, void* out, int64_t ldo, int vec) {
+__global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* q, int64_t ldq, const uint8_t* s, int chunks, int64_t rows,
+                                                         int cols, void* out, int64_t ldo, int vec) {
   using T = typename Elem<DT>::T;
-  const int64_t per_row = (cols + 7) / 8;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= rows * per_row) return;
-  const int64_t r = i / per_row, c = (i - r * per_row) * 8;
-  const uint32_t w = *reinterpret_cast<const uint32_t*>(q + r * ldq + c / 2);
-  const float sv = scale_value(s[scale_at(r, c / BLOCK, chunks)]);
-  float v[8];
+  const int c = ((int)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+  if (c >= cols) return;
+  constexpr int R = 4;
+  for (int64_t r0 = ((int64_t)blockIdx.y * blockDim.y + threadIdx.y) * R; r0 < rows; r0 += (int64_t)gridDim.y * blockDim.y * R) {
+    uint32_t w[R];
+    float sv[R];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float2 p = values2((w >> (8 * k)) & 0xFFu);
-    v[2 * k] = p.x * sv;
-    v[2 * k + 1] = p.y * sv;
-  }
-  T t[8];
+    for (int i = 0; i < R; ++i) {
+      const int64_t r = min64(r0 + i, rows - 1);
+      w[i] = __ldg(reinterpret_cast<const uint32_t*>(q + r * ldq + c / 2));
+      sv[i] = scale_value(__ldg(s + scale_at(r, c / BLOCK, chunks)));
+    }
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if constexpr (DT == FF_DTYPE_F32) t[k] = v[k];
-    else if constexpr (DT == FF_DTYPE_BF16) t[k] = __float2bfloat16_rn(v[k]);
-    else t[k] = __float2half_rn(v[k]);
-  }
-  T* o = reinterpret_cast<T*>(out) + r * ldo + c;
-  if (vec && c + 8 <= cols) {
+    for (int i = 0; i < R; ++i) {
+      if (r0 + i >= rows) break;
+      alignas(16) T t[8];
 #pragma unroll
-    for (int k = 0; k < (int)(8 * sizeof(T) / 16); ++k)
-      reinterpret_cast<uint4*>(o)[k] = reinterpret_cast<const uint4*>(t)[k];
-  } else {
+      for (int k = 0; k < 4; ++k) {
+        const float2 p = values2((w[i] >> (8 * k)) & 0xFFu);
+        const float a = p.x * sv[i], b = p.y * sv[i];
+        if constexpr (DT == FF_DTYPE_F32) {
+          t[2 * k] = a;
+          t[2 * k + 1] = b;
+        } else if constexpr (DT == FF_DTYPE_BF16) {
+          reinterpret_cast<uint32_t*>(t)[k] = pack_bf16x2(mk2(a, b));
+        } else {
+          t[2 * k] = __float2half_rn(a);
+          t[2 * k + 1] = __float2half_rn(b);
+        }
+      }
+      T* o = reinterpret_cast<T*>(out) + (r0 + i) * ldo + c;
+      if (vec && c + 8 <= cols) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (c + k < cols) o[k] = t[k];
+        for (int k = 0; k < (int)(8 * sizeof(T) / 16); ++k)
+          reinterpret_cast<uint4*>(o)[k] = reinterpret_cast<const uint4*>(t)[k];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (c + k < cols) o[k] = t[k];
+      }
+    }
   }
 }
 
@@ -500,12 +597,33 @@ inline int allow_smem(K kernel, int bytes, bool* done, const char* name) {
   return FF_OK;
 }
 
+inline int num_sms() {
+  static int cache[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!cache[dev]) {
+    int n = 0;
+    cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    cache[dev] = n > 0 ? n : 148;
+  }
+  return cache[dev];
+}
+
 template <int DT>
 inline int launch_quant(const void* x, int64_t ldx, int64_t tiles_r, int64_t tiles_c, const Out& o, cudaStream_t st) {
   static bool done[64] = {false};
   int rc = allow_smem(mx_quant_kernel<DT>, quant_smem<DT>(), done, "ff_mxfp4_quant");
   if (rc) return rc;
   const int vec = aligned(x, 16) && (ldx * dtype_size(DT)) % 16 == 0;
+  if constexpr (DT != FF_DTYPE_F32) {
+    if (vec && tiles_r * tiles_c > num_sms()) {  // fewer tiles than SMs: nothing to overlap
+      static bool pdone[64] = {false};
+      if ((rc = allow_smem(mx_quant_pipe_kernel<DT>, pipe_smem<DT>(), pdone, "ff_mxfp4_quant"))) return rc;
+      const int64_t grid = min64(tiles_r * tiles_c, (int64_t)num_sms() * 3);
+      mx_quant_pipe_kernel<DT><<<(unsigned)grid, THREADS, pipe_smem<DT>(), st>>>(x, ldx, (int)tiles_c, (int)(tiles_r * tiles_c), o);
+      return check_launch("ff_mxfp4_quant");
+    }
+  }
   mx_quant_kernel<DT><<<(unsigned)(tiles_r * tiles_c), THREADS, quant_smem<DT>(), st>>>(x, ldx, tiles_c, o, vec);
   return check_launch("ff_mxfp4_quant");
 }
@@ -616,15 +734,19 @@ extern "C" int ff_mxfp4_dequant(const uint8_t* q, int64_t ldq, const uint8_t* s,
   FF_REQUIRE(ldo >= cols, FF_ERR_INVALID_ARG, "ff_mxfp4_dequant: ldo=%lld < cols=%lld", (long long)ldo, (long long)cols);
   if (rows == 0) return FF_OK;
   FF_REQUIRE(q && s && out, FF_ERR_INVALID_ARG, "ff_mxfp4_dequant: null pointer");
-  const int64_t blocks = (rows * ((cols + 7) / 8) + 255) / 256;
-  FF_REQUIRE(blocks < ((int64_t)1 << 31), FF_ERR_UNSUPPORTED, "ff_mxfp4_dequant: too large");
+  const int64_t per_row = (cols + 7) / 8;
+  int bx = 32;
+  while (bx < 256 && bx < per_row) bx *= 2;
+  const int by = 256 / bx;
+  const dim3 block(bx, by), grid((unsigned)((per_row + bx - 1) / bx), (unsigned)ff::min64(65535, (rows + by * 4 - 1) / (by * 4)));
   const int vec = ff::aligned(out, 16) && (ldo * ff::dtype_size(dtype)) % 16 == 0;
   cudaStream_t st = ff::as_stream(stream);
+  const int ch = (int)o.chunks_r, nc = (int)cols;
   if (dtype == FF_DTYPE_F32)
-    mx_dequant_kernel<FF_DTYPE_F32><<<(unsigned)blocks, 256, 0, st>>>(q, ldq, s, o.chunks_r, rows, cols, out, ldo, vec);
+    mx_dequant_kernel<FF_DTYPE_F32><<<grid, block, 0, st>>>(q, ldq, s, ch, rows, nc, out, ldo, vec);
   else if (dtype == FF_DTYPE_BF16)
-    mx_dequant_kernel<FF_DTYPE_BF16><<<(unsigned)blocks, 256, 0, st>>>(q, ldq, s, o.chunks_r, rows, cols, out, ldo, vec);
+    mx_dequant_kernel<FF_DTYPE_BF16><<<grid, block, 0, st>>>(q, ldq, s, ch, rows, nc, out, ldo, vec);
   else
-    mx_dequant_kernel<FF_DTYPE_F16><<<(unsigned)blocks, 256, 0, st>>>(q, ldq, s, o.chunks_r, rows, cols, out, ldo, vec);
+    mx_dequant_kernel<FF_DTYPE_F16><<<grid, block, 0, st>>>(q, ldq, s, ch, rows, nc, out, ldo, vec);
   return ff::check_launch("ff_mxfp4_dequant");
 }
