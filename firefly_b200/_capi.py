@@ -83,6 +83,11 @@ SIGNATURES = {
     "ff_mxfp4_swiglu_bwd_quant": (_I, [_P, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P, _P]),
     "ff_mxfp4_gemm": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P]),
     "ff_mxfp4_swiglu_gemm": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P]),
+    "ff_mxfp4_linear_ws_bytes": (_I64, [_I64, _I64]),
+    "ff_mxfp4_swiglu_mlp_ws_bytes": (_I64, [_I64, _I64, _I64]),
+    "ff_mxfp4_linear": (_I, [_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P]),
+    "ff_mxfp4_swiglu_mlp": (_I, [_P, _I, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64, _I64, _P,
+                                 _I64, _P]),
     "ff_distill_loss": (_I, [_P, _I, _P, _P, _P, _I64, _P, _P, _P]),
     "ff_distill_grad": (_I, [_P, _I, _P, _P, _I, _P, _P, _I64, _P]),
     "ff_ipc_alloc": (_I, [_I64, ctypes.POINTER(ctypes.c_void_p)]),
@@ -134,7 +139,7 @@ _KERNELS_PER_CALL = {"ff_quant_rows_i8": 1, "ff_quant_dual_i8": 2, "ff_quant_dua
                      "ff_adamw8_blockwise": 1,
                      "ff_mxfp4_quant": 1, "ff_mxfp4_dequant": 1, "ff_mxfp4_swiglu_quant": 1,
                      "ff_mxfp4_swiglu_bwd_quant": 1, "ff_mxfp4_gemm": 1, "ff_mxfp4_swiglu_gemm": 1,
-                     "ff_distill_loss": 3, "ff_distill_grad": 1,
+                     "ff_distill_loss": 3, "ff_distill_grad": 1, "ff_mxfp4_linear": 2, "ff_mxfp4_swiglu_mlp": 3,
                      "ff_adamw32_multi": 1}
 
 
@@ -181,6 +186,22 @@ def _ptr(t: torch.Tensor | None):
 
 def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+class _OnDevice:
+    """``torch.cuda.device(dev)`` that costs nothing when ``dev`` is the current device."""
+    __slots__ = ("guard",)
+
+    def __init__(self, dev: torch.device):
+        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
@@ -787,7 +808,7 @@ def mxfp4_quant(x: torch.Tensor, rows: bool = True, cols: bool = False, colsum: 
     if colsum:
         sums = torch.empty((C,), dtype=torch.float32, device=dev)
         ws = torch.empty(((R + 127) // 128 * C,), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_mxfp4_quant", _ptr(x), _dtype_code(x.dtype), R, C, ldx, _ptr(q), (C + 31) // 32 * 16, _ptr(s),
               _ptr(qt), (R + 31) // 32 * 16, _ptr(st), _ptr(sums), _ptr(ws), _stream(dev))
     return (None if q is None else (q, s)), (None if qt is None else (qt, st)), sums
@@ -796,7 +817,7 @@ def mxfp4_quant(x: torch.Tensor, rows: bool = True, cols: bool = False, colsum: 
 def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: int, dtype: torch.dtype) -> torch.Tensor:
     dev = _require_cuda(codes, scales)
     out = torch.empty((rows, cols), dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_mxfp4_dequant", _ptr(codes), codes.stride(0) if rows > 1 else codes.shape[1], _ptr(scales), rows, cols,
               _ptr(out), _dtype_code(dtype), cols, _stream(dev))
     return out
@@ -809,7 +830,7 @@ def mxfp4_gemm(a, b, M: int, N: int, K: int, bias: torch.Tensor | None = None,
     if out_dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"MXFP4 product: output dtype {out_dtype} (bfloat16 or float32)")
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_mxfp4_gemm", _ptr(a[0]), a[0].shape[1], _ptr(a[1]), _ptr(b[0]), b[0].shape[1], _ptr(b[1]), _ptr(bias),
               _ptr(out), N, FF_OUT_F32 if out_dtype == torch.float32 else FF_OUT_BF16, M, N, K, _stream(dev))
     return out
@@ -819,7 +840,7 @@ def mxfp4_swiglu_gemm(a, b, M: int, F: int, K: int) -> tuple[torch.Tensor, torch
     """``(codes, scales)`` of h = silu(g)·u, [g | u] = A·Bᵀ, B the 2F gate and up rows (F % 128 == 0)."""
     dev = _require_cuda(a[0], a[1], b[0], b[1])
     hq, hs = _mx_alloc(M, F, dev)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_mxfp4_swiglu_gemm", _ptr(a[0]), a[0].shape[1], _ptr(a[1]), _ptr(b[0]), b[0].shape[1], _ptr(b[1]),
               _ptr(hq), hq.shape[1], _ptr(hs), M, F, K, _stream(dev))
     return hq, hs
@@ -832,7 +853,7 @@ def mxfp4_swiglu_quant(gu: torch.Tensor, cols: bool = False):
     T = gu.shape[0]
     q, s = _mx_alloc(T, F, dev)
     qt, st = _mx_alloc(F, T, dev) if cols else (None, None)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_mxfp4_swiglu_quant", _ptr(gu), ld, T, F, _ptr(q), q.shape[1], _ptr(s), _ptr(qt), (T + 31) // 32 * 16,
               _ptr(st), _stream(dev))
     return (q, s), (qt, st) if cols else None
@@ -848,10 +869,40 @@ def mxfp4_swiglu_bwd_quant(dh: torch.Tensor, gu: torch.Tensor, rows: bool = True
     T = gu.shape[0]
     q, s = _mx_alloc(T, 2 * F, dev) if rows else (None, None)
     qt, st = _mx_alloc(2 * F, T, dev) if cols else (None, None)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_mxfp4_swiglu_bwd_quant", _ptr(dh), lddh, _ptr(gu), ld, T, F, _ptr(q), (2 * F + 31) // 32 * 16, _ptr(s),
               _ptr(qt), (T + 31) // 32 * 16, _ptr(st), _stream(dev))
     return (q, s) if rows else None, (qt, st) if cols else None
+
+
+def mxfp4_linear(x: torch.Tensor, w, N: int, K: int, bias: torch.Tensor | None) -> torch.Tensor:
+    """bf16 ``x·Wᵀ (+ bias)`` of a matrix and ``(codes, scales)`` of a weight [N, K], in one call."""
+    x, ldx = _mx_float(x)
+    dev = x.device
+    M = x.shape[0]
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    nbytes = (M * ((K + 31) // 32 * 16) + 1023) // 1024 * 1024 + (M + 127) // 128 * ((K + 255) // 256) * 1024
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)  # ff_mxfp4_linear_ws_bytes(M, K)
+    with _OnDevice(dev):
+        _call("ff_mxfp4_linear", x.data_ptr(), _dtype_code(x.dtype), ldx, w[0].data_ptr(), w[0].shape[1], w[1].data_ptr(),
+              None if bias is None else bias.data_ptr(), out.data_ptr(), N, FF_OUT_BF16, M, N, K, ws.data_ptr(), nbytes,
+              _stream(dev))
+    return out
+
+
+def mxfp4_swiglu_mlp(x: torch.Tensor, gu, w, F: int, N: int) -> torch.Tensor:
+    """bf16 ``down(silu(g)·u)``, ``[g | u] = x·GUᵀ``, both weights ``(codes, scales)``, in one call (F % 128 == 0)."""
+    x, ldx = _mx_float(x)
+    dev = x.device
+    M, K = x.shape
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    nbytes = lib().ff_mxfp4_swiglu_mlp_ws_bytes(M, K, F)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    with _OnDevice(dev):
+        _call("ff_mxfp4_swiglu_mlp", x.data_ptr(), _dtype_code(x.dtype), ldx, gu[0].data_ptr(), gu[0].shape[1],
+              gu[1].data_ptr(), w[0].data_ptr(), w[0].shape[1], w[1].data_ptr(), out.data_ptr(), N, FF_OUT_BF16, M, K, F, N,
+              ws.data_ptr(), nbytes, _stream(dev))
+    return out
 
 
 # ---------------------------------------------------------------------------
@@ -881,7 +932,7 @@ def distill_loss(rows: DistillRows, logits: torch.Tensor, reduction: str, grad: 
         if grad:
             g = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev)
             held = torch.empty((1,), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_distill_loss", ctypes.byref(rows), FF_REDUCE[reduction], _ptr(row), _ptr(loss), _ptr(g),
               logits.shape[1], _ptr(held), _ptr(counts), _stream(dev))
     return row, loss, g, held, counts
@@ -895,7 +946,7 @@ def distill_grad(rows: DistillRows, logits: torch.Tensor, reduction: str, upstre
     dev = logits.device
     if grad is None:
         grad, held = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev), None
-    with torch.cuda.device(dev):
+    with _OnDevice(dev):
         _call("ff_distill_grad", ctypes.byref(rows), FF_REDUCE[reduction], _ptr(upstream), _ptr(held), int(keep_held),
               _ptr(counts), _ptr(grad), logits.shape[1], _stream(dev))
     return grad

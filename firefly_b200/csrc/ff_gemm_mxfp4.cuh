@@ -100,30 +100,63 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows of A.  One work item is 128 rows of B (NW = 2: 128 gate rows and the same 128 up rows)
-// against MP rows of A; the CTAs of a cluster take equal runs of its k-blocks.  Their fp32 partial
-// sums meet in shared memory: each warp of the cluster adds its (row of A, 32 columns) pieces over
-// the CTAs in rank order, so the result does not depend on timing and no workspace is needed.
+// Few rows of A: a stream over B.  One work item is 128 rows of B (NW = 2: 128 gate rows and the same
+// 128 up rows) against MP rows of A; the CTAs of a cluster take equal runs of its k-blocks.  Persistent
+// clusters, one CTA per SM: the loads run on from item to item.  The fp32 partial sums meet in shared
+// memory: each warp of the cluster adds its (row of A, 32 columns) pieces over the CTAs in rank order,
+// so the result does not depend on timing and no workspace is needed.  Two barriers per CTA order the
+// exchange: `pfull` (every CTA's partial sums are written) and `pfree` (every CTA has read them).
 // ---------------------------------------------------------------------------
 __host__ __device__ constexpr int nr_stage_bytes(int mp, int nw) { return nw * (ROWS_BYTES + SF_BYTES) + mp * 128 + SF_BYTES; }
-// two CTAs per SM where a stage is small, else one
+__host__ __device__ constexpr int nr_part_bytes(int mp, int nw) { return nw * mp * 128 * 4; }
 __host__ __device__ constexpr int nr_stages(int mp, int nw) {
-  return (nw == 1 && mp <= 32 ? 105 * 1024 : 208 * 1024) / nr_stage_bytes(mp, nw) > 8
-             ? 8
-             : (nw == 1 && mp <= 32 ? 105 * 1024 : 208 * 1024) / nr_stage_bytes(mp, nw);
+  return (224 * 1024 - nr_part_bytes(mp, nw)) / nr_stage_bytes(mp, nw) > 10
+             ? 10
+             : (224 * 1024 - nr_part_bytes(mp, nw)) / nr_stage_bytes(mp, nw);
 }
-__host__ __device__ constexpr int nr_smem(int mp, int nw) { return nr_stages(mp, nw) * nr_stage_bytes(mp, nw) + 1024 + 256; }
+__host__ __device__ constexpr int nr_smem(int mp, int nw) {
+  return nr_stages(mp, nw) * nr_stage_bytes(mp, nw) + nr_part_bytes(mp, nw) + 1024 + 256;
+}
 __host__ __device__ constexpr int pow2_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512; }
-__host__ __device__ constexpr int nr_tmem(int mp, int nw) { return pow2_cols(nw * mp + nr_stages(mp, nw) * (nw + 1) * 8); }
+__host__ __device__ constexpr int nr_tmem(int mp, int nw) { return pow2_cols(2 * nw * mp + nr_stages(mp, nw) * (nw + 1) * 8); }
+
+// wait for a barrier on which other CTAs of the cluster arrive
+__device__ __forceinline__ bool wait_bar_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  auto ready = [&]() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+  };
+  if (ready()) return true;
+  const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns();
+  while (true) {
+    if (ready()) return true;
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - t0 > limit) {
+      *abort_flag = 1;
+      raise_status(FF_DEVICE_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+using mx::let_next_kernel_start;
+using mx::wait_for_previous_kernel;
 
 template <int MP, int NW>
-__global__ void __launch_bounds__(NUM_THREADS)
+__global__ void __launch_bounds__(NUM_THREADS, 1)
     mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW,
                           const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmSX, int num_kb,
-                          Epi ep) {
+                          int tiles_w, int tiles_x, Epi ep) {
   constexpr int ST = nr_stages(MP, NW), SB = nr_stage_bytes(MP, NW), TC = nr_tmem(MP, NW);
-  static_assert(ST >= 2 && ST * SB >= NW * MP * 128 * 4, "the partial sums reuse the stages");
-  static_assert(NW * MP + ST * (NW + 1) * 8 <= 512, "TMEM columns");
+  static_assert(ST >= 2 && nr_smem(MP, NW) <= 232448, "shared memory");
+  static_assert(2 * NW * MP + ST * (NW + 1) * 8 <= 512, "TMEM columns");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t pad = (1024u - (raw & 1023u)) & 1023u;
@@ -134,25 +167,36 @@ __global__ void __launch_bounds__(NUM_THREADS)
   auto sX = [&](int s) { return sbase + s * SB + NW * ROWS_BYTES; };
   auto sSW = [&](int s, int w) { return sX(s) + MP * 128 + w * SF_BYTES; };
   auto sSX = [&](int s) { return sX(s) + MP * 128 + NW * SF_BYTES; };
-  uint8_t* ctrl = smem + ST * SB;
-  const uint32_t cbase = sbase + ST * SB;
+  float* part = reinterpret_cast<float*>(smem + ST * SB);  // [w][row of A][128]
+  const uint32_t part_addr = sbase + ST * SB;
+  uint8_t* ctrl = smem + ST * SB + nr_part_bytes(MP, NW);
+  const uint32_t cbase = part_addr + nr_part_bytes(MP, NW);
   auto full_bar = [&](int s) { return cbase + 8u * s; };
   auto empty_bar = [&](int s) { return cbase + 8u * (ST + s); };
-  const uint32_t tfull = cbase + 8u * (2 * ST);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (2 * ST + 1));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * ST + 1) + 4);
+  auto tfull_bar = [&](int a) { return cbase + 8u * (2 * ST + a); };
+  auto tempty_bar = [&](int a) { return cbase + 8u * (2 * ST + 2 + a); };
+  const uint32_t pfull = cbase + 8u * (2 * ST + 4), pfree = pfull + 8u, drain = pfull + 16u;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (2 * ST + 7));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * ST + 7) + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)blockIdx.x, csize = (int)gridDim.x;  // the cluster spans grid x
   const int kb0 = (int)((int64_t)num_kb * rank / csize), kb1 = (int)((int64_t)num_kb * (rank + 1) / csize);
-  const int tw = (int)blockIdx.y, tx = (int)blockIdx.z;
+  const int items = tiles_w * tiles_x, first = (int)blockIdx.y, stride = (int)gridDim.y;
+  const bool direct = NW == 1 && csize == 1;  // no exchange
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
     }
-    mbar_init(tfull, 1);
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(tfull_bar(a), 1);
+      mbar_init(tempty_bar(a), 4);
+    }
+    mbar_init(pfull, 4 * csize);
+    mbar_init(pfree, 4 * csize);
+    mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     tma_prefetch_desc(&tmW);
@@ -166,30 +210,57 @@ __global__ void __launch_bounds__(NUM_THREADS)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
+  if (csize > 1) cluster_sync_all();  // every CTA's barriers are there
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  bool live = true;  // epilogue warps: the accumulator was complete
+  let_next_kernel_start();  // after the TMEM allocation: the next kernel's CTAs may allocate theirs now
 
   if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
-      int s = 0;
-      uint32_t phase = 0, used = 0, last = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!wait_bar(empty_bar(s), phase ^ 1u, abort_flag)) break;
-        mbar_arrive_expect_tx(full_bar(s), SB);
+      auto load_w = [&](int s, int it, int kb) {
+        const int tw = it / tiles_x;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
           tma_load_2d(sW(s, w), &tmW, kb * 128, (int)(w * ep.F) + tw * 128, full_bar(s));
           tma_load_2d(sSW(s, w), &tmSW, kb * 256, (int)(w * (ep.F / 128)) + tw, full_bar(s));
         }
+      };
+      auto load_x = [&](int s, int it, int kb) {
+        const int tx = it % tiles_x;
         tma_load_2d(sX(s), &tmX, kb * 128, tx * MP, full_bar(s));
-        tma_load_2d(sSX(s), &tmSX, kb * 256, tx, full_bar(s));
-        used |= 1u << s;
-        last = (last & ~(1u << s)) | (phase << s);
-        if (++s == ST) {
-          s = 0;
-          phase ^= 1u;
+        tma_load_2d(sSX(s), &tmSX, kb * 256, tx * MP / 128, full_bar(s));
+      };
+      // the weights of the first stages are asked for before A (the last kernel's output) is waited for
+      int ahead = 0;
+      if (first < items) {
+        for (; ahead < ST && ahead < kb1 - kb0; ++ahead) {
+          mbar_arrive_expect_tx(full_bar(ahead), SB);
+          load_w(ahead, first, kb0 + ahead);
+        }
+      }
+      wait_for_previous_kernel();
+      int s = 0, n = 0;
+      uint32_t phase = 0, used = 0, last = 0;
+      bool ok = true;
+      for (int it = first; ok && it < items; it += stride) {
+        for (int kb = kb0; kb < kb1; ++kb, ++n) {
+          if (n >= ahead) {
+            if (!wait_bar(empty_bar(s), phase ^ 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            mbar_arrive_expect_tx(full_bar(s), SB);
+            load_w(s, it, kb);
+          }
+          load_x(s, it, kb);
+          used |= 1u << s;
+          last = (last & ~(1u << s)) | (phase << s);
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1u;
+          }
         }
       }
       for (int k = 0; k < ST; ++k)
@@ -197,52 +268,73 @@ __global__ void __launch_bounds__(NUM_THREADS)
     }
     __syncwarp();
   } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_mx(128, MP);
-      int s = 0;
-      uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!wait_bar(full_bar(s), phase, abort_flag)) break;
+      int s = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int it = first; ok && it < items; it += stride) {
+        if (!wait_bar(tempty_bar(acc), acc_phase ^ 1u, abort_flag)) break;
         tc_fence_after();
-        // this stage's scales: 8 columns per operand, slots as many as stages
-        const uint32_t sf = tmem + (uint32_t)(NW * MP + s * (NW + 1) * 8);
+        const uint32_t d = tmem + (uint32_t)(acc * NW * MP);
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!wait_bar(full_bar(s), phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          // this stage's scales: 8 columns per operand, slots as many as stages.  A's chunks cover 128 rows,
+          // 32 to a column: the second half of them belongs to an odd tile of 64.
+          const uint32_t sf = tmem + (uint32_t)(2 * NW * MP + s * (NW + 1) * 8);
+          const uint32_t sfx = sf + NW * 8 + (uint32_t)(it % tiles_x * MP % 128 / 32);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+          for (int c = 0; c < 2; ++c) {
 #pragma unroll
-          for (int w = 0; w < NW; ++w) sf_copy<1>(sf + w * 8 + c * 4, sSW(s, w) + c * 512);
-          sf_copy<1>(sf + NW * 8 + c * 4, sSX(s) + c * 512);
+            for (int w = 0; w < NW; ++w) sf_copy<1>(sf + w * 8 + c * 4, sSW(s, w) + c * 512);
+            sf_copy<1>(sf + NW * 8 + c * 4, sSX(s) + c * 512);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int w = 0; w < NW; ++w)
+              mma_mx<1>(d + w * MP, smem_desc_k_sw128(sW(s, w) + k * 32), smem_desc_k_sw128(sX(s) + k * 32),
+                        idesc | idesc_sf((k & 1) * 2), sf + w * 8 + (k >> 1) * 4, sfx + (k >> 1) * 4,
+                        (kb != kb0 || k != 0) ? 1u : 0u);
+          }
+          tc_commit(empty_bar(s));
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1u;
+          }
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-#pragma unroll
-          for (int w = 0; w < NW; ++w)
-            mma_mx<1>(tmem + w * MP, smem_desc_k_sw128(sW(s, w) + k * 32), smem_desc_k_sw128(sX(s) + k * 32),
-                      idesc | idesc_sf((k & 1) * 2), sf + w * 8 + (k >> 1) * 4, sf + NW * 8 + (k >> 1) * 4,
-                      (kb != kb0 || k != 0) ? 1u : 0u);
-        }
-        tc_commit(empty_bar(s));
-        if (++s == ST) {
-          s = 0;
-          phase ^= 1u;
+        if (!ok) break;
+        tc_commit(tfull_bar(acc));
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
         }
       }
-      tc_commit(tfull);
-      drain_bar(tfull, 0);
+      tc_commit(drain);
+      drain_bar(drain, 0);
     }
     __syncwarp();
   } else {
+    // ------------------------------------------------------------ epilogue
     const int lg = warp & 3;
-    live = __all_sync(0xffffffffu, wait_bar(tfull, 0, abort_flag)) && !*abort_flag;
-    tc_fence_after();
-    if (live) {
-      const uint32_t tb = tmem + ((uint32_t)(lg * 32) << 16);
+    int acc = 0;
+    uint32_t acc_phase = 0, xphase = 0;
+    for (int it = first; it < items; it += stride) {
+      const int tw = it / tiles_x, tx = it % tiles_x;
       const int jn = (int)min64(MP, ep.M - (int64_t)tx * MP);
-      if (NW == 1 && csize == 1) {
+      if (!__all_sync(0xffffffffu, wait_bar(tfull_bar(acc), acc_phase, abort_flag))) break;
+      tc_fence_after();
+      const uint32_t tb = tmem + ((uint32_t)(lg * 32) << 16) + (uint32_t)(acc * NW * MP);
+      if (direct) {
         const int64_t n = (int64_t)tw * 128 + lg * 32 + lane;
         const float b = ep.bias && n < ep.N ? __ldg(ep.bias + n) : 0.f;
 #pragma unroll 1
-        for (int c = 0; c < MP; c += 16) {
-          if (c >= jn) break;
+        for (int c = 0; c < jn; c += 16) {
           uint32_t r[16];
           tmem_ld16(tb + c, r);
           tmem_wait_ld();
@@ -256,9 +348,12 @@ __global__ void __launch_bounds__(NUM_THREADS)
             }
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty_bar(acc));
       } else {
-        // partial sums [w][row of A][128] over the stages' memory (every load has landed and been read)
-        float* part = reinterpret_cast<float*>(smem);
+        // the partial sums of the last item have been read everywhere
+        if (!__all_sync(0xffffffffu, wait_bar_cluster(pfree, xphase ^ 1u, abort_flag))) break;
 #pragma unroll 1
         for (int c = 0; c < NW * MP; c += 16) {
           if (c % MP >= jn) continue;
@@ -268,58 +363,63 @@ __global__ void __launch_bounds__(NUM_THREADS)
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(c + j) * 128 + lg * 32 + lane] = __uint_as_float(r[j]);
         }
-      }
-    }
-  }
-
-  if (NW == 2 || csize > 1) {
-    cluster_sync_all();
-    if (warp >= 2 && live) {
-      const int jn = (int)min64(MP, ep.M - (int64_t)tx * MP);
-      const int total = jn * 4;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty_bar(acc));
+        if (lane < csize) mbar_arrive_remote(mapa_shared(pfull, (uint32_t)lane));
+        if (!__all_sync(0xffffffffu, wait_bar_cluster(pfull, xphase, abort_flag))) break;
 #pragma unroll 1
-      for (int it = rank * 4 + (warp - 2); it < total; it += csize * 4) {
-        const int j = it >> 2, lq = it & 3;
-        const uint32_t at = sbase + (uint32_t)((j * 128 + lq * 32 + lane) * 4);
-        float v = 0.f, u = 0.f;
+        for (int p = rank * 4 + (warp - 2); p < jn * 4; p += csize * 4) {
+          const int j = p >> 2, lq = p & 3;
+          const uint32_t at = part_addr + (uint32_t)((j * 128 + lq * 32 + lane) * 4);
+          float v = 0.f, u = 0.f;
 #pragma unroll 4
-        for (int r = 0; r < csize; ++r) {
-          const uint32_t a = mapa_shared(at, (uint32_t)r);
-          v += ld_cluster_f32(a);
-          if constexpr (NW == 2) u += ld_cluster_f32(a + MP * 128 * 4);
-        }
-        const int64_t m = (int64_t)tx * MP + j;
-        if constexpr (NW == 1) {
-          const int64_t n = (int64_t)tw * 128 + lq * 32 + lane;
-          if (n < ep.N) {
-            if (ep.bias) v += __ldg(ep.bias + n);
-            if (ep.out_f32) static_cast<float*>(ep.D)[m * ep.ldd + n] = v;
-            else static_cast<__nv_bfloat16*>(ep.D)[m * ep.ldd + n] = __float2bfloat16_rn(v);
+          for (int r = 0; r < csize; ++r) {
+            const uint32_t a = mapa_shared(at, (uint32_t)r);
+            v += ld_cluster_f32(a);
+            if constexpr (NW == 2) u += ld_cluster_f32(a + MP * 128 * 4);
           }
-        } else {
-          // one block of h: 32 features, a lane each
-          const float h = swiglu_h(v, u);
-          const uint32_t S = mx::scale_code(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7FFFFFFFu));
-          const float t[8] = {h * mx::inv_scale(S), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          uint32_t w = S == mx::kScaleNan ? 0u : (mx::codes8(t) & 0xFu) << (4 * (lane & 7));
-          w |= __shfl_xor_sync(0xffffffffu, w, 1);
-          w |= __shfl_xor_sync(0xffffffffu, w, 2);
-          w |= __shfl_xor_sync(0xffffffffu, w, 4);
-          const int64_t blk = (int64_t)tw * 4 + lq;
-          if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(ep.hq + m * ep.ldh + blk * 16 + (lane >> 3) * 4) = w;
-          if (lane == 0) ep.hs[mx::scale_at(m, blk, ep.hchunks)] = (uint8_t)S;
+          const int64_t m = (int64_t)tx * MP + j;
+          if constexpr (NW == 1) {
+            const int64_t n = (int64_t)tw * 128 + lq * 32 + lane;
+            if (n < ep.N) {
+              if (ep.bias) v += __ldg(ep.bias + n);
+              if (ep.out_f32) static_cast<float*>(ep.D)[m * ep.ldd + n] = v;
+              else static_cast<__nv_bfloat16*>(ep.D)[m * ep.ldd + n] = __float2bfloat16_rn(v);
+            }
+          } else {
+            // one block of h: 32 features, a lane each
+            const float h = swiglu_h(v, u);
+            const uint32_t S = mx::scale_code(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7FFFFFFFu));
+            const float t[8] = {h * mx::inv_scale(S), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            uint32_t w = S == mx::kScaleNan ? 0u : (mx::codes8(t) & 0xFu) << (4 * (lane & 7));
+            w |= __shfl_xor_sync(0xffffffffu, w, 1);
+            w |= __shfl_xor_sync(0xffffffffu, w, 2);
+            w |= __shfl_xor_sync(0xffffffffu, w, 4);
+            const int64_t blk = (int64_t)tw * 4 + lq;
+            if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(ep.hq + m * ep.ldh + blk * 16 + (lane >> 3) * 4) = w;
+            if (lane == 0) ep.hs[mx::scale_at(m, blk, ep.hchunks)] = (uint8_t)S;
+          }
         }
+        if constexpr (NW == 2) {  // the padding chunk of h's scales
+          if (rank == 0 && tw == tiles_w - 1 && tx % (128 / MP) == 0 && ep.hchunks * 128 > ep.F)
+            reinterpret_cast<uint32_t*>(ep.hs)[((int64_t)(tx * MP / 128) * ep.hchunks + ep.F / 128) * 128 + (threadIdx.x - 64)] = 0;
+        }
+        __syncwarp();
+        if (lane < csize) mbar_arrive_remote(mapa_shared(pfree, (uint32_t)lane));
+        xphase ^= 1u;
       }
-      if constexpr (NW == 2) {  // the padding chunk of h's scales
-        if (rank == 0 && tw == (int)gridDim.y - 1 && tx % (128 / MP) == 0 && ep.hchunks * 128 > ep.F)
-          reinterpret_cast<uint32_t*>(ep.hs)[((int64_t)(tx * MP / 128) * ep.hchunks + ep.F / 128) * 128 + (threadIdx.x - 64)] = 0;
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
       }
     }
-    cluster_sync_all();  // no CTA leaves while another reads its partial sums
+    __syncwarp();
   }
 
   tc_fence_before();
-  __syncthreads();
+  if (csize > 1) cluster_sync_all();  // no CTA leaves while another reads its partial sums or arrives on its barriers
+  else __syncthreads();
   tc_fence_after();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TC) : "memory");
@@ -446,10 +546,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  let_next_kernel_start();  // after the TMEM allocation: the next kernel's CTAs may allocate theirs now
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
+      wait_for_previous_kernel();
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -657,8 +759,47 @@ struct Operand {
   const uint8_t* s;
 };
 
+// attributes of a cluster launch; `early`: the kernel may start before the one ahead of it on the stream
+// has finished (it waits for it where it reads that kernel's output)
+struct LaunchAttrs {
+  cudaLaunchAttribute a[2];
+  LaunchAttrs(cudaLaunchConfig_t& cfg, int cluster, bool early) {
+    a[0].id = cudaLaunchAttributeClusterDimension;
+    a[0].val.clusterDim.x = (unsigned)cluster;
+    a[0].val.clusterDim.y = 1;
+    a[0].val.clusterDim.z = 1;
+    a[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = a;
+    cfg.numAttrs = early ? 2 : 1;
+  }
+};
+
+// clusters of `csize` CTAs (one per SM) that run at once, cached per device
 template <int MP, int NW>
-inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int csize, int64_t brows,
+inline int narrow_clusters(int csize) {
+  static int cache[64][4] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms_current() / csize / 2 + 1;
+  const int lc = csize == 1 ? 0 : csize == 2 ? 1 : csize == 4 ? 2 : 3;
+  if (!cache[dev][lc]) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)csize);
+    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.dynamicSmemBytes = nr_smem(MP, NW);
+    LaunchAttrs at(cfg, csize, false);
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, mx_gemm_narrow_kernel<MP, NW>, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 1;
+    }
+    cache[dev][lc] = n;
+  }
+  return cache[dev][lc];
+}
+
+template <int MP, int NW>
+inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, bool early,
                          cudaStream_t st) {
   static bool done[64] = {false};
   int rc = mx::allow_smem(mx_gemm_narrow_kernel<MP, NW>, nr_smem(MP, NW), done, "ff_mxfp4_gemm");
@@ -668,26 +809,36 @@ inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Ep
   if ((rc = make_map_sf(&tsw, b.s, brows, K))) return rc;
   if ((rc = make_map_codes(&tx, a.q, ep.M, K, a.ld, MP))) return rc;
   if ((rc = make_map_sf(&tsx, a.s, ep.M, K))) return rc;
-  const int64_t tiles_w = ((NW == 2 ? ep.F : ep.N) + 127) / 128, tiles_x = (ep.M + MP - 1) / MP;
+  const int64_t tiles_w = ((NW == 2 ? ep.F : ep.N) + 127) / 128, tiles_x = (ep.M + MP - 1) / MP, items = tiles_w * tiles_x;
+  FF_REQUIRE(items < ((int64_t)1 << 31), FF_ERR_UNSUPPORTED, "ff_mxfp4_gemm: too many tiles");
+  const int64_t num_kb = (K + KB - 1) / KB;
+  // The cluster size whose busiest CTA has the least to do: its turns times the k-blocks of a turn, plus
+  // about two k-blocks' time for the exchange of a turn where K is split.
+  int csize = 1, clusters = 1;
+  int64_t best = INT64_MAX;
+  for (int c = 1; c <= 8 && c <= num_kb; c *= 2) {
+    const int n = narrow_clusters<MP, NW>(c);
+    const int64_t turns = (items + n - 1) / n, cost = turns * ((num_kb + c - 1) / c + (c > 1 ? 2 : 0));
+    if (cost < best) {
+      best = cost;
+      csize = c;
+      clusters = (int)min64(items, n);
+    }
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)csize, (unsigned)tiles_w, (unsigned)tiles_x);
+  cfg.gridDim = dim3((unsigned)csize, (unsigned)clusters);
   cfg.blockDim = dim3(NUM_THREADS);
   cfg.dynamicSmemBytes = nr_smem(MP, NW);
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)csize;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_narrow_kernel<MP, NW>, tw, tsw, tx, tsx, (int)((K + KB - 1) / KB), ep),
+  LaunchAttrs at(cfg, csize, early);
+  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_narrow_kernel<MP, NW>, tw, tsw, tx, tsx, (int)num_kb, (int)tiles_w, (int)tiles_x, ep),
               "ff_mxfp4_gemm launch");
   return check_launch("ff_mxfp4_gemm");
 }
 
 template <bool GATED>
-inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, int64_t brows, int max_pairs, cudaStream_t st) {
+inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, int64_t brows, int max_pairs, bool early,
+                       cudaStream_t st) {
   static bool done[64] = {false};
   int rc = mx::allow_smem(mx_gemm_pair_kernel<GATED>, PR_SMEM, done, "ff_mxfp4_gemm");
   if (rc) return rc;
@@ -705,13 +856,7 @@ inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, in
   cfg.blockDim = dim3(PR_THREADS);
   cfg.dynamicSmemBytes = PR_SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  LaunchAttrs at(cfg, 2, early);
   FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel<GATED>, ta, tsa, tb, tsb, td, (int)((K + KB - 1) / KB), tiles_m,
                                  tiles_n, ep),
               "ff_mxfp4_gemm pair launch");
@@ -729,20 +874,22 @@ inline bool use_pair(const Epi& ep, int64_t K, int max_pairs) {
 }
 
 template <int NW>
-inline int launch_narrow_mp(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, cudaStream_t st) {
-  const int64_t num_kb = (K + KB - 1) / KB;
-  const int mp = ep.M <= 16 ? 16 : ep.M <= 32 ? 32 : ep.M <= 64 ? 64 : 128;
-  const int64_t items = ((NW == 2 ? ep.F : ep.N) + 127) / 128 * ((ep.M + mp - 1) / mp);
-  const int nsm = num_sms_current();
-  // split K while the items leave SMs idle or unevenly filled, and every CTA keeps four k-blocks
-  int c = 1;
-  while (c < 8 && items * c < 4 * nsm && num_kb >= 4 * (2 * c)) c *= 2;
-  switch (mp) {
-    case 16: return launch_narrow<16, NW>(a, b, K, ep, c, brows, st);
-    case 32: return launch_narrow<32, NW>(a, b, K, ep, c, brows, st);
-    case 64: return launch_narrow<64, NW>(a, b, K, ep, c, brows, st);
-    default: return launch_narrow<128, NW>(a, b, K, ep, c, brows, st);
-  }
+inline int launch_narrow_mp(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, bool early,
+                            cudaStream_t st) {
+  if (ep.M <= 16) return launch_narrow<16, NW>(a, b, K, ep, brows, early, st);
+  if (ep.M <= 32) return launch_narrow<32, NW>(a, b, K, ep, brows, early, st);
+  // two 128-row accumulators and their partial sums leave no room for 128 rows of A
+  if (NW == 2 || ep.M <= 64) return launch_narrow<64, NW>(a, b, K, ep, brows, early, st);
+  return launch_narrow<128, 1>(a, b, K, ep, brows, early, st);
+}
+
+// the product with whichever kernel suits it
+template <int NW>
+inline int launch_product(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, bool early,
+                          cudaStream_t st) {
+  const int pairs = max_pairs_current();
+  if (use_pair<NW == 2>(ep, K, pairs)) return launch_pair<NW == 2>(a, b, K, ep, brows, pairs, early, st);
+  return launch_narrow_mp<NW>(a, b, K, ep, brows, early, st);
 }
 
 inline int check_operand(const char* name, const char* which, const Operand& o, int64_t K) {
@@ -778,9 +925,7 @@ extern "C" int ff_mxfp4_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, c
   ep.bias = bias;
   ep.out_f32 = out_kind == FF_OUT_F32;
   ep.vec = ff::aligned(D, 16) && (ldd * (ep.out_f32 ? 4 : 2)) % 16 == 0;
-  const int pairs = max_pairs_current();
-  if (use_pair<false>(ep, K, pairs)) return launch_pair<false>(a, b, K, ep, N, pairs, ff::as_stream(stream));
-  return launch_narrow_mp<1>(a, b, K, ep, N, ff::as_stream(stream));
+  return launch_product<1>(a, b, K, ep, N, false, ff::as_stream(stream));
 }
 
 extern "C" int ff_mxfp4_swiglu_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, const uint8_t* B, int64_t ldb,
@@ -806,7 +951,99 @@ extern "C" int ff_mxfp4_swiglu_gemm(const uint8_t* A, int64_t lda, const uint8_t
   ep.hs = hs;
   ep.ldh = ldh;
   ep.hchunks = ff::mx::chunks_of(F);
-  const int pairs = max_pairs_current();
-  if (use_pair<true>(ep, K, pairs)) return launch_pair<true>(a, b, K, ep, 2 * F, pairs, ff::as_stream(stream));
-  return launch_narrow_mp<2>(a, b, K, ep, 2 * F, ff::as_stream(stream));
+  return launch_product<2>(a, b, K, ep, 2 * F, false, ff::as_stream(stream));
+}
+
+// Workspace of the fused calls: codes, then scales, of each intermediate matrix, 1024-byte aligned parts.
+namespace ff {
+namespace mxg {
+inline int64_t part_bytes(int64_t rows, int64_t cols) {
+  return (rows * ((cols + 31) / 32 * 16) + 1023) / 1024 * 1024 + mx::scale_bytes(rows, cols);
+}
+inline Operand part_at(uint8_t* ws, int64_t rows, int64_t cols) {
+  const int64_t ld = (cols + 31) / 32 * 16;
+  return Operand{ws, ld, ws + (rows * ld + 1023) / 1024 * 1024};
+}
+}  // namespace mxg
+}  // namespace ff
+
+extern "C" int64_t ff_mxfp4_linear_ws_bytes(int64_t M, int64_t K) {
+  return M < 1 || K < 1 ? 0 : ff::mxg::part_bytes(M, K);
+}
+
+extern "C" int64_t ff_mxfp4_swiglu_mlp_ws_bytes(int64_t M, int64_t K, int64_t F) {
+  return M < 1 || K < 1 || F < 1 ? 0 : ff::mxg::part_bytes(M, K) + ff::mxg::part_bytes(M, F);
+}
+
+extern "C" int ff_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* sW,
+                               const float* bias, void* D, int64_t ldd, int out_kind, int64_t M, int64_t N, int64_t K,
+                               uint8_t* ws, int64_t ws_bytes, void* stream) {
+  using namespace ff::mxg;
+  FF_REQUIRE(M >= 0 && N >= 0 && K >= 1, FF_ERR_INVALID_ARG, "ff_mxfp4_linear: M=%lld N=%lld K=%lld", (long long)M, (long long)N,
+             (long long)K);
+  FF_REQUIRE(out_kind == FF_OUT_F32 || out_kind == FF_OUT_BF16, FF_ERR_INVALID_ARG, "ff_mxfp4_linear: bad out_kind %d", out_kind);
+  if (M == 0 || N == 0) return FF_OK;
+  FF_REQUIRE(D && ldd >= N, FF_ERR_INVALID_ARG, "ff_mxfp4_linear: null output or ldd=%lld < N=%lld", (long long)ldd, (long long)N);
+  FF_REQUIRE(M <= 65535 * 128 && N < ((int64_t)1 << 22) && K < ((int64_t)1 << 30), FF_ERR_UNSUPPORTED,
+             "ff_mxfp4_linear: dimension too large (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
+  FF_REQUIRE(ws && ff::aligned(ws, 16) && ws_bytes >= part_bytes(M, K), FF_ERR_INVALID_ARG,
+             "ff_mxfp4_linear: workspace of %lld bytes (16-byte aligned) needed, got %lld", (long long)part_bytes(M, K),
+             (long long)ws_bytes);
+  const Operand a = part_at(ws, M, K), b{W, ldw, sW};
+  int rc;
+  if ((rc = check_operand("ff_mxfp4_linear", "W", b, K))) return rc;
+  rc = ff_mxfp4_quant(x, dtype, M, K, ldx, const_cast<uint8_t*>(a.q), a.ld, const_cast<uint8_t*>(a.s), nullptr, 0, nullptr, nullptr,
+                      nullptr, stream);
+  if (rc) return rc;
+  Epi ep{};
+  ep.D = D;
+  ep.ldd = ldd;
+  ep.M = M;
+  ep.N = N;
+  ep.bias = bias;
+  ep.out_f32 = out_kind == FF_OUT_F32;
+  ep.vec = ff::aligned(D, 16) && (ldd * (ep.out_f32 ? 4 : 2)) % 16 == 0;
+  return launch_product<1>(a, b, K, ep, N, true, ff::as_stream(stream));
+}
+
+extern "C" int ff_mxfp4_swiglu_mlp(const void* x, int dtype, int64_t ldx, const uint8_t* GU, int64_t ldgu, const uint8_t* sGU,
+                                   const uint8_t* W, int64_t ldw, const uint8_t* sW, void* D, int64_t ldd, int out_kind,
+                                   int64_t M, int64_t K, int64_t F, int64_t N, uint8_t* ws, int64_t ws_bytes, void* stream) {
+  using namespace ff::mxg;
+  FF_REQUIRE(M >= 0 && N >= 0 && K >= 1 && F >= 1, FF_ERR_INVALID_ARG, "ff_mxfp4_swiglu_mlp: M=%lld K=%lld F=%lld N=%lld",
+             (long long)M, (long long)K, (long long)F, (long long)N);
+  FF_REQUIRE(F % 128 == 0, FF_ERR_UNSUPPORTED, "ff_mxfp4_swiglu_mlp: F=%lld is not a multiple of 128", (long long)F);
+  FF_REQUIRE(out_kind == FF_OUT_F32 || out_kind == FF_OUT_BF16, FF_ERR_INVALID_ARG, "ff_mxfp4_swiglu_mlp: bad out_kind %d", out_kind);
+  if (M == 0 || N == 0) return FF_OK;
+  FF_REQUIRE(D && ldd >= N, FF_ERR_INVALID_ARG, "ff_mxfp4_swiglu_mlp: null output or ldd=%lld < N=%lld", (long long)ldd, (long long)N);
+  FF_REQUIRE(M <= 65535 * 128 && N < ((int64_t)1 << 22) && F < ((int64_t)1 << 21) && K < ((int64_t)1 << 30), FF_ERR_UNSUPPORTED,
+             "ff_mxfp4_swiglu_mlp: dimension too large (M=%lld K=%lld F=%lld N=%lld)", (long long)M, (long long)K, (long long)F,
+             (long long)N);
+  const int64_t need = part_bytes(M, K) + part_bytes(M, F);
+  FF_REQUIRE(ws && ff::aligned(ws, 16) && ws_bytes >= need, FF_ERR_INVALID_ARG,
+             "ff_mxfp4_swiglu_mlp: workspace of %lld bytes (16-byte aligned) needed, got %lld", (long long)need, (long long)ws_bytes);
+  const Operand a = part_at(ws, M, K), h = part_at(ws + part_bytes(M, K), M, F), gu{GU, ldgu, sGU}, w{W, ldw, sW};
+  int rc;
+  if ((rc = check_operand("ff_mxfp4_swiglu_mlp", "gate_up", gu, K)) || (rc = check_operand("ff_mxfp4_swiglu_mlp", "down", w, F)))
+    return rc;
+  rc = ff_mxfp4_quant(x, dtype, M, K, ldx, const_cast<uint8_t*>(a.q), a.ld, const_cast<uint8_t*>(a.s), nullptr, 0, nullptr, nullptr,
+                      nullptr, stream);
+  if (rc) return rc;
+  Epi eh{};
+  eh.M = M;
+  eh.N = 2 * F;
+  eh.F = F;
+  eh.hq = const_cast<uint8_t*>(h.q);
+  eh.hs = const_cast<uint8_t*>(h.s);
+  eh.ldh = h.ld;
+  eh.hchunks = ff::mx::chunks_of(F);
+  if ((rc = launch_product<2>(a, gu, K, eh, 2 * F, true, ff::as_stream(stream)))) return rc;
+  Epi ep{};
+  ep.D = D;
+  ep.ldd = ldd;
+  ep.M = M;
+  ep.N = N;
+  ep.out_f32 = out_kind == FF_OUT_F32;
+  ep.vec = ff::aligned(D, 16) && (ldd * (ep.out_f32 ? 4 : 2)) % 16 == 0;
+  return launch_product<1>(h, w, F, ep, N, true, ff::as_stream(stream));
 }

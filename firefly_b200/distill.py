@@ -44,7 +44,8 @@ class DistillationLossFn(torch.autograd.Function):
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
     """[..., width] as a matrix with unit column stride."""
-    t = t.reshape(-1, width)
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
     return t if t.stride(1) == 1 and t.stride(0) >= width else t.contiguous()
 
 
@@ -91,9 +92,13 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     _capi._require_cuda(logits, teacher_ids, teacher_logits, labels, teacher_lse)
     lab = None if labels is None else labels.reshape(-1).contiguous()
     lse = None if teacher_lse is None else teacher_lse.reshape(-1).to(torch.float32).contiguous()
-    out = DistillationLossFn.apply(_rows(logits, V), _rows(teacher_ids, k), _rows(teacher_logits, k), lab, lse, temperature,
-                                   alpha, int(ignore_index), reduction, torch.is_grad_enabled())
-    return out.view(lead) if reduction == "none" else out
+    args = (_rows(logits, V), _rows(teacher_ids, k), _rows(teacher_logits, k), lab, lse, temperature, alpha, int(ignore_index))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        out = DistillationLossFn.apply(*args, reduction, True)
+    else:
+        row, loss, *_ = _capi.distill_loss(_capi.distill_rows(*args), args[0], reduction, False)
+        out = row if reduction == "none" else loss
+    return out.view(lead) if reduction == "none" and len(lead) != 1 else out
 
 
 __all__ = ["DistillationLossFn", "distillation_loss"]

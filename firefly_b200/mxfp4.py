@@ -55,6 +55,14 @@ class MXFP4Tensor:
             raise ValueError(f"transposed form of a {rows} x {cols} matrix has shape {transposed.shape}")
         self.codes, self.scales, self.shape, self.transposed = codes, scales, (rows, cols), transposed
 
+    @classmethod
+    def _made(cls, pair, rows: int, cols: int, transposed=None) -> "MXFP4Tensor":
+        """From a kernel's own output."""
+        q = cls.__new__(cls)
+        q.codes, q.scales = pair
+        q.shape, q.transposed = (rows, cols), transposed
+        return q
+
     @property
     def device(self) -> torch.device:
         return self.codes.device
@@ -80,7 +88,9 @@ class MXFP4Tensor:
 def _matrix(x: torch.Tensor, what: str) -> torch.Tensor:
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError(f"{what} must be a 2-D tensor, got {tuple(x.shape) if isinstance(x, torch.Tensor) else type(x)}")
-    return x.detach() if x.dtype in (torch.float32, torch.bfloat16, torch.float16) else x.detach().float()
+    if x.requires_grad:
+        x = x.detach()
+    return x if x.dtype in (torch.float32, torch.bfloat16, torch.float16) else x.float()
 
 
 def quantize_fp_to_mxfp4(x: torch.Tensor, transposed: bool = False) -> MXFP4Tensor:
@@ -90,7 +100,7 @@ def quantize_fp_to_mxfp4(x: torch.Tensor, transposed: bool = False) -> MXFP4Tens
     x = _matrix(x, "x")
     rows, cols, _ = _capi.mxfp4_quant(x, rows=True, cols=transposed)
     R, C = x.shape
-    return MXFP4Tensor(*rows, (R, C), MXFP4Tensor(*cols, (C, R)) if transposed else None)
+    return MXFP4Tensor._made(rows, R, C, MXFP4Tensor._made(cols, C, R) if transposed else None)
 
 
 def quantize_fp_to_mxfp4_dual(x: torch.Tensor) -> tuple[MXFP4Tensor, MXFP4Tensor]:
@@ -115,7 +125,9 @@ def _bias(bias: torch.Tensor | None, n: int) -> torch.Tensor | None:
         return None
     if tuple(bias.shape) != (n,):
         raise ValueError(f"bias must have shape ({n},), got {tuple(bias.shape)}")
-    return bias.detach().to(torch.float32).contiguous()
+    if bias.requires_grad:
+        bias = bias.detach()
+    return bias if bias.dtype == torch.float32 and bias.is_contiguous() else bias.to(torch.float32).contiguous()
 
 
 def _product(a, b, M, N, K, bias=None, dtype=torch.bfloat16) -> torch.Tensor:
@@ -250,7 +262,7 @@ def _check_input(x: torch.Tensor, k: int, *others) -> torch.Tensor:
         elif o is not None:
             tensors.append(o)
     _capi._require_cuda(*tensors)
-    return x.reshape(-1, k)
+    return x if x.dim() == 2 else x.reshape(-1, k)
 
 
 def mxfp4_linear(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor", bias: torch.Tensor | None = None) -> torch.Tensor:
@@ -259,9 +271,15 @@ def mxfp4_linear(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor", bias: to
     w, packed = _split(weight, "weight")
     O, K = weight.shape
     x2 = _check_input(x, K, weight, bias)
-    _bias(bias, O)
-    grad = torch.is_grad_enabled()
-    return MXFP4LinearFn.apply(x2, w, bias, packed, grad).view(*x.shape[:-1], O)
+    if bias is not None and tuple(bias.shape) != (O,):
+        raise ValueError(f"bias must have shape ({O},), got {tuple(bias.shape)}")
+    grad = torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
+                                        or (bias is not None and bias.requires_grad))
+    if not grad and packed is not None and x2.shape[0] > 0:
+        y = _capi.mxfp4_linear(_matrix(x2, "x"), packed._pair(), O, K, None if bias is None else _bias(bias, O))
+    else:
+        y = MXFP4LinearFn.apply(x2, w, bias, packed, grad)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], O)
 
 
 def mxfp4_swiglu(x: torch.Tensor, gate_up: "torch.Tensor | MXFP4Tensor", down: "torch.Tensor | MXFP4Tensor") -> torch.Tensor:
@@ -275,7 +293,13 @@ def mxfp4_swiglu(x: torch.Tensor, gate_up: "torch.Tensor | MXFP4Tensor", down: "
         raise ValueError(f"gated block shapes: gate_up {tuple(gate_up.shape)}, down {tuple(down.shape)} "
                          "(gate_up [2F, K], down [O, F], F a multiple of 32)")
     x2 = _check_input(x, K, gate_up, down)
-    return MXFP4SwiGLUFn.apply(x2, wgu, wd, (pgu, pd), torch.is_grad_enabled()).view(*x.shape[:-1], O)
+    grad = torch.is_grad_enabled() and (x.requires_grad or (wgu is not None and wgu.requires_grad)
+                                        or (wd is not None and wd.requires_grad))
+    if not grad and pgu is not None and pd is not None and F % 128 == 0 and x2.shape[0] > 0:
+        y = _capi.mxfp4_swiglu_mlp(_matrix(x2, "x"), pgu._pair(), pd._pair(), F, O)
+    else:
+        y = MXFP4SwiGLUFn.apply(x2, wgu, wd, (pgu, pd), grad)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], O)
 
 
 class _Frozen(nn.Module):

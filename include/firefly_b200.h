@@ -576,6 +576,23 @@ FF_API int ff_mxfp4_swiglu_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA
                                 int64_t K, void* stream);
 
 /*
+ * Serving forms, activations in, activations out, on one stream in one call: x [M, K] (dtype, ldx elements)
+ * is quantised and multiplied with a weight held in MXFP4 (ff_mxfp4_linear: D = x W^T + bias), or taken
+ * through a SwiGLU block (ff_mxfp4_swiglu_mlp: GU [2F, K], then W [N, F]; F a multiple of 128).  The
+ * intermediate codes and scales lie in ws (16-byte aligned, *_ws_bytes(..) bytes, no initial content); the
+ * later kernels are launched early and wait on the device for the earlier ones.
+ */
+FF_API int64_t ff_mxfp4_linear_ws_bytes(int64_t M, int64_t K);
+FF_API int64_t ff_mxfp4_swiglu_mlp_ws_bytes(int64_t M, int64_t K, int64_t F);
+FF_API int ff_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint8_t* W, int64_t ldw, const uint8_t* sW,
+                           const float* bias, void* D, int64_t ldd, int out_kind, int64_t M, int64_t N, int64_t K,
+                           uint8_t* ws, int64_t ws_bytes, void* stream);
+FF_API int ff_mxfp4_swiglu_mlp(const void* x, int dtype, int64_t ldx, const uint8_t* GU, int64_t ldgu,
+                               const uint8_t* sGU, const uint8_t* W, int64_t ldw, const uint8_t* sW, void* D,
+                               int64_t ldd, int out_kind, int64_t M, int64_t K, int64_t F, int64_t N, uint8_t* ws,
+                               int64_t ws_bytes, void* stream);
+
+/*
  * Distillation loss from a teacher's top logits (the reference has no counterpart).  Row r: student
  * logits s [vocab]; `top` entries (token id, teacher logit t), an entry with a negative id or t = -inf
  * being absent; optionally a label and the teacher's log-sum-exp of its logits / T.
