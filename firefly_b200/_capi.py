@@ -174,7 +174,7 @@ def _raise(rc: int, name: str) -> None:
 
 def _call(name: str, *args) -> None:
     global LAUNCHES
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != FF_OK:
         _raise(rc, name)
     LAUNCHES += _KERNELS_PER_CALL.get(name, 0)
@@ -202,6 +202,16 @@ class _OnDevice:
     def __exit__(self, *exc):
         if self.guard is not None:
             self.guard.__exit__(*exc)
+
+
+def _addr(t: torch.Tensor | None):
+    """A tensor's address for a ``void*`` argument (an int needs no ctypes object of its own)."""
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(dev: torch.device) -> int:
+    """torch's current stream of ``dev`` as an address."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
@@ -809,8 +819,8 @@ def mxfp4_quant(x: torch.Tensor, rows: bool = True, cols: bool = False, colsum: 
         sums = torch.empty((C,), dtype=torch.float32, device=dev)
         ws = torch.empty(((R + 127) // 128 * C,), dtype=torch.float32, device=dev)
     with _OnDevice(dev):
-        _call("ff_mxfp4_quant", _ptr(x), _dtype_code(x.dtype), R, C, ldx, _ptr(q), (C + 31) // 32 * 16, _ptr(s),
-              _ptr(qt), (R + 31) // 32 * 16, _ptr(st), _ptr(sums), _ptr(ws), _stream(dev))
+        _call("ff_mxfp4_quant", _addr(x), _dtype_code(x.dtype), R, C, ldx, _addr(q), (C + 31) // 32 * 16, _addr(s),
+              _addr(qt), (R + 31) // 32 * 16, _addr(st), _addr(sums), _addr(ws), _raw_stream(dev))
     return (None if q is None else (q, s)), (None if qt is None else (qt, st)), sums
 
 
@@ -818,8 +828,8 @@ def mxfp4_dequant(codes: torch.Tensor, scales: torch.Tensor, rows: int, cols: in
     dev = _require_cuda(codes, scales)
     out = torch.empty((rows, cols), dtype=dtype, device=dev)
     with _OnDevice(dev):
-        _call("ff_mxfp4_dequant", _ptr(codes), codes.stride(0) if rows > 1 else codes.shape[1], _ptr(scales), rows, cols,
-              _ptr(out), _dtype_code(dtype), cols, _stream(dev))
+        _call("ff_mxfp4_dequant", _addr(codes), codes.stride(0) if rows > 1 else codes.shape[1], _addr(scales), rows, cols,
+              _addr(out), _dtype_code(dtype), cols, _raw_stream(dev))
     return out
 
 
@@ -831,8 +841,8 @@ def mxfp4_gemm(a, b, M: int, N: int, K: int, bias: torch.Tensor | None = None,
         raise ValueError(f"MXFP4 product: output dtype {out_dtype} (bfloat16 or float32)")
     out = torch.empty((M, N), dtype=out_dtype, device=dev)
     with _OnDevice(dev):
-        _call("ff_mxfp4_gemm", _ptr(a[0]), a[0].shape[1], _ptr(a[1]), _ptr(b[0]), b[0].shape[1], _ptr(b[1]), _ptr(bias),
-              _ptr(out), N, FF_OUT_F32 if out_dtype == torch.float32 else FF_OUT_BF16, M, N, K, _stream(dev))
+        _call("ff_mxfp4_gemm", _addr(a[0]), a[0].shape[1], _addr(a[1]), _addr(b[0]), b[0].shape[1], _addr(b[1]), _addr(bias),
+              _addr(out), N, FF_OUT_F32 if out_dtype == torch.float32 else FF_OUT_BF16, M, N, K, _raw_stream(dev))
     return out
 
 
@@ -841,8 +851,8 @@ def mxfp4_swiglu_gemm(a, b, M: int, F: int, K: int) -> tuple[torch.Tensor, torch
     dev = _require_cuda(a[0], a[1], b[0], b[1])
     hq, hs = _mx_alloc(M, F, dev)
     with _OnDevice(dev):
-        _call("ff_mxfp4_swiglu_gemm", _ptr(a[0]), a[0].shape[1], _ptr(a[1]), _ptr(b[0]), b[0].shape[1], _ptr(b[1]),
-              _ptr(hq), hq.shape[1], _ptr(hs), M, F, K, _stream(dev))
+        _call("ff_mxfp4_swiglu_gemm", _addr(a[0]), a[0].shape[1], _addr(a[1]), _addr(b[0]), b[0].shape[1], _addr(b[1]),
+              _addr(hq), hq.shape[1], _addr(hs), M, F, K, _raw_stream(dev))
     return hq, hs
 
 
@@ -854,8 +864,8 @@ def mxfp4_swiglu_quant(gu: torch.Tensor, cols: bool = False):
     q, s = _mx_alloc(T, F, dev)
     qt, st = _mx_alloc(F, T, dev) if cols else (None, None)
     with _OnDevice(dev):
-        _call("ff_mxfp4_swiglu_quant", _ptr(gu), ld, T, F, _ptr(q), q.shape[1], _ptr(s), _ptr(qt), (T + 31) // 32 * 16,
-              _ptr(st), _stream(dev))
+        _call("ff_mxfp4_swiglu_quant", _addr(gu), ld, T, F, _addr(q), q.shape[1], _addr(s), _addr(qt), (T + 31) // 32 * 16,
+              _addr(st), _raw_stream(dev))
     return (q, s), (qt, st) if cols else None
 
 
@@ -870,8 +880,8 @@ def mxfp4_swiglu_bwd_quant(dh: torch.Tensor, gu: torch.Tensor, rows: bool = True
     q, s = _mx_alloc(T, 2 * F, dev) if rows else (None, None)
     qt, st = _mx_alloc(2 * F, T, dev) if cols else (None, None)
     with _OnDevice(dev):
-        _call("ff_mxfp4_swiglu_bwd_quant", _ptr(dh), lddh, _ptr(gu), ld, T, F, _ptr(q), (2 * F + 31) // 32 * 16, _ptr(s),
-              _ptr(qt), (T + 31) // 32 * 16, _ptr(st), _stream(dev))
+        _call("ff_mxfp4_swiglu_bwd_quant", _addr(dh), lddh, _addr(gu), ld, T, F, _addr(q), (2 * F + 31) // 32 * 16, _addr(s),
+              _addr(qt), (T + 31) // 32 * 16, _addr(st), _raw_stream(dev))
     return (q, s) if rows else None, (qt, st) if cols else None
 
 
@@ -886,7 +896,7 @@ def mxfp4_linear(x: torch.Tensor, w, N: int, K: int, bias: torch.Tensor | None) 
     with _OnDevice(dev):
         _call("ff_mxfp4_linear", x.data_ptr(), _dtype_code(x.dtype), ldx, w[0].data_ptr(), w[0].shape[1], w[1].data_ptr(),
               None if bias is None else bias.data_ptr(), out.data_ptr(), N, FF_OUT_BF16, M, N, K, ws.data_ptr(), nbytes,
-              _stream(dev))
+              _raw_stream(dev))
     return out
 
 
@@ -901,7 +911,7 @@ def mxfp4_swiglu_mlp(x: torch.Tensor, gu, w, F: int, N: int) -> torch.Tensor:
     with _OnDevice(dev):
         _call("ff_mxfp4_swiglu_mlp", x.data_ptr(), _dtype_code(x.dtype), ldx, gu[0].data_ptr(), gu[0].shape[1],
               gu[1].data_ptr(), w[0].data_ptr(), w[0].shape[1], w[1].data_ptr(), out.data_ptr(), N, FF_OUT_BF16, M, K, F, N,
-              ws.data_ptr(), nbytes, _stream(dev))
+              ws.data_ptr(), nbytes, _raw_stream(dev))
     return out
 
 
@@ -933,8 +943,8 @@ def distill_loss(rows: DistillRows, logits: torch.Tensor, reduction: str, grad: 
             g = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev)
             held = torch.empty((1,), dtype=torch.float32, device=dev)
     with _OnDevice(dev):
-        _call("ff_distill_loss", ctypes.byref(rows), FF_REDUCE[reduction], _ptr(row), _ptr(loss), _ptr(g),
-              logits.shape[1], _ptr(held), _ptr(counts), _stream(dev))
+        _call("ff_distill_loss", ctypes.byref(rows), FF_REDUCE[reduction], _addr(row), _addr(loss), _addr(g),
+              logits.shape[1], _addr(held), _addr(counts), _raw_stream(dev))
     return row, loss, g, held, counts
 
 
@@ -947,8 +957,8 @@ def distill_grad(rows: DistillRows, logits: torch.Tensor, reduction: str, upstre
     if grad is None:
         grad, held = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev), None
     with _OnDevice(dev):
-        _call("ff_distill_grad", ctypes.byref(rows), FF_REDUCE[reduction], _ptr(upstream), _ptr(held), int(keep_held),
-              _ptr(counts), _ptr(grad), logits.shape[1], _stream(dev))
+        _call("ff_distill_grad", ctypes.byref(rows), FF_REDUCE[reduction], _addr(upstream), _addr(held), int(keep_held),
+              _addr(counts), _addr(grad), logits.shape[1], _raw_stream(dev))
     return grad
 
 
