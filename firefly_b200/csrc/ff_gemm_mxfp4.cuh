@@ -492,7 +492,8 @@ template <bool GATED>
 __global__ void __launch_bounds__(PR_THREADS, 1)
     mx_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmSA,
                         const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmSB,
-                        const __grid_constant__ CUtensorMap tmD, int num_kb, int tiles_m, int tiles_n, Epi ep) {
+                        const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmB2, int num_kb,
+                        int tiles_m, int tiles_n, int split, Epi ep) {
   constexpr int ST = PR_STAGES;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -518,6 +519,23 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank(), peer = rank ^ 1u;
   const int total = tiles_m * tiles_n, pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  // This pair's j-th item: tile pair + j * num_pairs; with `split` the tiles of the last partial wave (at
+  // most half as many as pairs) are cut into 256 x 128 halves, one per pair.  half = -1: a whole tile.
+  const int full_waves = split ? total / num_pairs : 0, rest = total - full_waves * num_pairs;
+  auto item = [&](int j, int& tm, int& tn, int& half) -> bool {
+    int t = pair + j * num_pairs;
+    half = -1;
+    if (split && j >= full_waves) {
+      if (j > full_waves || pair >= 2 * rest) return false;
+      t = full_waves * num_pairs + (pair >> 1);
+      half = pair & 1;
+    }
+    if (t >= total) return false;
+    tile_coords(t, tiles_m, tiles_n, tm, tn);
+    return true;
+  };
+  const uint32_t num_items = split ? (uint32_t)(full_waves + (pair < 2 * rest ? 1 : 0))
+                                   : (pair < total ? (uint32_t)((total - pair + num_pairs - 1) / num_pairs) : 0u);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
@@ -555,11 +573,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       int s = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; ok && t < total; t += num_pairs) {
-        int tm, tn;
-        tile_coords(t, tiles_m, tiles_n, tm, tn);
+      int tm, tn, half;
+      for (int j = 0; ok && item(j, tm, tn, half); ++j) {
         const int ra = tm * 2 + (int)rank;  // this CTA's 128 rows of A, in units of 128
-        const int rb0 = GATED ? tn : tn * 2, rb1 = GATED ? (int)(ep.F / 128) + tn : tn * 2 + 1;
+        // the 128-row groups of B: both halves of the tile, or twice the one half
+        const int rb0 = GATED ? tn : tn * 2 + (half > 0), rb1 = GATED ? (int)(ep.F / 128) + tn : tn * 2 + (half != 0);
         const int rb = rank ? rb1 : rb0;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!wait_bar(empty_bar(s), phase ^ 1u, abort_flag)) {
@@ -567,12 +585,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
             break;
           }
           const uint32_t lbar = mapa_shared(full_bar(s), 0);
-          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * PR_STAGE);
+          if (rank == 0) mbar_arrive_expect_tx(full_bar(s), 2 * (half < 0 ? PR_STAGE : PR_STAGE - ROWS_BYTES / 2));
           tma_load_2d_pair(sSA(s), &tmSA, kb * 256, ra, lbar);
           tma_load_2d_pair(sSB(s, 0), &tmSB, kb * 256, rb0, lbar);
           tma_load_2d_pair(sSB(s, 1), &tmSB, kb * 256, rb1, lbar);
           tma_load_2d_pair(sA(s), &tmA, kb * 128, ra * 128, lbar);
-          tma_load_2d_pair(sB(s), &tmB, kb * 128, rb * 128, lbar);
+          if (half < 0) tma_load_2d_pair(sB(s), &tmB, kb * 128, rb * 128, lbar);
+          else tma_load_2d_pair(sB(s), &tmB2, kb * 128, rb0 * 128 + (int)rank * 64, lbar);  // its 64 rows of the half
           if (++s == ST) {
             s = 0;
             phase ^= 1u;
@@ -584,11 +603,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader only)
     if (rank == 0 && lane == 0) {
-      constexpr uint32_t idesc = idesc_mx(256, 256);
-      int s = 0, acc = 0, tile = 0;
+      int s = 0, acc = 0, tm_, tn_, half;
       uint32_t phase = 0;
       bool ok = true;
-      for (int t = pair; ok && t < total; t += num_pairs, ++tile) {
+      for (int tile = 0; ok && item(tile, tm_, tn_, half); ++tile) {
+        const uint32_t idesc = half < 0 ? idesc_mx(256, 256) : idesc_mx(256, 128);
         if (tile > 0 && !wait_bar(shared_bar, (uint32_t)(tile - 1) & 1u, abort_flag)) break;
         const uint32_t d = tmem + (uint32_t)(acc * PR_ACC1);
         for (int kb = 0; kb < num_kb; ++kb) {
@@ -619,7 +638,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
   } else if (warp == 2 + PR_EPI_WARPS) {
     // ------------------------------------------------------------ scales into TMEM (leader only)
     if (rank == 0 && lane == 0) {
-      const uint32_t steps = pair < total ? (uint32_t)((total - pair + num_pairs - 1) / num_pairs) * (uint32_t)num_kb : 0u;
+      const uint32_t steps = num_items * (uint32_t)num_kb;
       int s = 0;
       uint32_t phase = 0, g = 0;
       for (; g < steps; ++g) {
@@ -646,11 +665,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     uint8_t* stage = ctrl + 512 + (warp - 2) * 4096;
     const uint32_t stage_addr = cbase + 512 + (uint32_t)(warp - 2) * 4096;
     uint32_t nst = 0;
-    int tile = 0;
+    int tm, tn, half;
     const uint32_t sbar = mapa_shared(shared_bar, 0);
-    for (int t = pair; t < total; t += num_pairs, ++tile) {
-      int tm, tn;
-      tile_coords(t, tiles_m, tiles_n, tm, tn);
+    for (int tile = 0; item(tile, tm, tn, half); ++tile) {
       const int acc = tile & 1;
       if (!__all_sync(0xffffffffu, wait_bar(tfull_bar(acc), (uint32_t)(tile >> 1) & 1u, abort_flag))) break;
       tc_fence_after();
@@ -658,7 +675,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       const uint32_t tb = tmem + ((uint32_t)(lg * 32) << 16) + (uint32_t)(acc * PR_ACC1);
       // the columns that the accumulators share (the upper half of accumulator 0, the lower half of
       // accumulator 1) are read first: two 32-column chunks per warp, then the next tile may start
-      const int sh = acc ? 0 : 4;
+      const int sh = acc || half >= 0 ? 0 : 4;  // a half tile has no other columns (and no next tile)
       uint32_t r0[32], r1[32];
       tmem_ld32(tb + (sh + eh * 2) * 32, r0);
       tmem_ld32(tb + (sh + eh * 2 + 1) * 32, r1);
@@ -667,11 +684,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(sbar);
       if constexpr (!GATED) {
-        const int64_t col0 = (int64_t)tn * 256 + eh * 64;
+        const int64_t col0 = (int64_t)tn * 256 + (half > 0 ? 128 : 0) + eh * 64;
         pair_store(r0, row, col0 + sh * 32, ep, &tmD, lane, stage, stage_addr, nst);
         pair_store(r1, row, col0 + sh * 32 + 32, ep, &tmD, lane, stage, stage_addr, nst);
 #pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 2 && half < 0; ++i) {
           tmem_ld32(tb + ((4 - sh) + eh * 2 + i) * 32, r0);
           tmem_wait_ld();
           pair_store(r0, row, col0 + (4 - sh) * 32 + i * 32, ep, &tmD, lane, stage, stage_addr, nst);
@@ -842,7 +859,7 @@ inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, in
   static bool done[64] = {false};
   int rc = mx::allow_smem(mx_gemm_pair_kernel<GATED>, PR_SMEM, done, "ff_mxfp4_gemm");
   if (rc) return rc;
-  CUtensorMap ta, tsa, tb, tsb, td;
+  CUtensorMap ta, tsa, tb, tsb, td, tb2;
   memset(&td, 0, sizeof(td));
   if ((rc = make_map_codes(&ta, a.q, ep.M, K, a.ld, 128))) return rc;
   if ((rc = make_map_sf(&tsa, a.s, ep.M, K))) return rc;
@@ -851,14 +868,18 @@ inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, in
   ep.tma_store = !GATED && !ep.out_f32 && ep.vec;
   if (ep.tma_store && (rc = make_map_out_bf16(&td, ep.D, ep.M, ep.N, ep.ldd, true))) return rc;
   const int tiles_m = (int)((ep.M + 255) / 256), tiles_n = (int)(GATED ? ep.F / 128 : (ep.N + 255) / 256);
+  const int total = tiles_m * tiles_n, pairs = min(total, max_pairs), rest = total % pairs;
+  const int split = !GATED && total > pairs && rest > 0 && 2 * rest <= pairs;
+  tb2 = tb;
+  if (split && (rc = make_map_codes(&tb2, b.q, brows, K, b.ld, 64))) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * min64((int64_t)tiles_m * tiles_n, max_pairs)));
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
   cfg.blockDim = dim3(PR_THREADS);
   cfg.dynamicSmemBytes = PR_SMEM;
   cfg.stream = st;
   LaunchAttrs at(cfg, 2, early);
-  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel<GATED>, ta, tsa, tb, tsb, td, (int)((K + KB - 1) / KB), tiles_m,
-                                 tiles_n, ep),
+  FF_CUDA_TRY(cudaLaunchKernelEx(&cfg, mx_gemm_pair_kernel<GATED>, ta, tsa, tb, tsb, td, tb2, (int)((K + KB - 1) / KB),
+                                 tiles_m, tiles_n, split, ep),
               "ff_mxfp4_gemm pair launch");
   return check_launch("ff_mxfp4_gemm (pair)");
 }
