@@ -104,18 +104,23 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // 128 up rows) against MP rows of A; the CTAs of a cluster take equal runs of its k-blocks.  Persistent
 // clusters, one CTA per SM: the loads run on from item to item.  The fp32 partial sums meet in shared
 // memory: each warp of the cluster adds its (row of A, 32 columns) pieces over the CTAs in rank order,
-// so the result does not depend on timing and no workspace is needed.  Two barriers per CTA order the
-// exchange: `pfull` (every CTA's partial sums are written) and `pfree` (every CTA has read them).
+// so the result does not depend on timing and no workspace is needed.  Two barriers per CTA and buffer
+// order the exchange: `pfull` (every CTA's partial sums are written) and `pfree` (every CTA has read
+// them).  Where two buffers fit, an item's sums are added up after the next item's have been written,
+// so that a CTA does not stand still for the others' arrival.
 // ---------------------------------------------------------------------------
 __host__ __device__ constexpr int nr_stage_bytes(int mp, int nw) { return nw * (ROWS_BYTES + SF_BYTES) + mp * 128 + SF_BYTES; }
-__host__ __device__ constexpr int nr_part_bytes(int mp, int nw) { return nw * mp * 128 * 4; }
+__host__ __device__ constexpr int nr_bufs(int mp, int nw) { return nw * mp <= 64 ? 2 : 1; }
+__host__ __device__ constexpr int nr_part_one(int mp, int nw) { return nw * mp * 128 * 4; }
+__host__ __device__ constexpr int nr_part_bytes(int mp, int nw) { return nr_bufs(mp, nw) * nr_part_one(mp, nw); }
 __host__ __device__ constexpr int nr_stages(int mp, int nw) {
   return (224 * 1024 - nr_part_bytes(mp, nw)) / nr_stage_bytes(mp, nw) > 10
              ? 10
              : (224 * 1024 - nr_part_bytes(mp, nw)) / nr_stage_bytes(mp, nw);
 }
+constexpr int NR_THREADS = NUM_THREADS + 32;  // TMA, MMA, four epilogue warps, scale copies
 __host__ __device__ constexpr int nr_smem(int mp, int nw) {
-  return nr_stages(mp, nw) * nr_stage_bytes(mp, nw) + nr_part_bytes(mp, nw) + 1024 + 256;
+  return nr_stages(mp, nw) * nr_stage_bytes(mp, nw) + nr_part_bytes(mp, nw) + 1024 + 384;
 }
 __host__ __device__ constexpr int pow2_cols(int c) { return c <= 32 ? 32 : c <= 64 ? 64 : c <= 128 ? 128 : c <= 256 ? 256 : 512; }
 __host__ __device__ constexpr int nr_tmem(int mp, int nw) { return pow2_cols(2 * nw * mp + nr_stages(mp, nw) * (nw + 1) * 8); }
@@ -150,7 +155,7 @@ using mx::let_next_kernel_start;
 using mx::wait_for_previous_kernel;
 
 template <int MP, int NW>
-__global__ void __launch_bounds__(NUM_THREADS, 1)
+__global__ void __launch_bounds__(NR_THREADS, 1)
     mx_gemm_narrow_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmSW,
                           const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmSX, int num_kb,
                           int tiles_w, int tiles_x, Epi ep) {
@@ -175,9 +180,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
   auto empty_bar = [&](int s) { return cbase + 8u * (ST + s); };
   auto tfull_bar = [&](int a) { return cbase + 8u * (2 * ST + a); };
   auto tempty_bar = [&](int a) { return cbase + 8u * (2 * ST + 2 + a); };
-  const uint32_t pfull = cbase + 8u * (2 * ST + 4), pfree = pfull + 8u, drain = pfull + 16u;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (2 * ST + 7));
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * ST + 7) + 4);
+  constexpr int PB = nr_bufs(MP, NW);
+  auto pfull = [&](int b) { return cbase + 8u * (2 * ST + 4 + b); };
+  auto pfree = [&](int b) { return cbase + 8u * (2 * ST + 6 + b); };
+  const uint32_t drain = cbase + 8u * (2 * ST + 8);
+  auto sf_ready = [&](int s) { return cbase + 8u * (2 * ST + 9 + s); };  // the stage's scales are in TMEM
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ctrl + 8 * (3 * ST + 9));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (3 * ST + 9) + 4);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)blockIdx.x, csize = (int)gridDim.x;  // the cluster spans grid x
@@ -189,13 +198,16 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
     for (int s = 0; s < ST; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
+      mbar_init(sf_ready(s), 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
       mbar_init(tempty_bar(a), 4);
     }
-    mbar_init(pfull, 4 * csize);
-    mbar_init(pfree, 4 * csize);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(pfull(b), 4 * csize);
+      mbar_init(pfree(b), 4 * csize);
+    }
     mbar_init(drain, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -279,21 +291,14 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         tc_fence_after();
         const uint32_t d = tmem + (uint32_t)(acc * NW * MP);
         for (int kb = kb0; kb < kb1; ++kb) {
-          if (!wait_bar(full_bar(s), phase, abort_flag)) {
+          if (!wait_bar(sf_ready(s), phase, abort_flag)) {  // after the stage itself: the copies waited for it
             ok = false;
             break;
           }
           tc_fence_after();
-          // this stage's scales: 8 columns per operand, slots as many as stages.  A's chunks cover 128 rows,
-          // 32 to a column: the second half of them belongs to an odd tile of 64.
+          // the scales of A cover 128 rows, 32 to a column: the second half of them belongs to an odd tile of 64
           const uint32_t sf = tmem + (uint32_t)(2 * NW * MP + s * (NW + 1) * 8);
           const uint32_t sfx = sf + NW * 8 + (uint32_t)(it % tiles_x * MP % 128 / 32);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-#pragma unroll
-            for (int w = 0; w < NW; ++w) sf_copy<1>(sf + w * 8 + c * 4, sSW(s, w) + c * 512);
-            sf_copy<1>(sf + NW * 8 + c * 4, sSX(s) + c * 512);
-          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
 #pragma unroll
@@ -319,20 +324,103 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
       drain_bar(drain, 0);
     }
     __syncwarp();
+  } else if (warp == 6) {
+    // ------------------------------------------------------------ scales into TMEM
+    // by a warp of its own: one thread's copies and products do not overlap (4096 x 22016, one CTA: 0.5 us per
+    // k-block with the copies in the MMA thread)
+    if (lane == 0) {
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int it = first; ok && it < items; it += stride) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!wait_bar(full_bar(s), phase, abort_flag)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sf = tmem + (uint32_t)(2 * NW * MP + s * (NW + 1) * 8);  // slots as many as stages
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int w = 0; w < NW; ++w) sf_copy<1>(sf + w * 8 + c * 4, sSW(s, w) + c * 512);
+            sf_copy<1>(sf + NW * 8 + c * 4, sSX(s) + c * 512);
+          }
+          tc_commit(sf_ready(s));
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
     const int lg = warp & 3;
     int acc = 0;
-    uint32_t acc_phase = 0, xphase = 0;
-    for (int it = first; it < items; it += stride) {
+    uint32_t acc_phase = 0;
+    // adds up the sums of this CTA group's n-th item, which lie in buffer n % PB
+    auto finish = [&](int n) -> bool {
+      const int it = first + n * stride, b = n % PB;
       const int tw = it / tiles_x, tx = it % tiles_x;
       const int jn = (int)min64(MP, ep.M - (int64_t)tx * MP);
-      if (!__all_sync(0xffffffffu, wait_bar(tfull_bar(acc), acc_phase, abort_flag))) break;
+      if (!__all_sync(0xffffffffu, wait_bar_cluster(pfull(b), (uint32_t)(n / PB) & 1u, abort_flag))) return false;
+#pragma unroll 1
+      for (int p = rank * 4 + (warp - 2); p < jn * 4; p += csize * 4) {
+        const int j = p >> 2, lq = p & 3;
+        const uint32_t at = part_addr + (uint32_t)(b * nr_part_one(MP, NW) + (j * 128 + lq * 32 + lane) * 4);
+        float v = 0.f, u = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < csize; ++r) {
+          const uint32_t a = mapa_shared(at, (uint32_t)r);
+          v += ld_cluster_f32(a);
+          if constexpr (NW == 2) u += ld_cluster_f32(a + MP * 128 * 4);
+        }
+        const int64_t m = (int64_t)tx * MP + j;
+        if constexpr (NW == 1) {
+          const int64_t n_ = (int64_t)tw * 128 + lq * 32 + lane;
+          if (n_ < ep.N) {
+            if (ep.bias) v += __ldg(ep.bias + n_);
+            if (ep.out_f32) static_cast<float*>(ep.D)[m * ep.ldd + n_] = v;
+            else static_cast<__nv_bfloat16*>(ep.D)[m * ep.ldd + n_] = __float2bfloat16_rn(v);
+          }
+        } else {
+          // one block of h: 32 features, a lane each
+          const float h = swiglu_h(v, u);
+          const uint32_t S = mx::scale_code(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7FFFFFFFu));
+          const float t[8] = {h * mx::inv_scale(S), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+          uint32_t w = S == mx::kScaleNan ? 0u : (mx::codes8(t) & 0xFu) << (4 * (lane & 7));
+          w |= __shfl_xor_sync(0xffffffffu, w, 1);
+          w |= __shfl_xor_sync(0xffffffffu, w, 2);
+          w |= __shfl_xor_sync(0xffffffffu, w, 4);
+          const int64_t blk = (int64_t)tw * 4 + lq;
+          if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(ep.hq + m * ep.ldh + blk * 16 + (lane >> 3) * 4) = w;
+          if (lane == 0) ep.hs[mx::scale_at(m, blk, ep.hchunks)] = (uint8_t)S;
+        }
+      }
+      if constexpr (NW == 2) {  // the padding chunk of h's scales
+        if (rank == 0 && tw == tiles_w - 1 && tx % (128 / MP) == 0 && ep.hchunks * 128 > ep.F)
+          reinterpret_cast<uint32_t*>(ep.hs)[((int64_t)(tx * MP / 128) * ep.hchunks + ep.F / 128) * 128 + (threadIdx.x - 64)] = 0;
+      }
+      __syncwarp();
+      if (lane < csize) mbar_arrive_remote(mapa_shared(pfree(b), (uint32_t)lane));
+      return true;
+    };
+    int n = 0;
+    bool ok = true;
+    for (int it = first; ok && it < items; it += stride, ++n) {
+      const int tw = it / tiles_x, tx = it % tiles_x;
+      const int jn = (int)min64(MP, ep.M - (int64_t)tx * MP);
+      if (!__all_sync(0xffffffffu, wait_bar(tfull_bar(acc), acc_phase, abort_flag))) {
+        ok = false;
+        break;
+      }
       tc_fence_after();
       const uint32_t tb = tmem + ((uint32_t)(lg * 32) << 16) + (uint32_t)(acc * NW * MP);
       if (direct) {
-        const int64_t n = (int64_t)tw * 128 + lg * 32 + lane;
-        const float b = ep.bias && n < ep.N ? __ldg(ep.bias + n) : 0.f;
+        const int64_t n_ = (int64_t)tw * 128 + lg * 32 + lane;
+        const float b = ep.bias && n_ < ep.N ? __ldg(ep.bias + n_) : 0.f;
 #pragma unroll 1
         for (int c = 0; c < jn; c += 16) {
           uint32_t r[16];
@@ -340,8 +428,8 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            if (c + j < jn && n < ep.N) {
-              const int64_t at = ((int64_t)tx * MP + c + j) * ep.ldd + n;
+            if (c + j < jn && n_ < ep.N) {
+              const int64_t at = ((int64_t)tx * MP + c + j) * ep.ldd + n_;
               const float v = __uint_as_float(r[j]) + b;
               if (ep.out_f32) static_cast<float*>(ep.D)[at] = v;
               else static_cast<__nv_bfloat16*>(ep.D)[at] = __float2bfloat16_rn(v);
@@ -352,8 +440,13 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(tempty_bar(acc));
       } else {
-        // the partial sums of the last item have been read everywhere
-        if (!__all_sync(0xffffffffu, wait_bar_cluster(pfree, xphase ^ 1u, abort_flag))) break;
+        // the partial sums that lay in this buffer have been read everywhere
+        const int b = n % PB;
+        if (!__all_sync(0xffffffffu, wait_bar_cluster(pfree(b), ((uint32_t)(n / PB) & 1u) ^ 1u, abort_flag))) {
+          ok = false;
+          break;
+        }
+        float* dst = part + b * (nr_part_one(MP, NW) / 4);
 #pragma unroll 1
         for (int c = 0; c < NW * MP; c += 16) {
           if (c % MP >= jn) continue;
@@ -361,59 +454,20 @@ __global__ void __launch_bounds__(NUM_THREADS, 1)
           tmem_ld16(tb + c, r);
           tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) part[(c + j) * 128 + lg * 32 + lane] = __uint_as_float(r[j]);
+          for (int j = 0; j < 16; ++j) dst[(c + j) * 128 + lg * 32 + lane] = __uint_as_float(r[j]);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(tempty_bar(acc));
-        if (lane < csize) mbar_arrive_remote(mapa_shared(pfull, (uint32_t)lane));
-        if (!__all_sync(0xffffffffu, wait_bar_cluster(pfull, xphase, abort_flag))) break;
-#pragma unroll 1
-        for (int p = rank * 4 + (warp - 2); p < jn * 4; p += csize * 4) {
-          const int j = p >> 2, lq = p & 3;
-          const uint32_t at = part_addr + (uint32_t)((j * 128 + lq * 32 + lane) * 4);
-          float v = 0.f, u = 0.f;
-#pragma unroll 4
-          for (int r = 0; r < csize; ++r) {
-            const uint32_t a = mapa_shared(at, (uint32_t)r);
-            v += ld_cluster_f32(a);
-            if constexpr (NW == 2) u += ld_cluster_f32(a + MP * 128 * 4);
-          }
-          const int64_t m = (int64_t)tx * MP + j;
-          if constexpr (NW == 1) {
-            const int64_t n = (int64_t)tw * 128 + lq * 32 + lane;
-            if (n < ep.N) {
-              if (ep.bias) v += __ldg(ep.bias + n);
-              if (ep.out_f32) static_cast<float*>(ep.D)[m * ep.ldd + n] = v;
-              else static_cast<__nv_bfloat16*>(ep.D)[m * ep.ldd + n] = __float2bfloat16_rn(v);
-            }
-          } else {
-            // one block of h: 32 features, a lane each
-            const float h = swiglu_h(v, u);
-            const uint32_t S = mx::scale_code(__reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7FFFFFFFu));
-            const float t[8] = {h * mx::inv_scale(S), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            uint32_t w = S == mx::kScaleNan ? 0u : (mx::codes8(t) & 0xFu) << (4 * (lane & 7));
-            w |= __shfl_xor_sync(0xffffffffu, w, 1);
-            w |= __shfl_xor_sync(0xffffffffu, w, 2);
-            w |= __shfl_xor_sync(0xffffffffu, w, 4);
-            const int64_t blk = (int64_t)tw * 4 + lq;
-            if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(ep.hq + m * ep.ldh + blk * 16 + (lane >> 3) * 4) = w;
-            if (lane == 0) ep.hs[mx::scale_at(m, blk, ep.hchunks)] = (uint8_t)S;
-          }
-        }
-        if constexpr (NW == 2) {  // the padding chunk of h's scales
-          if (rank == 0 && tw == tiles_w - 1 && tx % (128 / MP) == 0 && ep.hchunks * 128 > ep.F)
-            reinterpret_cast<uint32_t*>(ep.hs)[((int64_t)(tx * MP / 128) * ep.hchunks + ep.F / 128) * 128 + (threadIdx.x - 64)] = 0;
-        }
-        __syncwarp();
-        if (lane < csize) mbar_arrive_remote(mapa_shared(pfree, (uint32_t)lane));
-        xphase ^= 1u;
+        if (lane < csize) mbar_arrive_remote(mapa_shared(pfull(b), (uint32_t)lane));
+        if (n >= PB - 1) ok = finish(n - (PB - 1));
       }
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1u;
       }
     }
+    if (ok && !direct && PB == 2 && n > 0) finish(n - 1);
     __syncwarp();
   }
 
@@ -802,7 +856,7 @@ inline int narrow_clusters(int csize) {
   if (!cache[dev][lc]) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)csize);
-    cfg.blockDim = dim3(NUM_THREADS);
+    cfg.blockDim = dim3(NR_THREADS);
     cfg.dynamicSmemBytes = nr_smem(MP, NW);
     LaunchAttrs at(cfg, csize, false);
     int n = 0;
@@ -815,6 +869,10 @@ inline int narrow_clusters(int csize) {
   return cache[dev][lc];
 }
 
+#ifndef MXN_X
+#define MXN_X 2
+#define MXN_Y 1
+#endif
 template <int MP, int NW>
 inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, bool early,
                          cudaStream_t st) {
@@ -829,22 +887,28 @@ inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Ep
   const int64_t tiles_w = ((NW == 2 ? ep.F : ep.N) + 127) / 128, tiles_x = (ep.M + MP - 1) / MP, items = tiles_w * tiles_x;
   FF_REQUIRE(items < ((int64_t)1 << 31), FF_ERR_UNSUPPORTED, "ff_mxfp4_gemm: too many tiles");
   const int64_t num_kb = (K + KB - 1) / KB;
-  // The cluster size whose busiest CTA has the least to do: its turns times the k-blocks of a turn, plus
-  // about two k-blocks' time for the exchange of a turn where K is split.
+  // The cluster size whose busiest CTA has the least to do, in k-blocks' time: its turns, each as long as
+  // its k-blocks or as the exchange that runs beside them, whichever takes longer, and one exchange at the
+  // end.
   int csize = 1, clusters = 1;
   int64_t best = INT64_MAX;
   for (int c = 1; c <= 8 && c <= num_kb; c *= 2) {
     const int n = narrow_clusters<MP, NW>(c);
-    const int64_t turns = (items + n - 1) / n, cost = turns * ((num_kb + c - 1) / c + (c > 1 ? 2 : 0));
+    const int64_t turns = (items + n - 1) / n, kbs = (num_kb + c - 1) / c;
+    const int64_t exchange = c == 1 && NW == 1 ? 0 : MXN_X + NW * MP * MXN_Y / 16;
+    const int64_t cost = turns * max64(kbs, exchange) + exchange;
     if (cost < best) {
       best = cost;
       csize = c;
       clusters = (int)min64(items, n);
     }
   }
+#ifdef MXN_FORCE
+  if (num_kb >= MXN_FORCE) { csize = MXN_FORCE; clusters = (int)min64(items, narrow_clusters<MP, NW>(csize)); }
+#endif
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)csize, (unsigned)clusters);
-  cfg.blockDim = dim3(NUM_THREADS);
+  cfg.blockDim = dim3(NR_THREADS);
   cfg.dynamicSmemBytes = nr_smem(MP, NW);
   cfg.stream = st;
   LaunchAttrs at(cfg, csize, early);
