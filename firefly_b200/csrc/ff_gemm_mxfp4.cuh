@@ -854,6 +854,8 @@ inline int narrow_clusters(int csize) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return num_sms_current() / csize / 2 + 1;
   const int lc = csize == 1 ? 0 : csize == 2 ? 1 : csize == 4 ? 2 : 3;
   if (!cache[dev][lc]) {
+    static bool done[64] = {false};
+    mx::allow_smem(mx_gemm_narrow_kernel<MP, NW>, nr_smem(MP, NW), done, "ff_mxfp4_gemm");  // or nothing would fit
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)csize);
     cfg.blockDim = dim3(NR_THREADS);
@@ -862,17 +864,39 @@ inline int narrow_clusters(int csize) {
     int n = 0;
     if (cudaOccupancyMaxActiveClusters(&n, mx_gemm_narrow_kernel<MP, NW>, &cfg) != cudaSuccess || n < 1) {
       cudaGetLastError();
-      n = 1;
+      n = max(1, num_sms_current() / csize - 1);
     }
     cache[dev][lc] = n;
   }
   return cache[dev][lc];
 }
 
-#ifndef MXN_X
-#define MXN_X 2
-#define MXN_Y 1
-#endif
+// Time of the narrow kernel in units of its k-block (0.45 us a CTA, the rate at which one SM's copies
+// arrive from HBM; 0.84 us with gate and up rows), and the cluster size that gives it.  A CTA takes
+// `turns` items of `kbs` k-blocks; the exchange of a turn runs beside the next turn's k-blocks, the last
+// one after them.  Measured on 1 to 128 rows, 512 to 22016 x 1024 to 11008, clusters of 1 to 8: an
+// exchange takes 5 + rows/16 (9/c + 1) k-blocks, e.g. 2.9 us for one row and 14 us for 128 in clusters
+// of 4; clusters of 1 need none (a local one for the activation).
+template <int MP, int NW>
+inline double narrow_cost(const Epi& ep, int64_t K, int* csize, int* clusters) {
+  const int64_t items = ((NW == 2 ? ep.F : ep.N) + 127) / 128 * ((ep.M + MP - 1) / MP), num_kb = (K + KB - 1) / KB;
+  const double rows = (double)min64(ep.M, MP) / 16.0;
+  double best = 1e300;
+  for (int c = 1; c <= 8 && c <= num_kb; c *= 2) {
+    const int n = narrow_clusters<MP, NW>(c);
+    const double turns = (double)((items + n - 1) / n), kbs = (double)((num_kb + c - 1) / c);
+    double x = c > 1 ? 5.0 + rows * (9.0 / c + 1.0) : (NW == 2 ? 5.0 + 2.0 * rows : 0.0);
+    if (NW == 2) x *= 0.7;
+    const double cost = (turns - 1) * (kbs > x ? kbs : x) + kbs + x + rows;
+    if (cost < best) {
+      best = cost;
+      *csize = c;
+      *clusters = (int)min64(items, n);
+    }
+  }
+  return best;
+}
+
 template <int MP, int NW>
 inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, bool early,
                          cudaStream_t st) {
@@ -887,25 +911,8 @@ inline int launch_narrow(const Operand& a, const Operand& b, int64_t K, const Ep
   const int64_t tiles_w = ((NW == 2 ? ep.F : ep.N) + 127) / 128, tiles_x = (ep.M + MP - 1) / MP, items = tiles_w * tiles_x;
   FF_REQUIRE(items < ((int64_t)1 << 31), FF_ERR_UNSUPPORTED, "ff_mxfp4_gemm: too many tiles");
   const int64_t num_kb = (K + KB - 1) / KB;
-  // The cluster size whose busiest CTA has the least to do, in k-blocks' time: its turns, each as long as
-  // its k-blocks or as the exchange that runs beside them, whichever takes longer, and one exchange at the
-  // end.
-  int csize = 1, clusters = 1;
-  int64_t best = INT64_MAX;
-  for (int c = 1; c <= 8 && c <= num_kb; c *= 2) {
-    const int n = narrow_clusters<MP, NW>(c);
-    const int64_t turns = (items + n - 1) / n, kbs = (num_kb + c - 1) / c;
-    const int64_t exchange = c == 1 && NW == 1 ? 0 : MXN_X + NW * MP * MXN_Y / 16;
-    const int64_t cost = turns * max64(kbs, exchange) + exchange;
-    if (cost < best) {
-      best = cost;
-      csize = c;
-      clusters = (int)min64(items, n);
-    }
-  }
-#ifdef MXN_FORCE
-  if (num_kb >= MXN_FORCE) { csize = MXN_FORCE; clusters = (int)min64(items, narrow_clusters<MP, NW>(csize)); }
-#endif
+  int csize, clusters;
+  narrow_cost<MP, NW>(ep, K, &csize, &clusters);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)csize, (unsigned)clusters);
   cfg.blockDim = dim3(NR_THREADS);
@@ -948,16 +955,6 @@ inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, in
   return check_launch("ff_mxfp4_gemm (pair)");
 }
 
-// Pair tiles or narrow items?  Times in units of a pair's tile per k-block, measured where noted.
-template <bool GATED>
-inline bool use_pair(const Epi& ep, int64_t K, int max_pairs) {
-  (void)K;
-  if (max_pairs < 1 || ep.M <= 128) return false;
-  const int64_t tiles = (ep.M + 255) / 256 * (GATED ? ep.F / 128 : (ep.N + 255) / 256);
-  if (tiles >= ((int64_t)1 << 31)) return false;
-  return tiles * 2 >= max_pairs;
-}
-
 template <int NW>
 inline int launch_narrow_mp(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, bool early,
                             cudaStream_t st) {
@@ -968,12 +965,31 @@ inline int launch_narrow_mp(const Operand& a, const Operand& b, int64_t K, const
   return launch_narrow<128, 1>(a, b, K, ep, brows, early, st);
 }
 
-// the product with whichever kernel suits it
+template <int NW>
+inline double narrow_cost_mp(const Epi& ep, int64_t K) {
+  int c, n;
+  if (ep.M <= 16) return narrow_cost<16, NW>(ep, K, &c, &n);
+  if (ep.M <= 32) return narrow_cost<32, NW>(ep, K, &c, &n);
+  if (NW == 2 || ep.M <= 64) return narrow_cost<64, NW>(ep, K, &c, &n);
+  return narrow_cost<128, 1>(ep, K, &c, &n);
+}
+
+// The product with whichever kernel is the faster.  Pair kernel, in the units of narrow_cost and beyond
+// the narrow kernel's fixed time: 4 + 7/8 of a k-block per wave and k-block (0.385 us; 6 + 0.6 with gate and
+// up rows).  Measured at both: 33 x 4096 x 11008 21 us narrow, 29 us pair; 128 x 512 x 11008 21 and 29;
+// 129 x 4096 x 4096 33 and 18; 16 x 22016 x 4096 23 and 27; 64 x 22016 x 4096 27 and 27;
+// 512 x 12288 x 4096 37 and 25 (each with about 6 us of an empty measurement).
 template <int NW>
 inline int launch_product(const Operand& a, const Operand& b, int64_t K, const Epi& ep, int64_t brows, bool early,
                           cudaStream_t st) {
   const int pairs = max_pairs_current();
-  if (use_pair<NW == 2>(ep, K, pairs)) return launch_pair<NW == 2>(a, b, K, ep, brows, pairs, early, st);
+  const int64_t tiles = (ep.M + 255) / 256 * (NW == 2 ? ep.F / 128 : (ep.N + 255) / 256), num_kb = (K + KB - 1) / KB;
+  if (pairs > 0 && tiles < ((int64_t)1 << 31)) {
+    const double waves = (double)((tiles + pairs - 1) / pairs);
+    const double cost = NW == 2 ? 6.0 + 0.6 * waves * (double)num_kb : 4.0 + 0.875 * waves * (double)num_kb;
+    if (ep.M > 512 || cost < narrow_cost_mp<NW>(ep, K))
+      return launch_pair<NW == 2>(a, b, K, ep, brows, pairs, early, st);
+  }
   return launch_narrow_mp<NW>(a, b, K, ep, brows, early, st);
 }
 

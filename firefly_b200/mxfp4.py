@@ -77,6 +77,8 @@ class MXFP4Tensor:
     def scale_bytes(self) -> torch.Tensor:
         """The E8M0 scale byte of every block, uint8 [rows, ceil(cols/32)]."""
         rows, cols = self.shape
+        if rows == 0:
+            return self.scales.new_empty((0, (cols + 31) // 32))
         s = self.scales.view((rows + 127) // 128, -1, 32, 4, 4)  # row tile, chunk, row % 32, row / 32, block % 4
         s = s.permute(0, 3, 2, 1, 4).reshape((rows + 127) // 128 * 128, -1)
         return s[:rows, :(cols + 31) // 32].contiguous()

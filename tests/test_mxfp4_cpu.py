@@ -121,3 +121,28 @@ def test_c_entries_refuse_before_any_launch():
     assert g(p, 32, p, p, 32, p, n, p, 1 << 23, 2, 4, 1 << 22, 64, n) == uns
     assert g(n, 32, n, n, 32, n, n, n, 8, 2, 0, 8, 64, n) == _capi.FF_OK
     assert lib.ff_mxfp4_swiglu_gemm(p, 32, p, p, 32, p, p, 16, p, 4, 96, 64, n) == uns
+
+
+def test_serving_entries_refuse_before_any_launch():
+    lib, bad, uns = _capi.lib(), _capi.FF_ERR_INVALID_ARG, _capi.FF_ERR_UNSUPPORTED
+    p, n = ctypes.c_void_p(4096), None
+    need = lib.ff_mxfp4_linear_ws_bytes(3, 64)
+    assert need == 1024 + 1024 and lib.ff_mxfp4_linear_ws_bytes(0, 64) == 0
+    f = lib.ff_mxfp4_linear
+    assert f(p, 1, 64, p, 32, p, n, p, 8, 2, 3, 8, 64, p, need - 1, n) == bad    # workspace
+    assert f(p, 1, 64, p, 32, p, n, p, 8, 2, 3, 8, 64, n, need, n) == bad
+    assert f(p, 1, 64, p, 16, p, n, p, 8, 2, 3, 8, 64, p, need, n) == bad        # ldw
+    assert f(p, 1, 64, n, 32, p, n, p, 8, 2, 3, 8, 64, p, need, n) == bad
+    assert f(p, 1, 64, p, 32, p, n, p, 7, 2, 3, 8, 64, p, need, n) == bad        # ldd
+    assert f(p, 1, 64, p, 32, p, n, p, 8, 0, 3, 8, 64, p, need, n) == bad        # int32 output
+    assert f(p, 5, 64, p, 32, p, n, p, 8, 2, 3, 8, 64, p, need, n) == bad        # type
+    assert f(p, 1, 63, p, 32, p, n, p, 8, 2, 3, 8, 64, p, need, n) == bad        # ldx
+    assert f(p, 1, 64, p, 32, p, n, p, 8, 2, 3, 8, 0, p, need, n) == bad
+    assert f(n, 1, 64, n, 32, n, n, n, 8, 2, 0, 8, 64, n, 0, n) == _capi.FF_OK
+    need = lib.ff_mxfp4_swiglu_mlp_ws_bytes(3, 64, 128)
+    g = lib.ff_mxfp4_swiglu_mlp
+    assert g(p, 1, 64, p, 32, p, p, 64, p, p, 8, 2, 3, 64, 96, 8, p, 1 << 20, n) == uns     # F
+    assert g(p, 1, 64, p, 32, p, p, 64, p, p, 8, 2, 3, 64, 128, 8, p, need - 1, n) == bad
+    assert g(p, 1, 64, p, 16, p, p, 64, p, p, 8, 2, 3, 64, 128, 8, p, need, n) == bad
+    assert g(p, 1, 64, p, 32, p, p, 48, p, p, 8, 2, 3, 64, 128, 8, p, need, n) == bad
+    assert g(p, 1, 64, p, 32, p, p, 64, p, p, 7, 2, 3, 64, 128, 8, p, need, n) == bad

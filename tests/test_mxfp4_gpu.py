@@ -132,7 +132,8 @@ SHAPES = [(1, 1, 1), (1, 128, 256), (1, 4096, 4096), (2, 130, 64), (16, 256, 512
           (33, 300, 777), (64, 128, 2000), (65, 129, 257), (128, 384, 1024), (129, 65, 320), (200, 500, 300),
           (255, 257, 288), (256, 256, 256), (257, 513, 1100), (512, 768, 2048), (700, 1300, 96), (1000, 3000, 640),
           (4096, 300, 128), (300, 5000, 31),
-          (1500, 3300, 1100), (2500, 1999, 288), (2304, 2560, 4096), (130, 20000, 512)]
+          (1500, 3300, 1100), (2500, 1999, 288), (2304, 2560, 4096), (130, 20000, 512),
+          (200, 512, 11008), (300, 130, 8200), (96, 3000, 2048), (50, 9000, 1056)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -280,7 +281,8 @@ def _flip_tolerance(v, mag, K, dtype, left, right):
 
 
 @pytest.mark.parametrize("T,K,F,N", [(1, 64, 128, 96), (3, 256, 32, 40), (16, 512, 384, 512), (40, 100, 160, 77),
-                                     (130, 256, 256, 300), (300, 320, 640, 256), (513, 512, 128, 260), (1300, 512, 1152, 640), (2200, 256, 640, 300)])
+                                     (130, 256, 256, 300), (300, 320, 640, 256), (513, 512, 128, 260), (1300, 512, 1152, 640), (2200, 256, 640, 300),
+                                     (100, 4096, 128, 64), (128, 8192, 256, 64), (20, 700, 1408, 90)])
 def test_gated_block_forward_and_gradients(T, K, F, N):
     x = _randn(T, K, 1).requires_grad_(True)
     wgu = _randn(2 * F, K, 2, scale=0.05).requires_grad_(True)
@@ -391,3 +393,75 @@ def test_two_streams_at_once():
     for k in range(2):
         for o in outs[k]:
             assert torch.equal(o, wants[k])
+
+
+def test_serving_calls_equal_their_parts():
+    """The fused calls against quantiser and products one by one, few and many rows, with odd widths."""
+    for T, K, F, N in ((1, 4096, 2048, 300), (15, 100, 128, 77), (40, 1000, 384, 260), (700, 512, 1280, 640)):
+        x = _randn(T, K, 1)
+        wgu, wd = quantize_fp_to_mxfp4(_randn(2 * F, K, 2, scale=0.05)), quantize_fp_to_mxfp4(_randn(N, F, 3, scale=0.05))
+        b = torch.randn(2 * F, device=DEV, generator=_gen(4))
+        assert torch.equal(mxfp4_linear(x, wgu, b), mxfp4_matmul(quantize_fp_to_mxfp4(x), wgu, b))
+        qx = quantize_fp_to_mxfp4(x)
+        h = MXFP4Tensor(*_capi.mxfp4_swiglu_quant(mxfp4_matmul(qx, wgu))[0], (T, F))
+        hq = MXFP4Tensor(*_capi.mxfp4_swiglu_gemm(qx._pair(), wgu._pair(), T, F, K), (T, F))
+        assert torch.equal(h.codes, hq.codes) and torch.equal(h.scale_bytes(), hq.scale_bytes())
+        assert torch.equal(mxfp4_swiglu(x, wgu, wd), mxfp4_matmul(h, wd))
+    assert _capi.device_status() == 0
+
+
+def test_a_weight_quantised_just_before_the_call():
+    """The serving kernels start early and ask for the weight first: it has to be there all the same."""
+    x = _randn(1, 4096, 1)
+    for s in range(6):
+        w = _randn(4096, 4096, 10 + s)
+        want = mxfp4_linear(x, quantize_fp_to_mxfp4(w))
+        torch.cuda.synchronize()
+        held = quantize_fp_to_mxfp4(torch.zeros_like(w))
+        torch.cuda.synchronize()
+        q = quantize_fp_to_mxfp4(w)
+        held.codes.copy_(q.codes)
+        held.scales.copy_(q.scales)
+        assert torch.equal(mxfp4_linear(x, held), want)
+
+
+def test_rows_of_nothing():
+    q = quantize_fp_to_mxfp4(torch.zeros(0, 64, device=DEV))
+    assert q.dequantize().shape == (0, 64) and q.scale_bytes().shape == (0, 2)
+    assert mxfp4_matmul(q, quantize_fp_to_mxfp4(_randn(5, 64, 1))).shape == (0, 5)
+
+
+def test_teacher_in_four_bits_distils_a_student():
+    """The operators as they are used together: a held MXFP4 teacher, its top logits, the distillation loss of an
+    MXFP4 student and the gradients of its weights, against the same chain in fp64 on the kernels' logits."""
+    from firefly_b200 import distillation_loss
+    from oracle import distill_oracle as D
+
+    d, f, V, T, k = 128, 256, 500, 40, 12
+    x = _randn(T, d, 1)
+    teacher = MXFP4SwiGLU(_randn(2 * f, d, 2, scale=0.05), _randn(d, f, 3, scale=0.05))
+    head_t = MXFP4Linear(_randn(V, d, 4, scale=0.2))
+    with torch.no_grad():
+        tl = head_t(teacher(x)).float()
+    top = tl.topk(k, dim=1)
+    lse = torch.logsumexp(tl / 2, 1)
+    wgu, wd, head = (_randn(*s, scale=c).requires_grad_(True)
+                     for s, c in (((2 * f, d, 5), 0.05), ((d, f, 6), 0.05), ((V, d, 7), 0.2)))
+    labels = torch.randint(0, V, (T,), device=DEV, generator=_gen(8))
+    hidden = mxfp4_swiglu(x, wgu, wd)
+    logits = mxfp4_linear(hidden, head)
+    logits.retain_grad()
+    hidden.retain_grad()
+    loss = distillation_loss(logits, top.indices, top.values, labels, teacher_lse=lse, temperature=2.0, alpha=0.5)
+    loss.backward()
+    s64 = logits.detach().double().requires_grad_(True)
+    rows, _, scale = D.losses(s64, top.indices, top.values, labels, lse, 2.0, 0.5)
+    assert abs(float(loss.detach()) - float(rows.detach().mean())) <= 2.0 ** -19 * (4 * (4 + float(scale.max())) + 16)
+    rows.mean().backward()
+    assert float((logits.grad.double() - s64.grad).abs().max()) <= 2.0 ** -8 * float(s64.grad.abs().max())
+    v, mag = O.product(O.values(logits.grad.t()), O.values(hidden.detach().t()))
+    assert bool(((head.grad.double() - v).abs() <= _tolerance(v, mag, T, torch.bfloat16)).all())
+    v, mag = O.product(O.values(logits.grad), O.values(head.detach().t()))
+    assert bool(((hidden.grad.double() - v).abs() <= _tolerance(v, mag, V, torch.bfloat16)).all())
+    for w in (wgu, wd):
+        assert torch.isfinite(w.grad).all() and bool(w.grad.any())
