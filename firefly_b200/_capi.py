@@ -88,6 +88,12 @@ SIGNATURES = {
     "ff_mxfp4_linear": (_I, [_P, _I, _I64, _P, _I64, _P, _P, _P, _I64, _I, _I64, _I64, _I64, _P, _I64, _P]),
     "ff_mxfp4_swiglu_mlp": (_I, [_P, _I, _I64, _P, _I64, _P, _P, _I64, _P, _P, _I64, _I, _I64, _I64, _I64, _I64, _P,
                                  _I64, _P]),
+    "ff_mxfp4_linear_train": (_I, [_P, _I, _I64, _P, _I, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P, _I64, _P]),
+    "ff_mxfp4_linear_bwd": (_I, [_P, _I, _I64, _P, _I64, _I, _I, _P, _I, _P, _I, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    "ff_mxfp4_swiglu_train": (_I, [_P, _I, _I64, _P, _I, _I64, _P, _I, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _I, _I,
+                                   _P, _I64, _P, _I64, _P]),
+    "ff_mxfp4_swiglu_bwd": (_I, [_P, _I, _I64, _P, _P, _P, _I64, _I, _I, _I, _P, _I, _P, _I, _P, _I, _I64, _I64, _I64,
+                                 _I64, _P, _I64, _P]),
     "ff_distill_loss": (_I, [_P, _I, _P, _P, _P, _I64, _P, _P, _P]),
     "ff_distill_grad": (_I, [_P, _I, _P, _P, _I, _P, _P, _I64, _P]),
     "ff_ipc_alloc": (_I, [_I64, ctypes.POINTER(ctypes.c_void_p)]),
@@ -140,6 +146,8 @@ _KERNELS_PER_CALL = {"ff_quant_rows_i8": 1, "ff_quant_dual_i8": 2, "ff_quant_dua
                      "ff_mxfp4_quant": 1, "ff_mxfp4_dequant": 1, "ff_mxfp4_swiglu_quant": 1,
                      "ff_mxfp4_swiglu_bwd_quant": 1, "ff_mxfp4_gemm": 1, "ff_mxfp4_swiglu_gemm": 1,
                      "ff_distill_loss": 3, "ff_distill_grad": 1, "ff_mxfp4_linear": 2, "ff_mxfp4_swiglu_mlp": 3,
+                     "ff_mxfp4_linear_train": 3, "ff_mxfp4_linear_bwd": 3, "ff_mxfp4_swiglu_train": 6,
+                     "ff_mxfp4_swiglu_bwd": 6,
                      "ff_adamw32_multi": 1}
 
 
@@ -913,6 +921,96 @@ def mxfp4_swiglu_mlp(x: torch.Tensor, gu, w, F: int, N: int) -> torch.Tensor:
               gu[1].data_ptr(), w[0].data_ptr(), w[0].shape[1], w[1].data_ptr(), out.data_ptr(), N, FF_OUT_BF16, M, K, F, N,
               ws.data_ptr(), nbytes, _raw_stream(dev))
     return out
+
+
+def _mx_part(rows: int, cols: int) -> int:
+    """``ff_mxfp4_linear_ws_bytes``: codes and scales of one matrix in a workspace."""
+    return (rows * ((cols + 31) // 32 * 16) + 1023) // 1024 * 1024 + (rows + 127) // 128 * ((cols + 255) // 256) * 1024
+
+
+def _mx_bytes(n: int, dev: torch.device) -> torch.Tensor | None:
+    return torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+
+
+def _mx_grad(shape, dtype: torch.dtype, dev: torch.device) -> tuple[torch.Tensor, int]:
+    """A gradient's buffer (fp32 where the parameter's type is not one of the kernel's outputs) and output kind."""
+    bf16 = dtype == torch.bfloat16
+    return torch.empty(shape, dtype=torch.bfloat16 if bf16 else torch.float32, device=dev), FF_OUT_BF16 if bf16 else FF_OUT_F32
+
+
+def mxfp4_linear_train(x, w, bias, need_dx: bool, need_dw: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """The linear layer's forward pass with a floating-point weight: ``(y, saved)``."""
+    x, ldx = _mx_float(x)
+    w, ldw = _mx_float(w)
+    dev, (M, K), N = x.device, x.shape, w.shape[0]
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    nt = _mx_part(M, K) + _mx_part(N, K)
+    ns = (_mx_part(K, M) if need_dw else 0) + (_mx_part(K, N) if need_dx else 0)
+    tmp, saved = _mx_bytes(nt, dev), _mx_bytes(ns, dev)
+    with _OnDevice(dev):
+        _call("ff_mxfp4_linear_train", x.data_ptr(), _dtype_code(x.dtype), ldx, w.data_ptr(), _dtype_code(w.dtype), ldw,
+              _addr(bias), y.data_ptr(), M, N, K, need_dx, need_dw, tmp.data_ptr(), nt, _addr(saved), ns, _raw_stream(dev))
+    return y, saved
+
+
+def mxfp4_linear_bwd(dy, saved, dims, had_dx, had_dw, dx_dtype, dw_dtype, need_db):
+    """``(dx, dw, db)`` of the linear layer; a gradient whose type is ``None`` is not formed.  db is fp32."""
+    dy, ld = _mx_float(dy)
+    dev, (M, N, K) = dy.device, dims
+    dx, kx = _mx_grad((M, K), dx_dtype, dev) if dx_dtype is not None else (None, FF_OUT_BF16)
+    dw, kw = _mx_grad((N, K), dw_dtype, dev) if dw_dtype is not None else (None, FF_OUT_BF16)
+    db = torch.empty((N,), dtype=torch.float32, device=dev) if need_db else None
+    nt = ((_mx_part(M, N) if dx is not None else 0) + (_mx_part(N, M) if dw is not None or need_db else 0)
+          + (((M + 127) // 128 * N * 4 + 15) // 16 * 16 if need_db else 0))
+    tmp = _mx_bytes(nt, dev)
+    with _OnDevice(dev):
+        _call("ff_mxfp4_linear_bwd", dy.data_ptr(), _dtype_code(dy.dtype), ld, _addr(saved),
+              0 if saved is None else saved.numel(), had_dx, had_dw, _addr(dx), kx, _addr(dw), kw, _addr(db), M, N, K,
+              _addr(tmp), nt, _raw_stream(dev))
+    if dx is not None and dx.dtype != dx_dtype:
+        dx = dx.to(dx_dtype)
+    if dw is not None and dw.dtype != dw_dtype:
+        dw = dw.to(dw_dtype)
+    return dx, dw, db
+
+
+def mxfp4_swiglu_train(x, wgu, wd, need_dx: bool, need_dgu: bool, need_dd: bool):
+    """The gated block's forward pass with floating-point weights: ``(y, gu, saved)``."""
+    x, ldx = _mx_float(x)
+    wgu, ldgu = _mx_float(wgu)
+    wd, ldd = _mx_float(wd)
+    dev, (M, K), (N, F) = x.device, x.shape, wd.shape
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    gu = torch.empty((M, 2 * F), dtype=torch.bfloat16, device=dev)
+    nt = _mx_part(M, K) + _mx_part(2 * F, K) + _mx_part(M, F) + _mx_part(N, F)
+    ns = ((_mx_part(K, M) if need_dgu else 0) + (_mx_part(K, 2 * F) if need_dx else 0) + (_mx_part(F, M) if need_dd else 0)
+          + (_mx_part(F, N) if need_dx or need_dgu else 0))
+    tmp, saved = _mx_bytes(nt, dev), _mx_bytes(ns, dev)
+    with _OnDevice(dev):
+        _call("ff_mxfp4_swiglu_train", x.data_ptr(), _dtype_code(x.dtype), ldx, wgu.data_ptr(), _dtype_code(wgu.dtype), ldgu,
+              wd.data_ptr(), _dtype_code(wd.dtype), ldd, gu.data_ptr(), y.data_ptr(), M, K, F, N, need_dx, need_dgu, need_dd,
+              tmp.data_ptr(), nt, _addr(saved), ns, _raw_stream(dev))
+    return y, gu, saved
+
+
+def mxfp4_swiglu_bwd(dy, gu, saved, dims, dx_dtype, dgu_dtype, dd_dtype):
+    """``(dx, dwgu, dwd)`` of the gated block; the types are those the forward pass saved for (``None``: not formed)."""
+    dy, ld = _mx_float(dy)
+    dev, (M, K, F, N) = dy.device, dims
+    need_dx, need_dgu, need_dd = dx_dtype is not None, dgu_dtype is not None, dd_dtype is not None
+    back = need_dx or need_dgu
+    dx, kx = _mx_grad((M, K), dx_dtype, dev) if need_dx else (None, FF_OUT_BF16)
+    dgu, kg = _mx_grad((2 * F, K), dgu_dtype, dev) if need_dgu else (None, FF_OUT_BF16)
+    dd, kd = _mx_grad((N, F), dd_dtype, dev) if need_dd else (None, FF_OUT_BF16)
+    dh = torch.empty((M, F), dtype=torch.bfloat16, device=dev) if back else None
+    nt = ((_mx_part(M, N) if back else 0) + (_mx_part(N, M) if need_dd else 0) + (_mx_part(M, 2 * F) if need_dx else 0)
+          + (_mx_part(2 * F, M) if need_dgu else 0))
+    tmp = _mx_bytes(nt, dev)
+    with _OnDevice(dev):
+        _call("ff_mxfp4_swiglu_bwd", dy.data_ptr(), _dtype_code(dy.dtype), ld, _addr(gu), _addr(dh), _addr(saved),
+              0 if saved is None else saved.numel(), need_dx, need_dgu, need_dd, _addr(dx), kx, _addr(dgu), kg, _addr(dd), kd,
+              M, K, F, N, _addr(tmp), nt, _raw_stream(dev))
+    return tuple(g if g is None or g.dtype == t else g.to(t) for g, t in ((dx, dx_dtype), (dgu, dgu_dtype), (dd, dd_dtype)))
 
 
 # ---------------------------------------------------------------------------

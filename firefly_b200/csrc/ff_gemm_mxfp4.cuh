@@ -1148,3 +1148,179 @@ extern "C" int ff_mxfp4_swiglu_mlp(const void* x, int dtype, int64_t ldx, const 
   ep.vec = ff::aligned(D, 16) && (ldd * (ep.out_f32 ? 4 : 2)) % 16 == 0;
   return launch_product<1>(h, w, F, ep, N, true, ff::as_stream(stream));
 }
+
+// ---------------------------------------------------------------------------
+// Training steps of the linear layer and of the gated block in one call each: the host's work of a small
+// step is most of its time.  `saved` keeps what the backward call reads (transposed codes), `tmp` the rest.
+// ---------------------------------------------------------------------------
+namespace ff {
+namespace mxg {
+struct Arena {  // parts of a workspace, in order
+  uint8_t* p;
+  int64_t left;
+  Operand take(int64_t rows, int64_t cols) {
+    const Operand o = part_at(p, rows, cols);
+    p += part_bytes(rows, cols);
+    left -= part_bytes(rows, cols);
+    return o;
+  }
+};
+inline uint8_t* mut(const uint8_t* p) { return const_cast<uint8_t*>(p); }
+// rows of x [R, C] and, with t, its columns
+inline int quant_to(const void* x, int dt, int64_t R, int64_t C, int64_t ld, const Operand* r, const Operand* t, float* sums,
+                    float* ws, void* stream) {
+  return ff_mxfp4_quant(x, dt, R, C, ld, r ? mut(r->q) : nullptr, r ? r->ld : 0, r ? mut(r->s) : nullptr, t ? mut(t->q) : nullptr,
+                        t ? t->ld : 0, t ? mut(t->s) : nullptr, sums, ws, stream);
+}
+// Launched early: the narrow kernel asks for B before it waits for the kernel ahead of it, so B is never
+// that kernel's output (the weight is quantised first, the activations last; the backward products' B is
+// saved).
+inline int product(const Operand& a, const Operand& b, const float* bias, void* D, int kind, int64_t M, int64_t N, int64_t K,
+                   void* stream) {
+  Epi ep{};
+  ep.D = D;
+  ep.ldd = N;
+  ep.M = M;
+  ep.N = N;
+  ep.bias = bias;
+  ep.out_f32 = kind == FF_OUT_F32;
+  ep.vec = aligned(D, 16) && (N * (ep.out_f32 ? 4 : 2)) % 16 == 0;
+  return launch_product<1>(a, b, K, ep, N, true, as_stream(stream));
+}
+inline bool float_kind(int k) { return k == FF_OUT_F32 || k == FF_OUT_BF16; }
+inline int check_dims(const char* name, int64_t M, int64_t N, int64_t K) {
+  // each of them is a row count of some product
+  FF_REQUIRE(M >= 1 && N >= 1 && K >= 1, FF_ERR_INVALID_ARG, "%s: M=%lld N=%lld K=%lld", name, (long long)M, (long long)N, (long long)K);
+  FF_REQUIRE(M < ((int64_t)1 << 22) && N < ((int64_t)1 << 22) && K < ((int64_t)1 << 22), FF_ERR_UNSUPPORTED,
+             "%s: dimension too large (M=%lld N=%lld K=%lld)", name, (long long)M, (long long)N, (long long)K);
+  return FF_OK;
+}
+inline int check_ws(const char* name, const char* what, const void* p, int64_t have, int64_t need) {
+  FF_REQUIRE(need == 0 || (p && aligned(p, 16) && have >= need), FF_ERR_INVALID_ARG,
+             "%s: %s of %lld bytes (16-byte aligned) needed, got %lld", name, what, (long long)need, (long long)have);
+  return FF_OK;
+}
+}  // namespace mxg
+}  // namespace ff
+
+extern "C" int ff_mxfp4_linear_train(const void* x, int x_dtype, int64_t ldx, const void* w, int w_dtype, int64_t ldw,
+                                     const float* bias, void* y, int64_t M, int64_t N, int64_t K, int need_dx, int need_dw,
+                                     uint8_t* tmp, int64_t tmp_bytes, uint8_t* saved, int64_t saved_bytes, void* stream) {
+  using namespace ff::mxg;
+  const char* name = "ff_mxfp4_linear_train";
+  int rc;
+  if ((rc = check_dims(name, M, N, K)) || (rc = check_ws(name, "tmp", tmp, tmp_bytes, part_bytes(M, K) + part_bytes(N, K))) ||
+      (rc = check_ws(name, "saved", saved, saved_bytes, (need_dw ? part_bytes(K, M) : 0) + (need_dx ? part_bytes(K, N) : 0))))
+    return rc;
+  FF_REQUIRE(y, FF_ERR_INVALID_ARG, "%s: null pointer", name);
+  Arena t{tmp, tmp_bytes}, k{saved, saved_bytes};
+  const Operand qx = t.take(M, K), qw = t.take(N, K);
+  Operand xt{}, wt{};
+  if (need_dw) xt = k.take(K, M);
+  if (need_dx) wt = k.take(K, N);
+  if ((rc = quant_to(w, w_dtype, N, K, ldw, &qw, need_dx ? &wt : nullptr, nullptr, nullptr, stream)) ||
+      (rc = quant_to(x, x_dtype, M, K, ldx, &qx, need_dw ? &xt : nullptr, nullptr, nullptr, stream)))
+    return rc;
+  return product(qx, qw, bias, y, FF_OUT_BF16, M, N, K, stream);
+}
+
+extern "C" int ff_mxfp4_linear_bwd(const void* dy, int dtype, int64_t lddy, const uint8_t* saved, int64_t saved_bytes,
+                                   int saved_dx, int saved_dw, void* dx, int dx_kind, void* dw, int dw_kind, float* db,
+                                   int64_t M, int64_t N, int64_t K, uint8_t* tmp, int64_t tmp_bytes, void* stream) {
+  using namespace ff::mxg;
+  const char* name = "ff_mxfp4_linear_bwd";
+  int rc;
+  const bool cols = dw || db;
+  const int64_t sums = db ? (ff_mxfp4_colsum_ws_elems(M, N) * 4 + 15) / 16 * 16 : 0;
+  if ((rc = check_dims(name, M, N, K)) ||
+      (rc = check_ws(name, "saved", saved, saved_bytes, (saved_dw ? part_bytes(K, M) : 0) + (saved_dx ? part_bytes(K, N) : 0))) ||
+      (rc = check_ws(name, "tmp", tmp, tmp_bytes, (dx ? part_bytes(M, N) : 0) + (cols ? part_bytes(N, M) : 0) + sums)))
+    return rc;
+  FF_REQUIRE((!dx || (saved_dx && float_kind(dx_kind))) && (!dw || (saved_dw && float_kind(dw_kind))), FF_ERR_INVALID_ARG,
+             "%s: a gradient whose operand was not saved, or a bad output kind", name);
+  Arena k{mut(saved), saved_bytes}, t{tmp, tmp_bytes};
+  Operand xt{}, wt{}, q{}, qt{};
+  if (saved_dw) xt = k.take(K, M);
+  if (saved_dx) wt = k.take(K, N);
+  if (dx) q = t.take(M, N);
+  if (cols) qt = t.take(N, M);
+  if ((rc = quant_to(dy, dtype, M, N, lddy, dx ? &q : nullptr, cols ? &qt : nullptr, db, db ? reinterpret_cast<float*>(t.p) : nullptr,
+                     stream)))
+    return rc;
+  if (dx && (rc = product(q, wt, nullptr, dx, dx_kind, M, K, N, stream))) return rc;
+  if (dw && (rc = product(qt, xt, nullptr, dw, dw_kind, N, K, M, stream))) return rc;
+  return FF_OK;
+}
+
+extern "C" int ff_mxfp4_swiglu_train(const void* x, int x_dtype, int64_t ldx, const void* wgu, int gu_dtype, int64_t ldgu,
+                                     const void* wd, int d_dtype, int64_t ldd, void* gu, void* y, int64_t M, int64_t K,
+                                     int64_t F, int64_t N, int need_dx, int need_dgu, int need_dd, uint8_t* tmp,
+                                     int64_t tmp_bytes, uint8_t* saved, int64_t saved_bytes, void* stream) {
+  using namespace ff::mxg;
+  const char* name = "ff_mxfp4_swiglu_train";
+  int rc;
+  const bool back = need_dx || need_dgu;
+  if ((rc = check_dims(name, M, N, K)) || (rc = check_dims(name, 2 * F, N, K)) ||
+      (rc = check_ws(name, "tmp", tmp, tmp_bytes, part_bytes(M, K) + part_bytes(2 * F, K) + part_bytes(M, F) + part_bytes(N, F))) ||
+      (rc = check_ws(name, "saved", saved, saved_bytes,
+                     (need_dgu ? part_bytes(K, M) : 0) + (need_dx ? part_bytes(K, 2 * F) : 0) + (need_dd ? part_bytes(F, M) : 0) +
+                         (back ? part_bytes(F, N) : 0))))
+    return rc;
+  FF_REQUIRE(y && gu, FF_ERR_INVALID_ARG, "%s: null pointer", name);
+  Arena t{tmp, tmp_bytes}, k{saved, saved_bytes};
+  const Operand qx = t.take(M, K), qgu = t.take(2 * F, K), qh = t.take(M, F), qd = t.take(N, F);
+  Operand xt{}, gut{}, ht{}, dt{};
+  if (need_dgu) xt = k.take(K, M);
+  if (need_dx) gut = k.take(K, 2 * F);
+  if (need_dd) ht = k.take(F, M);
+  if (back) dt = k.take(F, N);
+  if ((rc = quant_to(wd, d_dtype, N, F, ldd, &qd, back ? &dt : nullptr, nullptr, nullptr, stream)) ||
+      (rc = quant_to(wgu, gu_dtype, 2 * F, K, ldgu, &qgu, need_dx ? &gut : nullptr, nullptr, nullptr, stream)) ||
+      (rc = quant_to(x, x_dtype, M, K, ldx, &qx, need_dgu ? &xt : nullptr, nullptr, nullptr, stream)) ||
+      (rc = product(qx, qgu, nullptr, gu, FF_OUT_BF16, M, 2 * F, K, stream)) ||
+      (rc = ff_mxfp4_swiglu_quant(gu, 2 * F, M, F, mut(qh.q), qh.ld, mut(qh.s), need_dd ? mut(ht.q) : nullptr, ht.ld,
+                                  need_dd ? mut(ht.s) : nullptr, stream)))
+    return rc;
+  return product(qh, qd, nullptr, y, FF_OUT_BF16, M, N, F, stream);
+}
+
+extern "C" int ff_mxfp4_swiglu_bwd(const void* dy, int dtype, int64_t lddy, const void* gu, void* dh, const uint8_t* saved,
+                                   int64_t saved_bytes, int need_dx, int need_dgu, int need_dd, void* dx, int dx_kind,
+                                   void* dwgu, int gu_kind, void* dwd, int d_kind, int64_t M, int64_t K, int64_t F, int64_t N,
+                                   uint8_t* tmp, int64_t tmp_bytes, void* stream) {
+  using namespace ff::mxg;
+  const char* name = "ff_mxfp4_swiglu_bwd";
+  int rc;
+  const bool back = need_dx || need_dgu;
+  if ((rc = check_dims(name, M, N, K)) || (rc = check_dims(name, 2 * F, N, K)) ||
+      (rc = check_ws(name, "saved", saved, saved_bytes,
+                     (need_dgu ? part_bytes(K, M) : 0) + (need_dx ? part_bytes(K, 2 * F) : 0) + (need_dd ? part_bytes(F, M) : 0) +
+                         (back ? part_bytes(F, N) : 0))) ||
+      (rc = check_ws(name, "tmp", tmp, tmp_bytes,
+                     (back ? part_bytes(M, N) : 0) + (need_dd ? part_bytes(N, M) : 0) + (need_dx ? part_bytes(M, 2 * F) : 0) +
+                         (need_dgu ? part_bytes(2 * F, M) : 0))))
+    return rc;
+  FF_REQUIRE((!need_dx || (dx && float_kind(dx_kind))) && (!need_dgu || (dwgu && float_kind(gu_kind))) &&
+                 (!need_dd || (dwd && float_kind(d_kind))) && (!back || (gu && dh)),
+             FF_ERR_INVALID_ARG, "%s: null pointer or bad output kind", name);
+  Arena k{mut(saved), saved_bytes}, t{tmp, tmp_bytes};
+  Operand xt{}, gut{}, ht{}, dt{}, q{}, qt{}, p{}, pt{};
+  if (need_dgu) xt = k.take(K, M);
+  if (need_dx) gut = k.take(K, 2 * F);
+  if (need_dd) ht = k.take(F, M);
+  if (back) dt = k.take(F, N);
+  if (back) q = t.take(M, N);
+  if (need_dd) qt = t.take(N, M);
+  if (need_dx) p = t.take(M, 2 * F);
+  if (need_dgu) pt = t.take(2 * F, M);
+  if ((rc = quant_to(dy, dtype, M, N, lddy, back ? &q : nullptr, need_dd ? &qt : nullptr, nullptr, nullptr, stream))) return rc;
+  if (need_dd && (rc = product(qt, ht, nullptr, dwd, d_kind, N, F, M, stream))) return rc;
+  if (!back) return FF_OK;
+  if ((rc = product(q, dt, nullptr, dh, FF_OUT_BF16, M, F, N, stream)) ||
+      (rc = ff_mxfp4_swiglu_bwd_quant(dh, F, gu, 2 * F, M, F, need_dx ? mut(p.q) : nullptr, p.ld, need_dx ? mut(p.s) : nullptr,
+                                      need_dgu ? mut(pt.q) : nullptr, pt.ld, need_dgu ? mut(pt.s) : nullptr, stream)))
+    return rc;
+  if (need_dx && (rc = product(p, gut, nullptr, dx, dx_kind, M, K, 2 * F, stream))) return rc;
+  if (need_dgu && (rc = product(pt, xt, nullptr, dwgu, gu_kind, 2 * F, K, M, stream))) return rc;
+  return FF_OK;
+}

@@ -162,6 +162,12 @@ class MXFP4LinearFn(torch.autograd.Function):
         b = _bias(bias, O)
         ctx.dims, ctx.dtypes = (T, O, K), (x.dtype, None if packed is not None else weight.dtype,
                                            None if bias is None else bias.dtype)
+        ctx.whole = packed is None and T > 0 and O > 0
+        if ctx.whole:  # one call
+            ctx.had = need_dx, need_dw
+            y, saved = _capi.mxfp4_linear_train(_matrix(x, "x"), _matrix(weight, "weight"), b, need_dx, need_dw)
+            ctx.save_for_backward(saved)
+            return y
         if T == 0:
             ctx.save_for_backward(None, None, None, None)
             return torch.empty((0, O), dtype=torch.bfloat16, device=x.device)
@@ -181,6 +187,10 @@ class MXFP4LinearFn(torch.autograd.Function):
             return (torch.zeros((0, K), dtype=xd, device=dev) if need_dx else None,
                     torch.zeros((O, K), dtype=wd, device=dev) if need_dw else None,
                     torch.zeros((O,), dtype=bd, device=dev) if need_db else None, None, None)
+        if ctx.whole:
+            dx, dw, db = _capi.mxfp4_linear_bwd(_matrix(dy, "dy"), ctx.saved_tensors[0], ctx.dims, *ctx.had,
+                                                xd if need_dx else None, wd if need_dw else None, need_db)
+            return dx, dw, db.to(bd) if need_db else None, None, None
         qxt, sxt, qwt, swt = ctx.saved_tensors
         q, qt, db = _capi.mxfp4_quant(_matrix(dy, "dy"), rows=need_dx, cols=need_dw, colsum=need_db)
         dx = _product(q, (qwt, swt), T, K, O, None, xd) if need_dx else None
@@ -201,6 +211,13 @@ class MXFP4SwiGLUFn(torch.autograd.Function):
         need_dgu = need_dx or need_gu
         ctx.dims = (T, O, F, K)
         ctx.dtypes = (x.dtype, *(None if p is not None else w.dtype for p, w in zip(packed, (gate_up, down))))
+        ctx.whole = packed == (None, None) and need and T > 0 and O > 0
+        if ctx.whole:  # one call
+            ctx.need = need_dx, need_gu, need_d
+            y, gu, saved = _capi.mxfp4_swiglu_train(_matrix(x, "x"), _matrix(gate_up, "gate_up"), _matrix(down, "down"),
+                                                    need_dx, need_gu, need_d)
+            ctx.save_for_backward(gu if need_dgu else None, saved)
+            return y
         if T == 0:
             ctx.save_for_backward(*(None,) * 9)
             return torch.empty((0, O), dtype=torch.bfloat16, device=x.device)
@@ -228,6 +245,10 @@ class MXFP4SwiGLUFn(torch.autograd.Function):
             return (torch.zeros((0, K), dtype=xd, device=dev) if need_dx else None,
                     torch.zeros((2 * F, K), dtype=gud, device=dev) if need_gu else None,
                     torch.zeros((O, F), dtype=dd, device=dev) if need_d else None, None, None)
+        if ctx.whole:
+            gu, saved = ctx.saved_tensors
+            types = (t if n else None for t, n in zip((xd, gud, dd), ctx.need))
+            return *_capi.mxfp4_swiglu_bwd(_matrix(dy, "dy"), gu, saved, (T, K, F, O), *types), None, None
         gu, qxt, sxt, qht, sht, qgut, sgut, qdt, sdt = ctx.saved_tensors
         q, qt, _ = _capi.mxfp4_quant(_matrix(dy, "dy"), rows=need_dx or need_gu, cols=need_d)
         dx = dgu = dd_ = None

@@ -593,6 +593,32 @@ FF_API int ff_mxfp4_swiglu_mlp(const void* x, int dtype, int64_t ldx, const uint
                                int64_t ws_bytes, void* stream);
 
 /*
+ * A training step's forward and backward pass in one call each, weights in floating point.  Linear layer:
+ * y = Q(x) Q(w)^T + bias (bf16); dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, db = column sums of dy (any of them
+ * NULL).  SwiGLU block (F a multiple of 32): gu = Q(x) Q(wgu)^T (bf16 [M, 2F], kept by the caller),
+ * y = Q(h) Q(wd)^T; dh (bf16 [M, F]) is scratch.  All outputs are contiguous; *_kind: FF_OUT_BF16 or FF_OUT_F32.
+ * With P(r, c) = ff_mxfp4_linear_ws_bytes(r, c), `saved` has, in this order and as far as needed,
+ *   linear: P(K, M) for dw, P(K, N) for dx;
+ *   block:  P(K, M) for dwgu, P(K, 2F) for dx, P(F, M) for dwd, P(F, N) for dx or dwgu;
+ * and tmp has  P(M, K) + P(N, K);  P(M, N) for dx + P(N, M) for dw or db + 4 ff_mxfp4_colsum_ws_elems(M, N) (in 16s) for db;
+ *   P(M, K) + P(2F, K) + P(M, F) + P(N, F);  P(M, N) for dx or dwgu + P(N, M) for dwd + P(M, 2F) for dx + P(2F, M) for dwgu.
+ */
+FF_API int ff_mxfp4_linear_train(const void* x, int x_dtype, int64_t ldx, const void* w, int w_dtype, int64_t ldw,
+                                 const float* bias, void* y, int64_t M, int64_t N, int64_t K, int need_dx, int need_dw,
+                                 uint8_t* tmp, int64_t tmp_bytes, uint8_t* saved, int64_t saved_bytes, void* stream);
+FF_API int ff_mxfp4_linear_bwd(const void* dy, int dtype, int64_t lddy, const uint8_t* saved, int64_t saved_bytes,
+                               int saved_dx, int saved_dw, void* dx, int dx_kind, void* dw, int dw_kind, float* db,
+                               int64_t M, int64_t N, int64_t K, uint8_t* tmp, int64_t tmp_bytes, void* stream);
+FF_API int ff_mxfp4_swiglu_train(const void* x, int x_dtype, int64_t ldx, const void* wgu, int gu_dtype, int64_t ldgu,
+                                 const void* wd, int d_dtype, int64_t ldd, void* gu, void* y, int64_t M, int64_t K,
+                                 int64_t F, int64_t N, int need_dx, int need_dgu, int need_dd, uint8_t* tmp,
+                                 int64_t tmp_bytes, uint8_t* saved, int64_t saved_bytes, void* stream);
+FF_API int ff_mxfp4_swiglu_bwd(const void* dy, int dtype, int64_t lddy, const void* gu, void* dh, const uint8_t* saved,
+                               int64_t saved_bytes, int need_dx, int need_dgu, int need_dd, void* dx, int dx_kind,
+                               void* dwgu, int gu_kind, void* dwd, int d_kind, int64_t M, int64_t K, int64_t F,
+                               int64_t N, uint8_t* tmp, int64_t tmp_bytes, void* stream);
+
+/*
  * Distillation loss from a teacher's top logits (the reference has no counterpart).  Row r: student
  * logits s [vocab]; `top` entries (token id, teacher logit t), an entry with a negative id or t = -inf
  * being absent; optionally a label and the teacher's log-sum-exp of its logits / T.
