@@ -545,41 +545,43 @@ __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* q, int64
   if (c >= cols) return;
   constexpr int R = 4;
   for (int64_t r0 = ((int64_t)blockIdx.y * blockDim.y + threadIdx.y) * R; r0 < rows; r0 += (int64_t)gridDim.y * blockDim.y * R) {
-    uint32_t w[R];
-    float sv[R];
+    const int live = (int)min64(R, rows - r0);
+    const uint8_t* qr = q + r0 * ldq + c / 2;
+    const uint8_t* sr = s + scale_at(r0, c / BLOCK, chunks);  // the next three rows' scales follow 16 bytes apart
+    T* o = reinterpret_cast<T*>(out) + r0 * ldo + c;
+    uint32_t w[R], S[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int64_t r = min64(r0 + i, rows - 1);
-      w[i] = __ldg(reinterpret_cast<const uint32_t*>(q + r * ldq + c / 2));
-      sv[i] = scale_value(__ldg(s + scale_at(r, c / BLOCK, chunks)));
+      w[i] = i < live ? __ldg(reinterpret_cast<const uint32_t*>(qr + i * ldq)) : 0u;
+      S[i] = i < live ? __ldg(sr + i * 16) : 0u;
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      if (r0 + i >= rows) break;
+      if (i >= live) break;
       alignas(16) T t[8];
+      const float sv = scale_value(S[i]);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 p = values2((w[i] >> (8 * k)) & 0xFFu);
-        const float a = p.x * sv[i], b = p.y * sv[i];
         if constexpr (DT == FF_DTYPE_F32) {
-          t[2 * k] = a;
-          t[2 * k + 1] = b;
+          t[2 * k] = p.x * sv;
+          t[2 * k + 1] = p.y * sv;
         } else if constexpr (DT == FF_DTYPE_BF16) {
-          reinterpret_cast<uint32_t*>(t)[k] = pack_bf16x2(mk2(a, b));
+          reinterpret_cast<uint32_t*>(t)[k] = pack_bf16x2(mul2(mk2(p.x, p.y), splat(sv)));
         } else {
-          t[2 * k] = __float2half_rn(a);
-          t[2 * k + 1] = __float2half_rn(b);
+          t[2 * k] = __float2half_rn(p.x * sv);
+          t[2 * k + 1] = __float2half_rn(p.y * sv);
         }
       }
-      T* o = reinterpret_cast<T*>(out) + (r0 + i) * ldo + c;
+      T* d = o + i * ldo;
       if (vec && c + 8 <= cols) {
 #pragma unroll
         for (int k = 0; k < (int)(8 * sizeof(T) / 16); ++k)
-          reinterpret_cast<uint4*>(o)[k] = reinterpret_cast<const uint4*>(t)[k];
+          reinterpret_cast<uint4*>(d)[k] = reinterpret_cast<const uint4*>(t)[k];
       } else {
 #pragma unroll
         for (int k = 0; k < 8; ++k)
-          if (c + k < cols) o[k] = t[k];
+          if (c + k < cols) d[k] = t[k];
       }
     }
   }
