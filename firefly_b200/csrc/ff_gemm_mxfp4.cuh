@@ -107,7 +107,11 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
 // so the result does not depend on timing and no workspace is needed.  Two barriers per CTA and buffer
 // order the exchange: `pfull` (every CTA's partial sums are written) and `pfree` (every CTA has read
 // them).  Where two buffers fit, an item's sums are added up after the next item's have been written,
-// so that a CTA does not stand still for the others' arrival.
+// so that a CTA does not stand still for the others' arrival.  1x4096x22016: 17 us (48 MB; 15 us of it after
+// the quantiser, with which it overlaps); 33x11008x4096: 13 us.  One SM's copies bring a k-block in 0.45 us
+// (38 GB/s, the same with half the products or without the scale copies), so 148 SMs at work all the time would take
+// 8.6 us; launch, TMEM, the first load's latency and the last exchange are about 5 us, the rest is SMs
+// without an item.
 // ---------------------------------------------------------------------------
 __host__ __device__ constexpr int nr_stage_bytes(int mp, int nw) { return nw * (ROWS_BYTES + SF_BYTES) + mp * 128 + SF_BYTES; }
 __host__ __device__ constexpr int nr_bufs(int mp, int nw) { return nw * mp <= 64 ? 2 : 1; }
@@ -493,9 +497,11 @@ __global__ void __launch_bounds__(NR_THREADS, 1)
 // The scale copies are issued by a warp of their own.  In one thread's order copies and products do not
 // overlap (8192x4096x11008: 195 us with a k-block's six copies ahead of its products, 8 us for each of the
 // six, and no gain from copying earlier; 268 us with four warps writing the scales by tcgen05.st); issued
-// from two warps, with a commit and a barrier between them, they do: 144 us = 5.1 PFLOP/s, within 2% of
-// the time without any copies.  What is left is the fill of shared memory: 35 KB per k-block and CTA,
-// 10.8 TB/s over all SMs.
+// from two warps, with a commit and a barrier between them, they do: 144 us, within 2% of the time without
+// any copies.  A last wave of tiles that at most half fills the GPU is cut into 256 x 128 halves.
+// 8192x4096x11008 now 131 us = 5.6 PFLOP/s (22016x4096x8192 262 us, 8192x8192x2048 72 us = 3.8): the tensor
+// pipe is active 69% of the cycles, and the SM clock falls to 1.64 GHz under it; K = 2048 leaves eight
+// k-blocks per tile, over which the start of a tile (its accumulator's shared half has to be read) weighs.
 // ---------------------------------------------------------------------------
 constexpr int PR_STAGES = 5;
 constexpr int PR_CODES = 2 * ROWS_BYTES;                 // 128 rows of A and of B

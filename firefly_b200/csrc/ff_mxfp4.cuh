@@ -327,8 +327,8 @@ __host__ __device__ constexpr int quant_smem() {
   return TILE * row_bytes<DT>() + TILE * 4 + 4 * TILE * 4;
 }
 
-// One 128 x 128 tile per CTA: read once, quantised along either axis or both from shared memory.
-// Bound by HBM: 2 bytes read and 17/32 byte written per value and orientation.
+// One 128 x 128 tile per CTA: read once, quantised along either axis or both from shared memory (fp32
+// inputs, few tiles, unaligned rows).  fp32 8192 x 4096, both orientations: 49 us, 3.5 TB/s.
 template <int DT>
 __global__ void __launch_bounds__(THREADS, DT == FF_DTYPE_F32 ? 2 : 4) mx_quant_kernel(const void* x, int64_t ldx, int64_t tiles_c, Out o, int vec) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -343,7 +343,9 @@ __global__ void __launch_bounds__(THREADS, DT == FF_DTYPE_F32 ? 2 : 4) mx_quant_
 
 // The same for 16-bit inputs whose rows are 16-byte aligned: persistent CTAs, three per SM, each with two
 // tile buffers, so that the next tile arrives (cp.async) while one is quantised.
-// 8192 x 4096 bf16, both orientations: ... us (... us with one tile per CTA).
+// 8192 x 4096 bf16, both orientations: 27 us with 3.8 TB/s of algorithmic bytes (30 us with one tile per CTA; a
+// copy of as many bytes takes 18 us); along the rows alone 21 us.  Instruction issue bounds it: 14.8 instructions
+// per value for both orientations, the ALU pipe 63% busy.
 template <int DT>
 __host__ __device__ constexpr int pipe_smem() {
   return 2 * TILE * row_bytes<DT>() + TILE * 4 + 4 * TILE * 4;
@@ -413,7 +415,9 @@ __device__ __forceinline__ uint32_t swiglu_word(uint32_t wg, uint32_t wu) {
 }
 
 // h = bf16(silu(g) * u) of the bf16 gate/up activations gu = [g | u], quantised like mx_quant_kernel;
-// h itself is not written.
+// h itself is not written.  All 16 pieces of a thread are in flight before the first is used, three CTAs per
+// SM: 8192 x 11008 97 us, 4.7 TB/s (127 us with addresses worked out per piece); bound by instruction issue
+// (22 per value) and the latency of a tile's loads.
 __global__ void __launch_bounds__(THREADS, 3) mx_swiglu_quant_kernel(const __nv_bfloat16* gu, int64_t ld, int64_t F,
                                                                   int64_t tiles_c, Out o) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -453,7 +457,8 @@ __device__ __forceinline__ void swiglu_bwd_word(uint32_t wg, uint32_t wu, uint32
 
 // The gradient of gu from dh and gu (all bf16), quantised as the matrix [dg | du] of 2F columns
 // without being written:  dg = bf16(dh * u * sig(g) * (1 + g * (1 - sig(g)))),  du = bf16(dh * g * sig(g)).
-// One CTA takes the same 128 features of dg and of du.
+// One CTA takes the same 128 features of dg and of du.  8192 x 11008: 171 us, 4.2 TB/s; bound like the forward
+// kernel, at 38 instructions per value of dh.
 __global__ void __launch_bounds__(THREADS, 2) mx_swiglu_bwd_quant_kernel(const __nv_bfloat16* dh, int64_t lddh,
                                                                       const __nv_bfloat16* gu, int64_t ld, int64_t F,
                                                                       int64_t tiles_c, Out o) {
@@ -536,7 +541,8 @@ __global__ void __launch_bounds__(256) mx_colsum_kernel(const float* part, int64
 }
 
 // Eight values per thread and row: one word of codes -> 16 (or 32) bytes.  blockDim.x threads side by side
-// in a row, four rows per thread in flight.
+// in a row, four rows per thread in flight.  8192 x 4096 to bf16: 17.6 us, 4.8 TB/s; a copy of as many bytes takes
+// as long.
 template <int DT>
 __global__ void __launch_bounds__(256) mx_dequant_kernel(const uint8_t* q, int64_t ldq, const uint8_t* s, int chunks, int64_t rows,
                                                          int cols, void* out, int64_t ldo, int vec) {
