@@ -2,7 +2,8 @@
 
 Drop-in for the reference package's public API (fumitoshi0524/FireFly
 ``__init__.py:1-10``): ``BitLinear``, ``FireFlyOptim``,
-``collect_bitlinear_modules``, ``quantize_fp_to_int8``.  The compute runs in
+``collect_bitlinear_modules``, ``quantize_fp_to_int8``.  Beside it, new here: MXFP4 layers
+(``mxfp4``) and a distillation loss (``distill``).  The compute runs in
 libfirefly_b200.so (hand-written sm_100a kernels) through a C ABI
 (``include/firefly_b200.h``).
 """

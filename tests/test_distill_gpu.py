@@ -366,3 +366,41 @@ def test_decoder_distils_from_a_teacher():
         assert g is not None and torch.isfinite(g).all() and bool(g.any())
     for p in student.dense_parameters():
         assert p.grad is not None and torch.isfinite(p.grad).all()
+
+
+def test_more_than_2_31_logits():
+    """Offsets past 32 bits: the last rows of a long batch against the same rows by themselves."""
+    n, V, k = 68000, 32000, 8
+    s = torch.empty(n, V, device=DEV, dtype=torch.bfloat16)
+    s.normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    ids = torch.randint(0, V, (n, k), device=DEV)
+    t = torch.randn(n, k, device=DEV)
+    x = s.requires_grad_(True)
+    distillation_loss(x, ids, t, reduction="sum").backward()
+    y = s.detach()[-5:].clone().requires_grad_(True)
+    distillation_loss(y, ids[-5:], t[-5:], reduction="sum").backward()
+    # another cut of the row into slices: other sums, the same up to their rounding and the output's
+    assert bool(((x.grad[-5:].float() - y.grad.float()).abs() <= 2.0 ** -7 * y.grad.float().abs() + 1e-9).all())
+    with torch.no_grad():
+        rows = distillation_loss(s, ids, t, reduction="none")
+        want = distillation_loss(s[-5:].clone(), ids[-5:], t[-5:], reduction="none")
+    assert bool(((rows[-5:] - want).abs() <= 2.0 ** -19 * 32).all())
+
+
+@pytest.mark.parametrize("T", [1e-2, 1e4])
+def test_extreme_temperatures(T):
+    s, ids, t, lab, _ = _case(6, 900, 10, 30, labels=True)
+    x = s.clone().requires_grad_(True)
+    l = distillation_loss(x, ids, t, lab, temperature=T, alpha=0.5)
+    s64 = s.double().requires_grad_(True)
+    rows, counted, scale = O.losses(s64, ids, t, lab, None, T, 0.5)
+    want = rows.sum() / sum(counted)
+    want.backward()
+    tol = 2.0 ** -19 * float((T * T * (4 + scale) + 16).sum()) / sum(counted)
+    assert abs(float(l.detach()) - float(want.detach())) <= tol
+    l.backward()
+    assert torch.isfinite(x.grad).all()
+    # the exponential's argument is rounded to 2^-24 of itself, |s| / T log2 e
+    arg = float(s.abs().max()) / T * 1.5
+    lim = (2.0 ** -18 + 2.0 ** -23 * arg) * 4 * max(T, 1.0) + 2.0 ** -8 * float(s64.grad.abs().max())
+    assert float((x.grad.double() - s64.grad).abs().max()) <= lim

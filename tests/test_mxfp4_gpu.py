@@ -465,3 +465,72 @@ def test_teacher_in_four_bits_distils_a_student():
     assert bool(((hidden.grad.double() - v).abs() <= _tolerance(v, mag, V, torch.bfloat16)).all())
     for w in (wgu, wd):
         assert torch.isfinite(w.grad).all() and bool(w.grad.any())
+
+
+def test_more_than_2_31_elements():
+    """Offsets past 32 bits: the last rows of large matrices against the same rows by themselves."""
+    x = torch.empty(540000, 4096, device=DEV, dtype=torch.bfloat16)
+    x.normal_(generator=_gen(1))
+    q, qt = quantize_fp_to_mxfp4_dual(x)
+    _check_values(quantize_fp_to_mxfp4(x[-130:]), x[-130:])
+    assert torch.equal(q.codes[-130:], quantize_fp_to_mxfp4(x[-130:]).codes)
+    tail = x[-256:].t().contiguous()  # 540000 is a multiple of 32: the last 256 rows are whole blocks
+    assert torch.equal(qt.codes[:, -128:], quantize_fp_to_mxfp4(tail).codes)
+    back = q.dequantize()
+    assert torch.equal(back[-130:].double(), O.values(x[-130:]))
+    del back, qt, q, x
+    a, b = _randn(70000, 64, 2), _randn(33000, 64, 3)
+    y = mxfp4_matmul(quantize_fp_to_mxfp4(a), quantize_fp_to_mxfp4(b))
+    assert y.numel() > 2 ** 31
+    _check_product(y[-70:], O.values(a)[-70:], O.values(b))
+    _check_product(y[35000:35070], O.values(a)[35000:35070], O.values(b))
+
+
+def test_the_smallest_products():
+    for M, N, K in ((1, 1, 1), (1, 1, 33), (2, 3, 5), (300, 1, 1), (1, 300, 2)):
+        a, b = _randn(M, K, 1), _randn(N, K, 2)
+        _check_product(mxfp4_matmul(quantize_fp_to_mxfp4(a), quantize_fp_to_mxfp4(b), out_dtype=torch.float32), O.values(a),
+                       O.values(b))
+
+
+def test_gradients_through_a_broadcast_and_a_reused_input():
+    """One input in two layers, its gradient the sum; an expanded upstream gradient (stride 0)."""
+    x = _randn(40, 128, 1).requires_grad_(True)
+    w1, w2 = _randn(64, 128, 2), _randn(64, 128, 3)
+    (mxfp4_linear(x, w1) + mxfp4_linear(x, w2)).sum().backward()
+    ones = torch.ones(40, 64, device=DEV, dtype=torch.bfloat16)
+    got = x.grad.clone()
+    parts = []
+    for w in (w1, w2):
+        y = x.detach().clone().requires_grad_(True)
+        mxfp4_linear(y, w).backward(ones)
+        parts.append(y.grad)
+    assert torch.equal(got, parts[0] + parts[1]) or torch.equal(got, parts[1] + parts[0])
+
+
+def test_training_step_captured_and_replayed():
+    x = _randn(64, 256, 1).requires_grad_(True)
+    wgu, wd = _randn(512, 256, 2, scale=0.05).requires_grad_(True), _randn(128, 256, 3, scale=0.05).requires_grad_(True)
+    dy = _randn(64, 128, 4)
+
+    def step():
+        y = mxfp4_swiglu(x, wgu, wd)
+        return (y.detach(), *torch.autograd.grad(y, [x, wgu, wd], dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for k in (1, 2):
+        with torch.no_grad():
+            x.mul_(1.5)
+            wgu.add_(0.01 * k)
+            dy.mul_(0.75)
+        g.replay()
+        got = [t.clone() for t in out]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
