@@ -494,11 +494,12 @@ __global__ void __launch_bounds__(NR_THREADS, 1)
 // columns (the scales of one k-block: 8 of A, 16 of B) from column 384 on, so a slot is free as soon as
 // its stage is loaded again.
 //
-// The scale copies are issued by a warp of their own.  In one thread's order copies and products do not
+// The scale copies are issued by two warps of their own.  In one thread's order copies and products do not
 // overlap (8192x4096x11008: 195 us with a k-block's six copies ahead of its products, 8 us for each of the
 // six, and no gain from copying earlier; 268 us with four warps writing the scales by tcgen05.st); issued
-// from two warps, with a commit and a barrier between them, they do: 144 us, within 2% of the time without
-// any copies.  A last wave of tiles that at most half fills the GPU is cut into 256 x 128 halves.
+// by another warp, with a commit and a barrier between, they do: 144 us, within 2% of the time without
+// any copies.  Two copy warps with half of a stage's copies each: 1 to 3% less than one (measured in turn:
+// 22016x4096x8192 268 -> 262 us, 8192x2048x8192 63.5 -> 61.5, 4000x12288x4096 94.2 -> 92.1).  A last wave of tiles that at most half fills the GPU is cut into 256 x 128 halves.
 // 8192x4096x11008 now 131 us = 5.6 PFLOP/s (22016x4096x8192 262 us, 8192x8192x2048 72 us = 3.8): the tensor
 // pipe is active 69% of the cycles, and the SM clock falls to 1.64 GHz under it; K = 2048 leaves eight
 // k-blocks per tile, over which the start of a tile (its accumulator's shared half has to be read) weighs.
@@ -507,7 +508,8 @@ constexpr int PR_STAGES = 5;
 constexpr int PR_CODES = 2 * ROWS_BYTES;                 // 128 rows of A and of B
 constexpr int PR_STAGE = PR_CODES + 3 * SF_BYTES;        // and the scales of A (128 rows) and B (256 rows)
 constexpr int PR_EPI_WARPS = 8;
-constexpr int PR_THREADS = 64 + 32 * PR_EPI_WARPS + 32;  // TMA, MMA, epilogue, scale copies
+constexpr int PR_CP_WARPS = 2;
+constexpr int PR_THREADS = 64 + 32 * (PR_EPI_WARPS + PR_CP_WARPS);  // TMA, MMA, epilogue, scale copies
 constexpr int PR_ACC1 = 128, PR_SF = 384, PR_SF_COLS = 24;
 static_assert(PR_SF + PR_STAGES * PR_SF_COLS <= 512, "TMEM columns");
 constexpr int PR_STAGING = PR_EPI_WARPS * 2 * 2048;      // two 32 x 32 bf16 boxes per epilogue warp
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
     for (int s = 0; s < ST; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
-      mbar_init(sf_ready(s), 1);
+      mbar_init(sf_ready(s), PR_CP_WARPS);
     }
     mbar_init(tfull_bar(0), 1);
     mbar_init(tfull_bar(1), 1);
@@ -695,22 +697,22 @@ __global__ void __launch_bounds__(PR_THREADS, 1)
       drain_bar(drain, 0);
     }
     __syncwarp();
-  } else if (warp == 2 + PR_EPI_WARPS) {
+  } else if (warp >= 2 + PR_EPI_WARPS) {
     // ------------------------------------------------------------ scales into TMEM (leader only)
+    // Each of the two warps copies half of every stage's scales.  Both wait for every phase of every stage's
+    // barrier, in order, and the product of a stage waits for both, so no phase can pass either of them by.
     if (rank == 0 && lane == 0) {
       const uint32_t steps = num_items * (uint32_t)num_kb;
+      const uint32_t c = (uint32_t)(warp - 2 - PR_EPI_WARPS);
       int s = 0;
       uint32_t phase = 0, g = 0;
       for (; g < steps; ++g) {
         if (!wait_bar(full_bar(s), phase, abort_flag)) break;
         tc_fence_after();
         const uint32_t sf = tmem + PR_SF + (uint32_t)(s * PR_SF_COLS);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          sf_copy<2>(sf + c * 4, sSA(s) + c * 512);
-          sf_copy<2>(sf + 8 + c * 8, sSB(s, 0) + c * 512);
-          sf_copy<2>(sf + 8 + c * 8 + 4, sSB(s, 1) + c * 512);
-        }
+        sf_copy<2>(sf + c * 4, sSA(s) + c * 512);
+        sf_copy<2>(sf + 8 + c * 8, sSB(s, 0) + c * 512);
+        sf_copy<2>(sf + 8 + c * 8 + 4, sSB(s, 1) + c * 512);
         asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(sf_ready(s)) : "memory");
         if (++s == ST) {
           s = 0;
