@@ -949,7 +949,8 @@ inline int launch_pair(const Operand& a, const Operand& b, int64_t K, Epi ep, in
   if ((rc = make_map_sf(&tsa, a.s, ep.M, K))) return rc;
   if ((rc = make_map_codes(&tb, b.q, brows, K, b.ld, 128))) return rc;
   if ((rc = make_map_sf(&tsb, b.s, brows, K))) return rc;
-  ep.tma_store = !GATED && !ep.out_f32 && ep.vec;
+  // whole 16-byte pieces only: a tile store clipped at an odd column was seen to write a zero behind it
+  ep.tma_store = !GATED && !ep.out_f32 && ep.vec && ep.N % 8 == 0;
   if (ep.tma_store && (rc = make_map_out_bf16(&td, ep.D, ep.M, ep.N, ep.ldd, true))) return rc;
   const int tiles_m = (int)((ep.M + 255) / 256), tiles_n = (int)(GATED ? ep.F / 128 : (ep.N + 255) / 256);
   const int total = tiles_m * tiles_n, pairs = min(total, max_pairs), rest = total % pairs;

@@ -112,6 +112,24 @@ def test_dequantize_types(dtype):
     torch.testing.assert_close(got, O.values(x).to(dtype), rtol=0, atol=0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r,c,ld", [(1, 1, 1), (5, 264, 264), (9, 4095, 4095), (31, 257, 300), (300, 1001, 1001),
+                                    (130, 2056, 2056), (67, 520, 523)])
+def test_dequantize_writes_its_columns_only(r, c, ld, dtype):
+    """Rows of any alignment, through the C entry: what lies between and behind them stays."""
+    x = _randn(r, c, 21, scale=0.1)
+    q = quantize_fp_to_mxfp4(x)
+    buf = torch.full((r * ld + 40,), 7.0, dtype=dtype, device=DEV)
+    for skip in (0, 1):
+        buf.fill_(7.0)
+        codes, scales = q._pair()
+        _capi._call("ff_mxfp4_dequant", _capi._addr(codes), codes.shape[1], _capi._addr(scales), r, c,
+                    buf.data_ptr() + skip * buf.element_size(), _capi._dtype_code(dtype), ld, _capi._raw_stream(x.device))
+        view = buf[skip:skip + r * ld].view(r, ld)
+        torch.testing.assert_close(view[:, :c], O.values(x).to(dtype), rtol=0, atol=0)
+        assert bool((view[:, c:] == 7).all()) and bool((buf[:skip] == 7).all()) and bool((buf[skip + r * ld:] == 7).all())
+
+
 def _tolerance(v, mag, K, dtype):
     """fp32 accumulation of ceil(K / 32) scaled block sums, each step off by at most 2^-23 of the sum of
     magnitudes (a truncating adder), then one rounding of the output."""
@@ -144,6 +162,25 @@ def test_product_against_fp64(M, N, K, out):
     got = mxfp4_matmul(quantize_fp_to_mxfp4(a), quantize_fp_to_mxfp4(b), bias, out_dtype=out)
     assert got.shape == (M, N) and got.dtype == out
     _check_product(got, O.values(a), O.values(b), bias)
+    assert _capi.device_status() == 0
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("M,N,K,ld", [(300, 400, 512, 400), (300, 401, 512, 401), (700, 1025, 256, 1030), (1500, 2047, 288, 2048)])
+def test_product_writes_its_columns_only(M, N, K, ld, out):
+    a, b = _randn(M, K, 1), _randn(N, K, 2, scale=0.02)
+    qa, qb = quantize_fp_to_mxfp4(a), quantize_fp_to_mxfp4(b)
+    want = mxfp4_matmul(qa, qb, None, out_dtype=out)
+    _check_product(want, O.values(a), O.values(b))
+    for skip in (0, 1):
+        buf = torch.full((M * ld + 40,), 7.0, dtype=out, device=DEV)
+        (ca, sa), (cb, sb) = qa._pair(), qb._pair()
+        _capi._call("ff_mxfp4_gemm", ca.data_ptr(), ca.shape[1], sa.data_ptr(), cb.data_ptr(), cb.shape[1], sb.data_ptr(),
+                    None, buf.data_ptr() + skip * buf.element_size(), ld,
+                    _capi.FF_OUT_F32 if out == torch.float32 else _capi.FF_OUT_BF16, M, N, K, _capi._raw_stream(a.device))
+        view = buf[skip:skip + M * ld].view(M, ld)
+        assert torch.equal(view[:, :N], want)
+        assert bool((view[:, N:] == 7).all()) and bool((buf[:skip] == 7).all()) and bool((buf[skip + M * ld:] == 7).all())
     assert _capi.device_status() == 0
 
 
