@@ -1760,7 +1760,9 @@ inline int gemm_dispatch(const char* name, const int8_t* A, int64_t lda, const i
     const int t2m = (int)((M + 2 * C2_BM - 1) / (2 * C2_BM)), t2n = (int)((N + C2_BN - 1) / C2_BN);
     CUtensorMap md;
     memset(&md, 0, sizeof(md));
-    if (out_kind == FF_OUT_BF16 && ep.vec) {  // 16-byte aligned output rows: TMA tile stores
+    // 16-byte aligned output rows of whole 16-byte pieces: TMA tile stores (clipped at an odd column, one was
+    // seen to write a zero behind it)
+    if (out_kind == FF_OUT_BF16 && ep.vec && N % 8 == 0) {
       rc = make_map_out_bf16(&md, D, M, N, ldd, true);
       if (rc) return rc;
       ep.tma_store = 1;

@@ -498,11 +498,12 @@ __global__ void __launch_bounds__(NR_THREADS, 1)
 // overlap (8192x4096x11008: 195 us with a k-block's six copies ahead of its products, 8 us for each of the
 // six, and no gain from copying earlier; 268 us with four warps writing the scales by tcgen05.st); issued
 // by another warp, with a commit and a barrier between, they do: 144 us, within 2% of the time without
-// any copies.  Two copy warps with half of a stage's copies each: 1 to 3% less than one (measured in turn:
-// 22016x4096x8192 268 -> 262 us, 8192x2048x8192 63.5 -> 61.5, 4000x12288x4096 94.2 -> 92.1).  A last wave of tiles that at most half fills the GPU is cut into 256 x 128 halves.
-// 8192x4096x11008 now 131 us = 5.6 PFLOP/s (22016x4096x8192 262 us, 8192x8192x2048 72 us = 3.8): the tensor
-// pipe is active 69% of the cycles, and the SM clock falls to 1.64 GHz under it; K = 2048 leaves eight
-// k-blocks per tile, over which the start of a tile (its accumulator's shared half has to be read) weighs.
+// any copies.  Two copy warps with half of a stage's copies each take 1 to 3% less than one (timed in turn, L2
+// cold: 22016x4096x8192 268 -> 262 us = 5.6 PFLOP/s, 8192x2048x8192 63.5 -> 61.5, 4000x12288x4096 94.2 -> 92.1;
+// 8192x4096x11008 136 us = 5.4, 8192x8192x2048 78 us = 3.5).  A last wave of tiles that at most half fills the
+// GPU is cut into 256 x 128 halves.  The tensor pipe is active 69% of the cycles (with one copy warp), and the SM
+// clock falls to 1.64 GHz under it; K = 2048 leaves eight k-blocks per tile, over which the start of a tile (its
+// accumulator's shared half has to be read) weighs.
 // ---------------------------------------------------------------------------
 constexpr int PR_STAGES = 5;
 constexpr int PR_CODES = 2 * ROWS_BYTES;                 // 128 rows of A and of B

@@ -188,3 +188,14 @@ def test_skinny_split_k_equals_oracle_and_leaves_workspace_zero(M, N, K):
         if kind == _capi.FF_OUT_S32:
             np.testing.assert_array_equal(got.cpu().numpy().astype(np.int64), want)
     assert _capi.device_status() == 0
+
+
+@pytest.mark.parametrize("M,N,K,ld", [(2600, 2599, 1000, 2600), (2304, 2559, 512, 2568), (300, 401, 512, 408)])
+def test_gemm_bf16_leaves_the_padding_columns(M, N, K, ld):
+    g = torch.Generator(device="cuda").manual_seed(5)
+    a = torch.randint(-127, 128, (M, (K + 15) // 16 * 16), device="cuda", dtype=torch.int8, generator=g)
+    b = torch.randint(-127, 128, (N, (K + 15) // 16 * 16), device="cuda", dtype=torch.int8, generator=g)
+    buf = torch.full((M, ld), 7.0, dtype=torch.bfloat16, device="cuda")
+    _capi.gemm_i8(a, b, K, out=buf[:, :N])
+    assert torch.equal(buf[:, :N], _capi.gemm_i8(a, b, K))
+    assert bool((buf[:, N:] == 7).all())
