@@ -1,4 +1,4 @@
-"""Distillation loss from a teacher's top logits in fp64, one row at a time: the checker of the kernel."""
+"""Distillation loss from a teacher's top logits in fp64, one row at a time: the oracle of the kernel."""
 from __future__ import annotations
 
 import math

@@ -1,4 +1,4 @@
-"""MXFP4 in fp64 torch operations: the checker of the 4-bit kernels.
+"""MXFP4 in fp64 torch operations: the oracle of the 4-bit kernels.
 
 Format: 32 consecutive values of a row share the scale 2^max(floor(log2 A) - 2, -127), A their largest
 magnitude; a value is the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 times the scale (ties to the code whose
