@@ -41,6 +41,7 @@ SIGNATURES = {
     "ff_last_error": (ctypes.c_char_p, []),
     "ff_num_sms": (_I, [_P]),
     "ff_device_status": (_I, [_P, _I]),
+    "ff_capture_id": (_I, [_P, _P]),
     "ff_quant_rows_i8": (_I, [_P, _I, _I64, _I64, _I64, _P, _F, _P, _I64, _P, _P]),
     "ff_quant_dual_i8": (_I, [_P, _I, _I64, _I64, _I64, _P, _F, _P, _I64, _P, _P, _I64, _P, _P, _P]),
     "ff_quant_dual_i8_noalloc": (_I, [_P, _I, _I64, _I64, _I64, _P, _F, _P, _I64, _P, _P, _I64, _P, _P]),
@@ -220,6 +221,16 @@ def _addr(t: torch.Tensor | None):
 def _raw_stream(dev: torch.device) -> int:
     """torch's current stream of ``dev`` as an address."""
     return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def capture_id(dev: torch.device) -> int:
+    """The id of the graph capture under way on torch's current stream of ``dev``, 0 if there is none."""
+    with _OnDevice(dev):
+        if not torch.cuda.is_current_stream_capturing():
+            return 0
+        out = ctypes.c_uint64(0)
+        _call("ff_capture_id", ctypes.byref(out), _raw_stream(dev))
+        return out.value
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
@@ -1048,14 +1059,14 @@ def distill_loss(rows: DistillRows, logits: torch.Tensor, reduction: str, grad: 
 
 def distill_grad(rows: DistillRows, logits: torch.Tensor, reduction: str, upstream: torch.Tensor,
                  counts: torch.Tensor | None, grad: torch.Tensor | None = None, held: torch.Tensor | None = None,
-                 keep_held: bool = False) -> torch.Tensor:
+                 replayed: bool = False) -> torch.Tensor:
     """The gradient for ``upstream`` (fp32 scalar, or one per row), into ``grad`` when it holds the
-    gradient for ``held`` already."""
+    gradient for ``held`` already.  ``replayed``: the call is captured."""
     dev = logits.device
     if grad is None:
         grad, held = torch.empty(tuple(logits.shape), dtype=logits.dtype, device=dev), None
     with _OnDevice(dev):
-        _call("ff_distill_grad", ctypes.byref(rows), FF_REDUCE[reduction], _addr(upstream), _addr(held), int(keep_held),
+        _call("ff_distill_grad", ctypes.byref(rows), FF_REDUCE[reduction], _addr(upstream), _addr(held), int(replayed),
               _addr(counts), _addr(grad), logits.shape[1], _raw_stream(dev))
     return grad
 

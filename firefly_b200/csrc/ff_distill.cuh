@@ -717,7 +717,8 @@ __global__ void __launch_bounds__(1024) distill_finish_kernel(const float* row_l
     if (held) held[0] = 1.f;
   }
 }
-__global__ void distill_held_kernel(const float* upstream, float* held) { held[0] = upstream[0]; }
+// the gradient is its caller's from here on: no upstream is equal to this
+__global__ void distill_released_kernel(float* held) { held[0] = __uint_as_float(0x7FC00000u); }
 
 // ---------------------------------------------------------------------------
 // host side
@@ -868,7 +869,7 @@ extern "C" int ff_distill_loss(const FfDistillRows* in, int reduction, float* ro
 }
 
 extern "C" int ff_distill_grad(const FfDistillRows* in, int reduction, const float* upstream, float* held,
-                               int keep_held, const int32_t* counts, void* grad, int64_t ldg, void* stream) {
+                               int replayed, const int32_t* counts, void* grad, int64_t ldg, void* stream) {
   using namespace ff::distill;
   Args a;
   int rc = fill("ff_distill_grad", in, &a);
@@ -887,7 +888,7 @@ extern "C" int ff_distill_grad(const FfDistillRows* in, int reduction, const flo
   a.up_stride = reduction == FF_REDUCE_NONE ? 1 : 0;
   a.held = held;
   rc = launch_dt(a, in->dtype, ff::as_stream(stream), "ff_distill_grad");
-  if (rc || !held || !keep_held) return rc;
-  distill_held_kernel<<<1, 1, 0, ff::as_stream(stream)>>>(upstream, held);
+  if (rc || !held || !replayed) return rc;
+  distill_released_kernel<<<1, 1, 0, ff::as_stream(stream)>>>(held);
   return ff::check_launch("ff_distill_grad held");
 }

@@ -40,6 +40,16 @@ extern "C" int ff_device_status(uint32_t* out, int clear) {
   return FF_OK;
 }
 
+extern "C" int ff_capture_id(uint64_t* out, void* stream) {
+  FF_REQUIRE(out, FF_ERR_INVALID_ARG, "ff_capture_id: null pointer");
+  *out = 0;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  FF_CUDA_TRY(cudaStreamGetCaptureInfo(ff::as_stream(stream), &status, &id), "ff_capture_id");
+  if (status == cudaStreamCaptureStatusActive) *out = id;
+  return FF_OK;
+}
+
 extern "C" int ff_set_wait_limit_ns(uint64_t ns) {
   const uint64_t v = ns ? ns : ff::kWaitLimitNs;
   FF_CUDA_TRY(cudaMemcpyToSymbol(ff::g_wait_limit_ns, &v, sizeof(v)), "ff_set_wait_limit_ns");

@@ -4,7 +4,8 @@ The reference ships no loss; this stands beside the decoder's cross-entropy.  Th
 by its k largest logits per position, which is what a teacher run can afford to store.  Forward with
 a reduction reads the student's logits once and writes their gradient in the same pass, for an
 upstream gradient of 1; backward hands it out, or, when the upstream gradient on the device is
-another, recomputes it (no host synchronisation either way).
+another, recomputes it (no host synchronisation either way).  In CUDA graphs that holds where one graph has both; a
+backward captured without its forward, or run on a captured one, computes the gradient in a buffer of its own.
 """
 from __future__ import annotations
 
@@ -26,7 +27,7 @@ class DistillationLossFn(torch.autograd.Function):
         row, loss, g, held, counts = _capi.distill_loss(rows, logits, reduction, grad)
         if grad:
             ctx.save_for_backward(logits, ids, teacher_logits, labels, teacher_lse, counts)
-            ctx.ready = None if g is None else (g, held)
+            ctx.ready = None if g is None else (g, held, _capi.capture_id(logits.device))
         return row if reduction == "none" else loss
 
     @staticmethod
@@ -35,10 +36,14 @@ class DistillationLossFn(torch.autograd.Function):
         logits, ids, teacher_logits, labels, teacher_lse, counts = ctx.saved_tensors
         rows = _capi.distill_rows(logits, ids, teacher_logits, labels, teacher_lse, *ctx.args)
         up = up.to(torch.float32).contiguous()
-        g, held = ctx.ready or (None, None)
+        g, held, made_in = ctx.ready or (None, None, 0)
         ctx.ready = None  # the buffer is handed out: a second backward makes its own
-        g = _capi.distill_grad(rows, logits, ctx.reduction, up, counts, g, held,
-                               keep_held=torch.cuda.is_current_stream_capturing())
+        capture = _capi.capture_id(logits.device)
+        if made_in != capture:
+            # a forward and a backward that are not replayed together: the one's buffer would be rewritten under, or
+            # handed out a second time to, the other's caller
+            g = held = None
+        g = _capi.distill_grad(rows, logits, ctx.reduction, up, counts, g, held, replayed=capture != 0)
         return (g,) + (None,) * 9
 
 

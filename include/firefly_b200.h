@@ -68,6 +68,9 @@ FF_API int ff_num_sms(int* out);
  */
 FF_API int ff_device_status(uint32_t* out, int clear);
 
+/* The id of the graph capture that the stream takes part in (two captures have two ids), 0 if none. */
+FF_API int ff_capture_id(uint64_t* out, void* stream);
+
 /*
  * Per-row absmax int8 quantiser.
  * Replaces fireflykernels.py:96-104 quantize_fp_to_int8 (and bitLinear.py:15-27):
@@ -656,9 +659,10 @@ FF_API int ff_distill_loss(const FfDistillRows* in, int reduction, float* row_lo
 /*
  * The gradient for an upstream gradient on the device: a scalar, or one value per row for
  * FF_REDUCE_NONE.  held (or NULL): grad already holds the gradient for that scalar, and an equal
- * upstream leaves it as it is; keep_held updates held, for a call that is replayed.
+ * upstream leaves it as it is.  After the call grad is its caller's to change, so a call that is replayed sets
+ * replayed: held then becomes NaN, and grad is formed anew until ff_distill_loss has written both again.
  */
-FF_API int ff_distill_grad(const FfDistillRows* in, int reduction, const float* upstream, float* held, int keep_held,
+FF_API int ff_distill_grad(const FfDistillRows* in, int reduction, const float* upstream, float* held, int replayed,
                            const int32_t* counts, void* grad, int64_t ldg, void* stream);
 
 #ifdef __cplusplus

@@ -404,3 +404,87 @@ def test_extreme_temperatures(T):
     arg = float(s.abs().max()) / T * 1.5
     lim = (2.0 ** -18 + 2.0 ** -23 * arg) * 4 * max(T, 1.0) + 2.0 ** -8 * float(s64.grad.abs().max())
     assert float((x.grad.double() - s64.grad).abs().max()) <= lim
+
+
+def test_backward_alone_replayed_after_its_gradient_was_changed():
+    """What a replayed backward pass returns is its caller's: cleared, scaled or added to, it is formed anew."""
+    s, ids, t, lab, _ = _case(40, 5000, 16, 38, labels=True)
+    x = s.clone().requires_grad_(True)
+    y = s.clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(distillation_loss(y, ids, t, lab, alpha=0.5), y)
+    up = torch.ones((), device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        l = distillation_loss(x, ids, t, lab, alpha=0.5)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            grad = torch.autograd.grad(l, x, up)[0]
+    grad.zero_()  # before the first replay, too
+    for change in (lambda: grad.zero_(), lambda: grad.mul_(0.5), lambda: grad.add_(want), lambda: None):
+        g.replay()
+        assert torch.equal(grad, want)
+        change()
+
+
+def test_forward_and_backward_in_graphs_of_their_own():
+    s, ids, t, lab, _ = _case(40, 5000, 16, 39, labels=True)
+    x = s.clone().requires_grad_(True)
+    up = torch.ones((), device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        distillation_loss(x, ids, t, lab, alpha=0.5).backward()
+        x.grad = None
+        torch.cuda.synchronize()
+        fwd, bwd = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(fwd, stream=side):
+            l = distillation_loss(x, ids, t, lab, alpha=0.5)
+        with torch.cuda.graph(bwd, stream=side):
+            grad = torch.autograd.grad(l, x, up)[0]
+    for k in range(3):
+        x.data.copy_(s * (1 + 0.25 * k))
+        y = x.detach().clone().requires_grad_(True)
+        ref = distillation_loss(y, ids, t, lab, alpha=0.5)
+        (want,) = torch.autograd.grad(ref, y)
+        fwd.replay()
+        grad.zero_()
+        bwd.replay()
+        assert torch.equal(l, ref) and torch.equal(grad, want)
+
+
+def test_a_replayed_forward_leaves_earlier_gradients_alone():
+    """A captured loss whose backward pass runs eagerly, step after step: the gradients of earlier steps are summed."""
+    s, ids, t, lab, _ = _case(40, 5000, 16, 40, labels=True)
+    x = s.clone().requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            l = distillation_loss(x, ids, t, lab, alpha=0.5)
+        wants, gots = [], []
+        for k in range(3):
+            x.data.copy_(s * (1 + 0.25 * k))
+            g.replay()
+            gots.append(torch.autograd.grad(l, x, retain_graph=True)[0])
+            y = x.detach().clone().requires_grad_(True)
+            wants.append(torch.autograd.grad(distillation_loss(y, ids, t, lab, alpha=0.5), y)[0])
+        torch.cuda.synchronize()
+    for a, b in zip(gots, wants):
+        assert torch.equal(a, b)
+
+
+def test_c_entry_that_is_replayed_forms_its_gradient_anew():
+    """``held`` of a replayed ff_distill_grad: equal once, then only after ff_distill_loss has run again."""
+    s, ids, t, lab, _ = _case(10, 900, 8, 43, labels=True)
+    rows = _capi.distill_rows(s, ids, t, lab, None, 1.0, 0.5, -100)
+    up = torch.ones((), device=DEV)
+    for _ in range(2):
+        _, _, grad, held, counts = _capi.distill_loss(rows, s, "mean", True)
+        want = grad.clone()
+        for _ in range(3):
+            assert torch.equal(_capi.distill_grad(rows, s, "mean", up, counts, grad, held, replayed=True), want)
+            assert bool(torch.isnan(held))
+            grad.zero_()
