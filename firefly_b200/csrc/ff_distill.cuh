@@ -7,9 +7,10 @@
 //   q_v = softmax(s/T)_v,  q_rest = sum of q_v over the tokens outside the entries
 //   KD  = T^2 [ sum_j p_j (log p_j - log q_{i_j}) + p_rest (log p_rest - log q_rest) ]
 //   L   = alpha KD + (1 - alpha) (logsumexp(s) - s_y)
-//   dL/ds_v = alpha T (q_v - sum_{j: i_j = v} p_j)   on the entries' tokens,
-//             alpha T q_v (1 - p_rest / q_rest)       elsewhere (without lse: alpha T q_v),
+//   dL/ds_v = alpha T (w q_v - sum_{j: i_j = v} p_j)   on the entries' tokens, w = sum p + p_rest,
+//             alpha T q_v (w - p_rest / q_rest)         elsewhere (without lse: alpha T q_v),
 //             + (1 - alpha) (softmax(s)_v - [v = y]).
+// p_rest is not negative: w is 1, or sum p where a rounded lse or a token given twice make that more than 1.
 // A row whose label is ignore_index, or without labels a row without entries, counts nothing.
 //
 // One cluster of 1 to 8 CTAs per row, each holding its slice of the row in shared memory (bulk
@@ -572,7 +573,9 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
         if (grow && live) {
           const float up = a.upstream ? __ldg(a.upstream + r * a.up_stride) * inv_count : inv_count;
           const float fk = has ? up * a.alpha * a.T : 0.f, f1 = label >= 0 ? up * (1.f - a.alpha) : 0.f;
-          const float gq = fk / all.sum, g1 = f1 / sum1_all;  // factors of exp(..) for q and the softmax at 1
+          // log sum exp(s/T) stands in the loss with the weight sum p + p_rest: 1 unless the teacher's log-sum-exp is off
+          const float mass = a.lse && p_rest == 0.f ? c.t_sum[buf] : 1.f;
+          const float gq = mass * fk / all.sum, g1 = f1 / sum1_all;  // factors of exp(..) for q and the softmax at 1
           const float gr = p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;  // q outside the entries
           const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == (uint32_t)g.mis;
           const f2 kT2 = splat(kT), nT2 = splat(nMT), k12 = splat(k1), n12 = splat(nM1), gr2 = splat(two ? gr : gr + g1),

@@ -488,3 +488,132 @@ def test_c_entry_that_is_replayed_forms_its_gradient_anew():
             assert torch.equal(_capi.distill_grad(rows, s, "mean", up, counts, grad, held, replayed=True), want)
             assert bool(torch.isnan(held))
             grad.zero_()
+
+
+# ---------------------------------------------------------------------------
+# element by element, each rounding counted
+# ---------------------------------------------------------------------------
+def _bounds(s, ids, t, lab, lse, T, alpha):
+    """Rows' losses and gradients in fp64, which rows count, and what fp32 may be off by: per row for the loss, per
+    element for the gradient of the rows' sum.  With u = 2^-24, half a step of 1:
+      log p: 1/T, t/T and the difference rounded; without lse also log Z, K/32 + 8 additions of exponentials;
+      p: that and 4u for the exponential; sum p: K/32 + 8 additions more; p_rest = 1 - sum p: u more;
+      an exponential of q with the argument z (base 2): three roundings in log2(e)/T, one in the multiply-add, one where
+      the references of two CTAs differ, 5u |z|, and 4u;
+      sums over the row: V/512 + 28 additions (in a thread, over the warps, over the CTAs);
+      logarithms: 4u of their values;  the loss: K/256 + 16 additions.
+    At T = 2 and 4 the softmax at 1 is a square of exponentials: twice (four times) their errors.  The factor 1.05
+    covers the terms of second order."""
+    u = 2.0 ** -24
+    n, V = s.shape
+    K = ids.shape[1]
+    x = s.detach().double().requires_grad_(True)
+    rows, counted, _ = O.losses(x, ids, t, lab, lse, T, alpha)
+    rows.sum().backward()
+    rows, grad, x = rows.detach(), x.grad, x.detach()
+    zero = torch.zeros((), dtype=torch.float64, device=s.device)
+    on = (ids >= 0) & (ids < V) & (t != -math.inf)
+    at = torch.where(on, ids, 0).long()
+    has = on.any(1, keepdim=True)
+    tt = torch.where(on, t.double() / T, zero)
+    lz = torch.logsumexp(tt.masked_fill(~on, -math.inf), 1, keepdim=True) if lse is None else lse.double()[:, None]
+    lp = torch.where(on, tt - torch.where(has, lz, zero), zero)
+    p = torch.where(on, torch.exp(lp), zero)
+    d_lp = 4 * u * tt.abs() + 2 * u * lp.abs()
+    if lse is None:
+        d_lp = d_lp + 6 * u * tt.abs().amax(1, keepdim=True) + (K / 32 + 16) * u
+    e_p = d_lp + 4 * u
+    psum = p.sum(1, keepdim=True)
+    d_ps = (e_p * p).sum(1, keepdim=True) + (K / 32 + 8) * u * psum
+    gap = (x - x.amax(1, keepdim=True)).abs() * 1.4427
+    z = gap / T
+    logq = torch.log_softmax(x / T, 1)
+    q = torch.exp(logq)
+    e_sum = (V / 512 + 28) * u + 5 * u * torch.where(q > 0, q * z, zero).sum(1, keepdim=True)
+    e_q = 5 * u * z + 4 * u + e_sum
+    lq = logq.gather(1, at)
+    d_lq = e_q.gather(1, at) + 4 * u * (1 + math.log(V))
+    live = on & (p > 0)
+    size = torch.where(live, p * (lp.abs() + lq.abs()), zero).sum(1)
+    d_kd = torch.where(live, p * (e_p * (lp.abs() + lq.abs()) + d_lp + d_lq), zero).sum(1)
+    mark = torch.zeros(n, V, dtype=torch.bool, device=s.device)
+    mark[torch.arange(n, device=s.device)[:, None].expand_as(at)[on], at[on]] = True
+    pv = torch.zeros_like(q).scatter_add_(1, at, p)
+    tol = q * torch.where(q > 0, e_q, zero) + torch.zeros_like(q).scatter_add_(1, at, (e_p + 2 * u) * p)
+    if lse is not None:
+        other = ((~mark).any(1, keepdim=True)) & has
+        pr = torch.where(other, (1 - psum).clamp(min=0), zero)
+        d_pr = torch.where(other, d_ps + u, zero)
+        rest = logq.masked_fill(mark, -math.inf)
+        lr = torch.where(other, torch.logsumexp(rest, 1, keepdim=True), zero)
+        share = torch.where(other, torch.exp(rest - lr), zero)  # softmax over the tokens outside the entries
+        zr = lr.abs() * 1.4427
+        log_pr = torch.where(pr > 0, torch.log(pr), zero).abs()
+        # x log x + x |log q_rest|: by its slope, or where p_rest may be 0 by its size
+        d_rest = torch.where(pr > d_pr, 2 * d_pr * (log_pr + 1 + lr.abs()),
+                             2 * d_pr * (torch.log(2 * d_pr + 1e-30).abs() + lr.abs()))
+        d_kd = d_kd + (d_rest + pr * (e_sum + 10 * u * zr + 4 * u * (lr.abs() + log_pr + 2)))[:, 0]
+        size = size + (pr * (log_pr + lr.abs()))[:, 0]
+        zz = torch.where(share > 0, (x - x.masked_fill(mark, -math.inf).amax(1, keepdim=True)).abs() / T * 1.4427, zero)
+        # (below a rest of 2^-60 of the row, q itself is left out beside the rest's softmax)
+        tol = tol + share * (d_pr + pr * (5 * u * (zz + zr.clamp(max=90)) + 12 * u + e_sum + 2.0 ** -59))
+        tol = tol * psum.clamp(min=1) + q * d_ps
+    d_row = alpha * T * T * torch.where(has[:, 0], d_kd + (K / 256 + 16) * u * size, zero)
+    tol = alpha * T * torch.where(has, tol + 2.0 ** -120, zero)
+    if lab is not None:
+        y = lab.clamp(min=0)[:, None]
+        q1 = torch.softmax(x, 1)
+        e_1 = (V / 512 + 28) * u + 20 * u * torch.where(q1 > 0, q1 * gap, zero).sum(1, keepdim=True)
+        tol = tol + (1 - alpha) * (torch.where(q1 > 0, q1 * (20 * u * gap + 16 * u + e_1), zero) + 2.0 ** -120
+                                   + 4 * u * torch.zeros_like(q).scatter_(1, y, 1.0))
+        d_row = d_row + (1 - alpha) * (20 * u * gap.gather(1, y) + e_1 + 4 * u * (1 + math.log(V)))[:, 0]
+    ok = torch.tensor(counted, device=s.device)
+    d_row = torch.where(ok, 1.05 * d_row + 4 * u * rows.abs(), zero)
+    return rows, grad, ok, d_row, torch.where(ok[:, None], 1.05 * tol + 6 * u * grad.abs(), zero), mark
+
+
+def _check_each(s, ids, t, lab=None, lse=None, T=1.0, alpha=1.0):
+    """Row losses and the gradient of their sum against fp64, within ``_bounds`` and the gradient's own rounding.
+    Returns how much of the gradient off the entries is larger than its bound."""
+    rows, grad, ok, d_row, tol, mark = _bounds(s, ids, t, lab, lse, T, alpha)
+    kw = dict(teacher_lse=lse, temperature=T, alpha=alpha)
+    got = distillation_loss(s, ids, t, lab, reduction="none", **kw).double()
+    assert bool(((got - rows).abs() <= d_row).all()), (got.tolist()[:4], rows.tolist()[:4], d_row.tolist()[:4])
+    x = s.detach().clone().requires_grad_(True)
+    distillation_loss(x, ids, t, lab, reduction="sum", **kw).backward()
+    info = torch.finfo(s.dtype)
+    tol = tol * (1 + info.eps) + info.eps / 2 * grad.abs() + info.smallest_normal * info.eps
+    off = (x.grad.double() - grad).abs()
+    bad = ~(off <= tol)
+    assert not bool(bad.any()), (int(bad.sum()), float((off / tol.clamp(min=1e-300)).max()), torch.nonzero(bad)[:4].tolist())
+    assert _capi.device_status() == 0
+    return float((grad.abs() > tol)[~mark & ok[:, None]].double().mean())
+
+
+@pytest.mark.parametrize("V", [500, 40000])
+@pytest.mark.parametrize("T", [1.0, 2.0])
+def test_gradient_of_entries_that_sum_to_more_than_one(V, T):
+    """A teacher's log-sum-exp of 16 bits, repeated tokens: sum p lies above 1 by percents, and the gradient is still the
+    loss's."""
+    for dtype in DTYPES:
+        s, ids, t, lab, lse = _case(6, V, 24, 34, labels=True, tail=True, T=T, pad=False)
+        s = s.to(dtype)
+        low = (torch.logsumexp(t.double() / T, 1) - 0.03).float()
+        _check_each(s, ids, t, None, low, T)
+        _check_each(s, ids, t, lab, low, T, 0.5)
+        _check_each(s, ids, t, None, lse.bfloat16().float(), T)
+        ids[:, 5:9] = ids[:, :1]
+        _check_each(s, ids, t, lab, low, T, 0.5)
+    # against differences, in fp32
+    s, ids, t, _, _ = _case(2, 60, 6, 35, dtype=torch.float32, pad=False)
+    low = (torch.logsumexp(t.double() / T, 1) - 0.5).float()
+    x = s.clone().requires_grad_(True)
+    distillation_loss(x, ids, t, teacher_lse=low, temperature=T, reduction="sum").backward()
+    f = lambda z: O.losses(z, ids, t, None, low, T, 1.0)[0].sum()
+    h = 1e-4
+    for r, v in ((0, 3), (0, int(ids[0, 0])), (1, 59), (1, int(ids[1, 5]))):
+        a, b = s.double().clone(), s.double().clone()
+        a[r, v] += h
+        b[r, v] -= h
+        # the third derivative is at most sum p T^2 / T^3 in size: h^2 / 6 of it; fp32 in the kernel
+        assert abs(float((f(a) - f(b)) / (2 * h)) - float(x.grad[r, v])) <= h * h + 1e-10 / h + 2.0 ** -18 * 4
