@@ -460,7 +460,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
         const float ms = m == neg_inf() ? 0.f : m;  // a slice of -inf sums to 0
         // exp((s - m)/T) = 2^(s k - m k): one fused multiply-add with the rounded m k, the same for the
         // entries, so that its rounding cancels between q's numerator and denominator and in log q
-        const float nmT = -ms * kT, nm1 = -ms * k1;
+        const float nmT = -__fmul_rn(ms, kT), nm1 = -__fmul_rn(ms, k1);
         float sum = 0.f, sum1 = 0.f, rest = 0.f, dot = 0.f, psum = 0.f;
         for (int j = tid; j < a.K; j += THREADS) {
           const int pos = e_pos[j];
@@ -538,9 +538,10 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
           all.label = neg_inf();
           for (int k = 0; k < csize; ++k) {
             const Part q = c.parts[par][k];
-            // from 2^(s k - m k) to 2^(s k - M k): the difference of the two rounded products
-            const float d = q.m == neg_inf() ? 0.f : Ms * kT - q.m * kT;
-            const float f = ex2(-d), f1 = q.m == neg_inf() ? 1.f : ex2(q.m * k1 - Ms * k1);
+            // from 2^(s k - m k) to 2^(s k - M k): the difference of the two rounded products (not contracted into
+            // one multiply-add, which would leave the rounding of M k in the sums: 2^-14 for |M| / T of 1000)
+            const float d = q.m == neg_inf() ? 0.f : __fsub_rn(__fmul_rn(Ms, kT), __fmul_rn(q.m, kT));
+            const float f = ex2(-d), f1 = q.m == neg_inf() ? 1.f : ex2(__fsub_rn(__fmul_rn(q.m, k1), __fmul_rn(Ms, k1)));
             all.sum += q.sum * f;
             all.sum1 += q.sum1 * f1;
             all.rest += q.rest * f;
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
           }
           par ^= 1u;
         }
-        const float Ms = all.m == neg_inf() ? 0.f : all.m, nMT = -Ms * kT, nM1 = -Ms * k1;
+        const float Ms = all.m == neg_inf() ? 0.f : all.m, nMT = -__fmul_rn(Ms, kT), nM1 = -__fmul_rn(Ms, k1);
         const float sum1_all = two ? all.sum1 : all.sum;
         const bool has = c.t_any[buf] != 0;
         if (!a.labels) live = has;

@@ -617,3 +617,19 @@ def test_gradient_of_entries_that_sum_to_more_than_one(V, T):
         b[r, v] -= h
         # the third derivative is at most sum p T^2 / T^3 in size: h^2 / 6 of it; fp32 in the kernel
         assert abs(float((f(a) - f(b)) / (2 * h)) - float(x.grad[r, v])) <= h * h + 1e-10 / h + 2.0 ** -18 * 4
+
+
+@pytest.mark.parametrize("T,labels", [(0.01, False), (0.01, True), (0.05, False), (0.7, True)])
+def test_rows_cut_over_several_ctas_at_small_temperatures(T, labels):
+    """Logits that are large against their spread: what is rounded in M log2(e) / T has to cancel between the CTAs (of
+    logits near 10 at T = 0.01 it is up to 2^-14)."""
+    g = torch.Generator(device=DEV).manual_seed(37)
+    n, V, k = 12, 40000, 16
+    base = torch.rand(n, 1, device=DEV, generator=g) * 10 + 5
+    s = base + T * torch.rand(n, V, device=DEV, generator=g)
+    ids = torch.randint(0, V, (n, k), device=DEV, generator=g)
+    t = torch.rand(n, k, device=DEV, generator=g) * T
+    lab = torch.randint(0, V, (n,), device=DEV, generator=g) if labels else None
+    _check_each(s, ids, t, lab, None, T, 0.5 if labels else 1.0)
+    lse = torch.full((n,), math.log(V), device=DEV)
+    _check_each(s, ids, t, lab, lse, T, 0.5 if labels else 1.0)
