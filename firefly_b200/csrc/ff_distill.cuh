@@ -160,6 +160,45 @@ __device__ __forceinline__ typename Elem<DT>::T from_f32(float v) {
   else return __float2half_rn(v);
 }
 
+// exp((s - m)/T) = 2^(s k - m k), k = log2(e)/T: one fused multiply-add with the rounded product m k, the same
+// wherever m is the reference, so that its rounding cancels between q's numerator and denominator and in log q.
+// From |m| k = 2^31 on (a slice or row of nothing but a mask of -1e10 or the type's lowest value) that rounding exceeds
+// 2^6 and the product may overflow.  Two different fp32 logits lie 2^7 or more apart there in log2, so 2^(s k - m k) is 1
+// for s = m and 0 below: a power of two in the place of k, with |m| k about 2^100, gives just that with exact products.
+// At T = 2 and 4 (PW) the softmax at 1 is a power of this one, so its k counts (2^5 or more apart at T then).
+constexpr float kLn2 = 0.6931471805599453f;
+template <int PW>
+struct Ref {
+  float m, k;  // the reference (0 for -inf) and the true factor
+  bool far;
+  __device__ __forceinline__ Ref(float max_, float k_, float k_of_far) : m(max_ == neg_inf() ? 0.f : max_), k(k_) {
+    far = fabsf(m) * k_of_far >= 2147483648.f;
+  }
+  static __device__ __forceinline__ Ref at_t(float max_, float kT, float k1) { return Ref(max_, kT, PW == 2 || PW == 4 ? k1 : kT); }
+  static __device__ __forceinline__ Ref at_1(float max_, float k1) { return Ref(max_, k1, k1); }
+  // factor and addend of the multiply-add
+  __device__ __forceinline__ float mul() const {
+    return far ? __uint_as_float(min(354u - (__float_as_uint(fabsf(m)) >> 23), 254u) << 23) : k;
+  }
+  __device__ __forceinline__ float add() const { return -__fmul_rn(m, mul()); }
+  // one value's exponential in log2 and as (s - m)/T: the multiply-add's, and where that says no more than "far below"
+  // (a masked label or entry has a finite loss), the difference
+  __device__ __forceinline__ float log2_of(float s) const { return far ? (s - m) * k : fmaf(s, k, add()); }
+  __device__ __forceinline__ float log_of(float s) const {
+    const float z = log2_of(s);
+    return far || z == neg_inf() ? (s - m) * kLn2 * k : z * kLn2;
+  }
+  // log2 of the factor from sums relative to `o` to sums relative to this one: the difference of the two rounded
+  // products (not contracted into one multiply-add, which would leave the rounding of m k in the sums: 2^-14 for
+  // |m| / T of 1000)
+  __device__ __forceinline__ float log2_from(const Ref& o) const {
+    return far || o.far ? (o.m - m) * k : __fsub_rn(__fmul_rn(o.m, k), __fmul_rn(m, k));
+  }
+  __device__ __forceinline__ float log_from(const Ref& o) const {
+    return far || o.far ? (o.m - m) * kLn2 * k : log2_from(o) * kLn2;
+  }
+};
+
 // what a CTA tells the others about its slice
 struct Part {
   float m;        // largest logit
@@ -257,7 +296,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
     inv_count = 1.f / (float)max(n, 1);
   }
 
-  const float inv_t = 1.f / a.T, kT = 1.4426950408889634f * inv_t, k1 = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+  const float inv_t = 1.f / a.T, kT = 1.4426950408889634f * inv_t, k1 = 1.4426950408889634f;
   const int64_t v0 = (int64_t)rank * a.slice;
   const int len = (int)max64(0, min64(a.slice, a.V - v0)), bytes = len * ES;
   const uint4* w = reinterpret_cast<const uint4*>(data);
@@ -457,27 +496,24 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
         if (lane == 0) c.red[0][warp] = m;
         bar_compute();
         m = max8(c.red[0]);
-        const float ms = m == neg_inf() ? 0.f : m;  // a slice of -inf sums to 0
-        // exp((s - m)/T) = 2^(s k - m k): one fused multiply-add with the rounded m k, the same for the
-        // entries, so that its rounding cancels between q's numerator and denominator and in log q
-        const float nmT = -__fmul_rn(ms, kT), nm1 = -__fmul_rn(ms, k1);
+        const auto rT = Ref<PW>::at_t(m, kT, k1), r1 = Ref<PW>::at_1(m, k1);  // a slice of -inf sums to 0
         float sum = 0.f, sum1 = 0.f, rest = 0.f, dot = 0.f, psum = 0.f;
         for (int j = tid; j < a.K; j += THREADS) {
           const int pos = e_pos[j];
           if (pos == -1 || pos == -2) continue;
-          const float z = fmaf(e_s[j], kT, nmT), p = expf(e_p[j]);
-          if (p > 0.f) dot += p * (e_p[j] - z * kLn2);
+          const float z = rT.log2_of(e_s[j]), p = expf(e_p[j]);
+          if (p > 0.f) dot += p * (e_p[j] - rT.log_of(e_s[j]));
           else if (p != p) dot = p;
           psum += p;
           if (pos >= 0) {
             sum += ex2(z);
-            if (two) sum1 += ex2(fmaf(e_s[j], k1, nm1));
+            if (two) sum1 += ex2(r1.log2_of(e_s[j]));
           }
         }
         // ---- sums of exp over the tokens outside the entries
         f2 acc = splat(0.f), acc1 = splat(0.f);
         {
-          const f2 kT2 = splat(kT), nT2 = splat(nmT), k12 = splat(k1), n12 = splat(nm1);
+          const f2 kT2 = splat(rT.mul()), nT2 = splat(rT.add()), k12 = splat(r1.mul()), n12 = splat(r1.add());
 #pragma unroll 2
           for (int k = tid; k < g.words; k += THREADS) {
             f2 v[P];
@@ -533,25 +569,24 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
           gemm::cluster_sync_all();
           all = c.parts[par][0];
           for (int k = 1; k < csize; ++k) all.m = fmaxf(all.m, c.parts[par][k].m);
-          const float Ms = all.m == neg_inf() ? 0.f : all.m;
+          const auto RT = Ref<PW>::at_t(all.m, kT, k1), R1 = Ref<PW>::at_1(all.m, k1);
           all.sum = all.sum1 = all.rest = all.dot = all.psum = 0.f;
           all.label = neg_inf();
           for (int k = 0; k < csize; ++k) {
             const Part q = c.parts[par][k];
-            // from 2^(s k - m k) to 2^(s k - M k): the difference of the two rounded products (not contracted into
-            // one multiply-add, which would leave the rounding of M k in the sums: 2^-14 for |M| / T of 1000)
-            const float d = q.m == neg_inf() ? 0.f : __fsub_rn(__fmul_rn(Ms, kT), __fmul_rn(q.m, kT));
-            const float f = ex2(-d), f1 = q.m == neg_inf() ? 1.f : ex2(__fsub_rn(__fmul_rn(q.m, k1), __fmul_rn(Ms, k1)));
+            const auto o = Ref<PW>::at_t(q.m, kT, k1);
+            const bool any = q.m != neg_inf();
+            const float f = any ? ex2(RT.log2_from(o)) : 1.f, f1 = any ? ex2(R1.log2_from(Ref<PW>::at_1(q.m, k1))) : 1.f;
             all.sum += q.sum * f;
             all.sum1 += q.sum1 * f1;
             all.rest += q.rest * f;
-            all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot + q.psum * d * kLn2 : 0.f;
+            all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot - (any ? q.psum * RT.log_from(o) : 0.f) : 0.f;
             all.psum += q.psum;
             all.label = fmaxf(all.label, q.label);
           }
           par ^= 1u;
         }
-        const float Ms = all.m == neg_inf() ? 0.f : all.m, nMT = -__fmul_rn(Ms, kT), nM1 = -__fmul_rn(Ms, k1);
+        const auto RT = Ref<PW>::at_t(all.m, kT, k1), R1 = Ref<PW>::at_1(all.m, k1);
         const float sum1_all = two ? all.sum1 : all.sum;
         const bool has = c.t_any[buf] != 0;
         if (!a.labels) live = has;
@@ -566,7 +601,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
             if (p_rest > 0.f) kd += p_rest * (logf(p_rest) - logf(q_rest));
             kd *= a.T * a.T;
           }
-          if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - fmaf(all.label, two ? k1 : kT, two ? nM1 : nMT) * kLn2;
+          if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - (two ? R1 : RT).log_of(all.label);
           a.row_loss[r] = live ? (a.alpha != 0.f ? a.alpha * kd : 0.f) + (a.alpha != 1.f ? (1.f - a.alpha) * ce : 0.f) : 0.f;
         }
         // ---- the gradient, half the slice at a time; the next row's copies follow into each
@@ -579,7 +614,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
           const float gq = mass * fk / all.sum, g1 = f1 / sum1_all;  // factors of exp(..) for q and the softmax at 1
           const float gr = p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;  // q outside the entries
           const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == (uint32_t)g.mis;
-          const f2 kT2 = splat(kT), nT2 = splat(nMT), k12 = splat(k1), n12 = splat(nM1), gr2 = splat(two ? gr : gr + g1),
+          const f2 kT2 = splat(RT.mul()), nT2 = splat(RT.add()), k12 = splat(R1.mul()), n12 = splat(R1.add()), gr2 = splat(two ? gr : gr + g1),
                    g12 = splat(g1);
           const int step = (max(g.words, gn.words) + 2 * THREADS - 1) / (2 * THREADS) * THREADS;
           uint4* gw = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(grow) - g.mis);  // word k of the slice
@@ -634,13 +669,13 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
               for (int x = 0; x < a.K; ++x)
                 if (e_pos[x] == pos || e_pos[x] == -3 - pos) p += expf(e_p[x]);
             }
-            float gv = gq * ex2(fmaf(e_s[j], kT, nMT)) - fk * p;
-            if (f1 != 0.f) gv += g1 * ex2(fmaf(e_s[j], two ? k1 : kT, two ? nM1 : nMT)) - (v0 + pos == label ? f1 : 0.f);
+            float gv = gq * ex2(RT.log2_of(e_s[j])) - fk * p;
+            if (f1 != 0.f) gv += g1 * ex2((two ? R1 : RT).log2_of(e_s[j])) - (v0 + pos == label ? f1 : 0.f);
             grow[pos] = from_f32<DT>(gv);
           }
           if (tid == 0 && label >= v0 && label < v0 + len && !c.label_in_top[buf]) {
-            const float x = ex2(fmaf(c.label_logit, kT, nMT));
-            grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(fmaf(c.label_logit, k1, nM1)) : (gr + g1) * x) - f1);
+            const float x = ex2(RT.log2_of(c.label_logit));
+            grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(R1.log2_of(c.label_logit)) : (gr + g1) * x) - f1);
           }
         }
       }

@@ -507,7 +507,8 @@ def _bounds(s, ids, t, lab, lse, T, alpha):
     u = 2.0 ** -24
     n, V = s.shape
     K = ids.shape[1]
-    x = s.detach().double().requires_grad_(True)
+    x = s.detach().double()  # counted from the row's maximum, so that 64 bits hold the logarithms beside a mask of -1e30
+    x = (x - x.amax(1, keepdim=True).clamp(min=-1e300)).requires_grad_(True)
     rows, counted, _ = O.losses(x, ids, t, lab, lse, T, alpha)
     rows.sum().backward()
     rows, grad, x = rows.detach(), x.grad, x.detach()
@@ -633,3 +634,37 @@ def test_rows_cut_over_several_ctas_at_small_temperatures(T, labels):
     _check_each(s, ids, t, lab, None, T, 0.5 if labels else 1.0)
     lse = torch.full((n,), math.log(V), device=DEV)
     _check_each(s, ids, t, lab, lse, T, 0.5 if labels else 1.0)
+
+
+@pytest.mark.parametrize("T", [0.01, 0.7, 1.0, 2.0, 3.0, 4.0, 1000.0])
+@pytest.mark.parametrize("mask", [-1e9, -1e10, -1e30, "lowest"])
+def test_masks_that_fill_a_whole_slice_or_row(mask, T):
+    """A vocabulary whose upper half is masked (one CTA's slice and more hold nothing else), rows of nothing but the mask,
+    and rows of large logits of either sign."""
+    for dtype in (torch.float32, torch.bfloat16):
+        low = torch.finfo(dtype).min if mask == "lowest" else mask
+        s, ids, t, lab, _ = _case(5, 32768, 8, 36, labels=True, pad=False)
+        ids, lab = ids % 16000, torch.where(lab >= 0, lab % 16000, lab)
+        s = s.to(dtype)
+        s[:, 16384:] = low
+        s[1] = low
+        s[2, :16000] += 64 if mask == -1e9 else 0
+        _check_each(s, ids, t, None, None, T)
+        _check_each(s, ids, t, lab, None, T, 0.5)
+        big = s[3:4].clone()
+        big[:, 100] = -low  # one logit above all others: a softmax of one token
+        _check_each(big, torch.full_like(ids[3:4], 100), t[3:4], torch.full_like(lab[3:4], 100), None, T, 0.5)
+
+
+@pytest.mark.parametrize("V", [700, 40000])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_masked_label_and_a_masked_entry(V, dtype):
+    """The type's lowest value at the label, or at a token that the teacher keeps: a large loss, but a finite one."""
+    s, ids, t, lab, _ = _case(4, V, 8, 42, labels=True, pad=False, dtype=dtype)
+    lab = lab.clamp(min=0)
+    one = s.scatter(1, lab[:, None], torch.finfo(dtype).min)
+    _check_each(one, ids, t, lab, None, 1.0, 0.5)
+    t[:, 0] -= 8  # little of the teacher's mass: the loss stays in range
+    two = s.scatter(1, ids[:, :1], torch.finfo(dtype).min)
+    _check_each(two, ids, t)
+    _check_each(two, ids, t, None, torch.logsumexp(t.double(), 1).float() + 0.1)
