@@ -10,7 +10,9 @@
 //   dL/ds_v = alpha T (w q_v - sum_{j: i_j = v} p_j)   on the entries' tokens, w = sum p + p_rest,
 //             alpha T q_v (w - p_rest / q_rest)         elsewhere (without lse: alpha T q_v),
 //             + (1 - alpha) (softmax(s)_v - [v = y]).
-// p_rest is not negative: w is 1, or sum p where a rounded lse or a token given twice make that more than 1.
+// log q_rest and q_v / q_rest have the rest's own maximum as their reference where q_rest is below 2^-60 of the row.  Where
+// the entries cover the vocabulary there is no rest term; where the student has all other tokens at -inf it is infinite,
+// unless p_rest is below 1e-5, the rounding of 1 - sum p.  p_rest is not negative: w is 1, or sum p where a rounded lse or a token given twice make that more than 1.
 // A row whose label is ignore_index, or without labels a row without entries, counts nothing.
 //
 // One cluster of 1 to 8 CTAs per row, each holding its slice of the row in shared memory (bulk
@@ -43,6 +45,9 @@ static_assert(THREADS == 256, "bar_compute counts them");
 constexpr int MAX_TOP = 4096;
 constexpr int MAX_SMEM = 227 * 1024;
 constexpr int COUNT_CTAS = FF_DISTILL_WS_ELEMS;
+// a share below which the rest is summed relative to its own maximum: exponentials end at 2^-126, so a sum above this is
+// complete to 2^-60 of itself per token
+constexpr float kLittle = 8.673617379884035e-19f;  // 2^-60
 
 struct Args {
   const void* logits;
@@ -208,7 +213,8 @@ struct Part {
   float dot;      // sum over its entries of p (log p - (s - m)/T)
   float psum;     // sum of p over its entries
   float label;    // the label's logit where the label lies in the slice, else -inf
-  float pad;
+  float rest_m;   // what `rest` is relative to: m, or where that would leave next to nothing of it the largest logit of
+                  // the rest; without any rest -inf, or 0 where tokens are there but all of them at -inf
 };
 
 // shared memory: control, then K entries of 20 bytes, then the slice
@@ -550,19 +556,56 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
         }
         if (!grow) gemm::fence_proxy_async_smem();
         bar_compute();
+        float low = m;
+        rest = a.lse ? sum8(c.red[3]) : 0.f;
+        if (a.lse && rest < kLittle) {  // the same in every thread of the CTA
+          // The rest lies so far below m that its own exponentials are lost (or there is none): its sum once more,
+          // relative to its own maximum.
+          typename Vec<DT>::Max mr;
+          for (int k = tid; k < g.words; k += THREADS) mr.add(w[k]);
+          low = warp_max(mr.value());
+          if (lane == 0) c.red[0][warp] = low;
+          bar_compute();
+          low = max8(c.red[0]);
+          const auto rr = Ref<PW>::at_t(low, kT, k1);
+          rest = 0.f;
+          if (low != neg_inf()) {
+            f2 ar = splat(0.f);
+            for (int k = tid; k < g.words; k += THREADS) {
+              f2 v[P];
+              Vec<DT>::get(w[k], v);
+#pragma unroll
+              for (int e = 0; e < P; ++e) ar = add2(ar, ex2_2(fma2(v[e], splat(rr.mul()), splat(rr.add()))));
+            }
+            float p, q;
+            un2(ar, p, q);
+            rest = p + q;
+          } else {  // how many of the slice's tokens are entries
+            for (int j = tid; j < a.K; j += THREADS) rest += e_pos[j] >= 0 ? 1.f : 0.f;
+          }
+          rest = warp_sum(rest);
+          if (lane == 0) c.red[3][warp] = rest;
+          if (!grow) gemm::fence_proxy_async_smem();
+          bar_compute();
+          rest = sum8(c.red[3]);
+          if (low == neg_inf()) {
+            if (rest < (float)len) low = 0.f;  // tokens at -inf
+            rest = 0.f;
+          }
+        }
         if (!grow && ahead) {  // the slice has been read for the last time
           if (tid == 0) issue(gn, 0, gn.words);
           under_way = true;
         }
-        const Part mine = Part{m, sum8(c.red[1]), two ? sum8(c.red[2]) : 0.f, a.lse ? sum8(c.red[3]) : 0.f, sum8(c.red[4]),
-                               sum8(c.red[5]), c.label_logit, 0.f};
+        const Part mine = Part{m, sum8(c.red[1]), two ? sum8(c.red[2]) : 0.f, rest, sum8(c.red[4]),
+                               sum8(c.red[5]), c.label_logit, low};
         Part all = mine;
         if (csize > 1) {
           if (tid < csize * 8) {  // word tid % 8 of this CTA's part to CTA tid / 8
             const uint32_t dst = gemm::mapa_shared(gemm::smem_u32(&c.parts[par][rank]) + (tid & 7) * 4, (uint32_t)(tid >> 3));
             const float word = (tid & 7) == 0 ? mine.m : (tid & 7) == 1 ? mine.sum : (tid & 7) == 2 ? mine.sum1
                                : (tid & 7) == 3 ? mine.rest : (tid & 7) == 4 ? mine.dot : (tid & 7) == 5 ? mine.psum
-                               : (tid & 7) == 6 ? mine.label : 0.f;
+                               : (tid & 7) == 6 ? mine.label : mine.rest_m;
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst), "f"(word) : "memory");
           }
           __syncwarp();
@@ -579,7 +622,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
             const float f = any ? ex2(RT.log2_from(o)) : 1.f, f1 = any ? ex2(R1.log2_from(Ref<PW>::at_1(q.m, k1))) : 1.f;
             all.sum += q.sum * f;
             all.sum1 += q.sum1 * f1;
-            all.rest += q.rest * f;
+            all.rest += q.rest_m == q.m ? q.rest * f : q.rest > 0.f ? q.rest * ex2(RT.log2_from(Ref<PW>::at_t(q.rest_m, kT, k1))) : 0.f;
             all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot - (any ? q.psum * RT.log_from(o) : 0.f) : 0.f;
             all.psum += q.psum;
             all.label = fmaxf(all.label, q.label);
@@ -590,15 +633,44 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
         const float sum1_all = two ? all.sum1 : all.sum;
         const bool has = c.t_any[buf] != 0;
         if (!a.labels) live = has;
-        const float q_rest = all.rest / all.sum;
         float p_rest = a.lse && has ? fmaxf(1.f - c.t_sum[buf], 0.f) : 0.f;
-        if (q_rest == 0.f && p_rest < 1e-5f) p_rest = 0.f;  // nothing outside the entries: 1 - sum p is rounding
+        // ---- the rest bucket: q_rest, or where that is next to nothing its logarithm from the rest's own reference
+        float q_rest = 0.f, rest_m = neg_inf(), rest_sum = 0.f;
+        bool little = false;
+        if (a.lse) {
+          if (csize == 1 && low != m && rest > 0.f) all.rest = rest * ex2(RT.log2_from(Ref<PW>::at_t(low, kT, k1)));
+          q_rest = all.rest / all.sum;
+          little = q_rest < kLittle;  // (not for a NaN)
+        }
+        if (little) {
+          bool other = low != neg_inf();  // tokens outside the entries
+          rest_m = low;
+          rest_sum = rest;
+          if (csize > 1) {
+            const Part* q = c.parts[par ^ 1u];
+            rest_m = neg_inf();
+            rest_sum = 0.f;
+            for (int k = 0; k < csize; ++k) {
+              other |= q[k].rest_m != neg_inf();
+              if (q[k].rest > 0.f) rest_m = fmaxf(rest_m, q[k].rest_m);
+            }
+            const auto rr = Ref<PW>::at_t(rest_m, kT, k1);
+            for (int k = 0; k < csize; ++k)
+              if (q[k].rest > 0.f) rest_sum += q[k].rest * ex2(rr.log2_from(Ref<PW>::at_t(q[k].rest_m, kT, k1)));
+          }
+          // no other token: no bucket; none that the student can choose: 1 - sum p may be rounding alone
+          if (!other || (rest_sum == 0.f && p_rest < 1e-5f)) p_rest = 0.f;
+        }
         // ---- the loss
         if (a.row_loss && rank == 0 && tid == 0) {
           float kd = 0.f, ce = 0.f;
           if (has) {
             kd = all.dot + all.psum * logf(all.sum);
-            if (p_rest > 0.f) kd += p_rest * (logf(p_rest) - logf(q_rest));
+            if (p_rest > 0.f) {
+              float lq = logf(q_rest);
+              if (little) lq = rest_sum > 0.f ? RT.log_from(Ref<PW>::at_t(rest_m, kT, k1)) + (logf(rest_sum) - logf(all.sum)) : neg_inf();
+              kd += p_rest * (logf(p_rest) - lq);
+            }
             kd *= a.T * a.T;
           }
           if (label >= 0 && a.alpha != 1.f) ce = logf(sum1_all) - (two ? R1 : RT).log_of(all.label);
@@ -612,10 +684,17 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
           // log sum exp(s/T) stands in the loss with the weight sum p + p_rest: 1 unless the teacher's log-sum-exp is off
           const float mass = a.lse && p_rest == 0.f ? c.t_sum[buf] : 1.f;
           const float gq = mass * fk / all.sum, g1 = f1 / sum1_all;  // factors of exp(..) for q and the softmax at 1
-          const float gr = p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;  // q outside the entries
+          // Outside the entries: q (1 - p_rest / q_rest).  With next to no q there, q itself is nothing beside
+          // p_rest q / q_rest, and that is formed from the rest's own reference; so is then what the softmax at 1
+          // takes from the same exponentials.
+          const bool own = little && p_rest > 0.f && rest_sum > 0.f;
+          const auto GT = own ? Ref<PW>::at_t(rest_m, kT, k1) : RT;
+          const float gr = own ? -(fk * p_rest / rest_sum) : p_rest > 0.f && q_rest > 0.f ? gq * (1.f - p_rest / q_rest) : gq;
+          const float g1r = !own || PW == 0 ? g1
+                            : g1 * ex2(PW == 1 ? RT.log2_from(GT) : R1.log2_from(Ref<PW>::at_1(rest_m, k1)));
           const bool vec = (reinterpret_cast<uintptr_t>(grow) & 15u) == (uint32_t)g.mis;
-          const f2 kT2 = splat(RT.mul()), nT2 = splat(RT.add()), k12 = splat(R1.mul()), n12 = splat(R1.add()), gr2 = splat(two ? gr : gr + g1),
-                   g12 = splat(g1);
+          const f2 kT2 = splat(GT.mul()), nT2 = splat(GT.add()), k12 = splat(R1.mul()), n12 = splat(R1.add()),
+                   gr2 = splat(two ? gr : gr + g1r), g12 = splat(g1r);
           const int step = (max(g.words, gn.words) + 2 * THREADS - 1) / (2 * THREADS) * THREADS;
           uint4* gw = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(grow) - g.mis);  // word k of the slice
           auto grad_word = [&](int k) {
@@ -674,8 +753,8 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
             grow[pos] = from_f32<DT>(gv);
           }
           if (tid == 0 && label >= v0 && label < v0 + len && !c.label_in_top[buf]) {
-            const float x = ex2(RT.log2_of(c.label_logit));
-            grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(R1.log2_of(c.label_logit)) : (gr + g1) * x) - f1);
+            const float x = ex2(GT.log2_of(c.label_logit));
+            grow[label - v0] = from_f32<DT>((two ? gr * x + g1 * ex2(R1.log2_of(c.label_logit)) : (gr + g1r) * x) - f1);
           }
         }
       }

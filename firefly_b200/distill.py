@@ -64,7 +64,8 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     teacher_ids, teacher_logits [..., k]: the teacher's top tokens and logits; an entry with a negative id or
     a logit of -inf is absent, a token given twice counts with both entries.  p = softmax(teacher_logits / T)
     over the entries; with ``teacher_lse`` [...], the teacher's ``logsumexp(logits / T)`` over its whole
-    vocabulary, p are its true probabilities and the rest of the mass is one bucket for all other tokens.
+    vocabulary, p are its true probabilities and the rest of the mass is one bucket for all other tokens (none if the
+    entries cover the vocabulary; infinitely far from a student that has every other token at -inf).
     labels [...]: hard labels; a row with ``ignore_index`` counts nothing.  Without labels only the first
     term is left, and a row without entries counts nothing.
     reduction: "mean" over the rows that count (0 if none does), "sum", or "none" (a loss per row).

@@ -668,3 +668,94 @@ def test_a_masked_label_and_a_masked_entry(V, dtype):
     two = s.scatter(1, ids[:, :1], torch.finfo(dtype).min)
     _check_each(two, ids, t)
     _check_each(two, ids, t, None, torch.logsumexp(t.double(), 1).float() + 0.1)
+
+
+@pytest.mark.parametrize("n,V", [(5, 131071), (3, 250007), (6, 2001)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rest_bucket_gradient_of_every_token(n, V, dtype):
+    """Of nearly all the tokens outside the entries the gradient is larger than its bound, so none can be missing."""
+    for T in (1.0, 2.0, 4.0):
+        s, ids, t, lab, lse = _case(n, V, 100, V, dtype=dtype, labels=True, tail=True, T=T, pad=False)
+        seen = _check_each(s, ids, t, None, lse, T)
+        if dtype == torch.float32:  # (fp16 gradients of a long row are below the type's smallest steps)
+            assert seen > 0.95
+        _check_each(s, ids, t, lab, lse, T, 0.5)
+
+
+def _far_rest(n, V, k, seed, T, dtype, gap):
+    """A student that is sure of the teacher's tokens: every other logit lies about ``gap`` below them, while
+    the teacher leaves a tenth of its mass there."""
+    s, ids, t, lab, _ = _case(n, V, k, seed, labels=True, pad=False, dtype=torch.float32)
+    s = s.scatter(1, ids, s.gather(1, ids) + gap)
+    lse = torch.logsumexp(t.double() / T, 1).float() + 0.1
+    return s.to(dtype), ids, t, lab, lse
+
+
+@pytest.mark.parametrize("n,V", [(6, 700), (3, 40000)])
+@pytest.mark.parametrize("T,gap", [(1e-2, 10.0), (0.1, 30.0), (0.7, 100.0), (1.0, 80.0), (1.0, 200.0), (1.0, 1e4), (2.0, 400.0),
+                                   (3.0, 1000.0), (4.0, 1000.0)])
+def test_rest_bucket_far_below_the_entries(n, V, T, gap):
+    for dtype in (torch.float32, torch.bfloat16):
+        s, ids, t, lab, lse = _far_rest(n, V, 9, 31, T, dtype, gap)
+        _check_each(s, ids, t, None, lse, T)
+        for label in (lab, ids[:, 0].contiguous()):  # outside the entries, mostly, and among them
+            _check_each(s, ids, t, label, lse, T, 0.5)
+        ids = ids.clone()
+        ids[:, 4] = ids[:, 1]  # a token in two entries
+        _check_each(s, ids, t, lab, lse, T, 0.25)
+
+
+@pytest.mark.parametrize("V", [700, 40000])
+def test_rest_bucket_masked_in_the_student(V):
+    """Tokens outside the entries masked by -1e4 or the type's lowest value are still there, by -inf they are not: a rest that
+    the teacher keeps costs infinitely much then, and one that is only the rounding of 1 - sum p nothing."""
+    s, ids, t, _, _ = _case(4, V, 9, 32, pad=False, dtype=torch.float32)
+    exact = torch.logsumexp(t.double(), 1).float()
+    out = torch.ones_like(s, dtype=torch.bool).scatter_(1, ids, False)
+    _check_each(s.masked_fill(out, -1e4), ids, t, None, exact + 0.1)
+    far = s.masked_fill(out, -1e30).requires_grad_(True)  # 64 bits do not hold log R beside 1e30: the R tokens are equal, so
+    row = distillation_loss(far, ids, t, teacher_lse=exact + 0.1, reduction="none")  # each gets -p_rest / R
+    p = torch.exp(t.double() - (exact + 0.1).double()[:, None])
+    pr = 1 - p.sum(1)
+    # p_rest within 2^-18 (nine logits below 20, each rounded to 2^-24 of itself, nine exponentials)
+    assert bool(((row.double() / (pr * 1e30) - 1).abs() <= 2.0 ** -18 / pr).all())
+    row.sum().backward()
+    want = (-pr / out.sum(1))[:, None].expand_as(s)
+    assert bool(((far.grad - want)[out].abs() <= (2.0 ** -18 / out.sum(1))[:, None].expand_as(s)[out]).all())
+    q = torch.softmax(s.gather(1, ids).double(), 1)
+    assert bool(((far.grad.gather(1, ids) - (q - p)).abs() <= 2.0 ** -18).all())
+    gone = s.masked_fill(out, -math.inf)
+    x = gone.clone().requires_grad_(True)
+    rows = distillation_loss(x, ids, t, teacher_lse=exact + 0.1, reduction="none")
+    assert bool((rows == math.inf).all())
+    rows = distillation_loss(x, ids, t, teacher_lse=exact, reduction="none")
+    near = distillation_loss(x, ids, t, reduction="none")
+    # sum p is 1 to 2^-20: so are the losses, of logits below 20
+    assert bool(((rows - near).abs() <= 2.0 ** -20 * 64).all())
+    rows.sum().backward()
+    assert torch.isfinite(x.grad).all() and not x.grad[out].any()
+
+
+@pytest.mark.parametrize("off", [-0.05, 0.05, 0.0])
+@pytest.mark.parametrize("V", [1, 40, 1000, 4096])
+def test_entries_that_cover_the_vocabulary_leave_no_rest(V, off):
+    """No token is outside the entries: the bucket is empty whatever 1 - sum p says (a teacher's lse of 16 bits)."""
+    s, ids, t, lab, _ = _case(3, V, V, 33, labels=True, pad=False)
+    lse = torch.logsumexp(t.double(), 1).float() + off
+    _check_each(s, ids, t, None, lse)
+    _check_each(s, ids, t, lab, lse, 1.0, 0.5)
+
+
+@pytest.mark.parametrize("T", [0.01, 0.7, 1.0, 2.0, 4.0])
+@pytest.mark.parametrize("mask", [-1e10, "lowest"])
+def test_rest_bucket_over_whole_masked_slices(mask, T):
+    for dtype in (torch.float32, torch.bfloat16):
+        s, ids, t, lab, _ = _case(4, 32768, 8, 44, labels=True, pad=False)
+        ids, lab = ids % 16000, torch.where(lab >= 0, lab % 16000, lab)
+        s = s.to(dtype)
+        s[:, 16384:] = torch.finfo(dtype).min if mask == "lowest" else mask
+        lse = torch.logsumexp(t.double() / T, 1).float() + 0.1
+        _check_each(s, ids, t, None, lse, T)
+        _check_each(s, ids, t, lab, lse, T, 0.5)
+        s[1] = s[1, -1]  # nothing but the mask
+        _check_each(s, ids, t, None, lse, T)
