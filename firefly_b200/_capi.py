@@ -12,6 +12,7 @@ import ctypes
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libfirefly_b200.so"
 
@@ -221,6 +222,14 @@ def _addr(t: torch.Tensor | None):
 def _raw_stream(dev: torch.device) -> int:
     """torch's current stream of ``dev`` as an address."""
     return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def has_tangent(*tensors: torch.Tensor | None) -> bool:
+    """Whether one of the tensors carries a forward-mode tangent."""
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            return True
+    return False
 
 
 def capture_id(dev: torch.device) -> int:

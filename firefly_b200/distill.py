@@ -99,8 +99,9 @@ def distillation_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     lab = None if labels is None else labels.reshape(-1).contiguous()
     lse = None if teacher_lse is None else teacher_lse.reshape(-1).to(torch.float32).contiguous()
     args = (_rows(logits, V), _rows(teacher_ids, k), _rows(teacher_logits, k), lab, lse, temperature, alpha, int(ignore_index))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        out = DistillationLossFn.apply(*args, reduction, True)
+    grad = torch.is_grad_enabled() and logits.requires_grad
+    if grad or _capi.has_tangent(logits, teacher_logits, teacher_lse):  # (a tangent is refused there)
+        out = DistillationLossFn.apply(*args, reduction, grad)
     else:
         row, loss, *_ = _capi.distill_loss(_capi.distill_rows(*args), args[0], reduction, False)
         out = row if reduction == "none" else loss

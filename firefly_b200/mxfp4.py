@@ -298,7 +298,7 @@ def mxfp4_linear(x: torch.Tensor, weight: "torch.Tensor | MXFP4Tensor", bias: to
         raise ValueError(f"bias must have shape ({O},), got {tuple(bias.shape)}")
     grad = torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
                                         or (bias is not None and bias.requires_grad))
-    if not grad and packed is not None and x2.shape[0] > 0:
+    if not grad and packed is not None and x2.shape[0] > 0 and not _capi.has_tangent(x, bias):  # (refused by the function)
         y = _capi.mxfp4_linear(_matrix(x2, "x"), packed._pair(), O, K, None if bias is None else _bias(bias, O))
     else:
         y = MXFP4LinearFn.apply(x2, w, bias, packed, grad)
@@ -318,7 +318,7 @@ def mxfp4_swiglu(x: torch.Tensor, gate_up: "torch.Tensor | MXFP4Tensor", down: "
     x2 = _check_input(x, K, gate_up, down)
     grad = torch.is_grad_enabled() and (x.requires_grad or (wgu is not None and wgu.requires_grad)
                                         or (wd is not None and wd.requires_grad))
-    if not grad and pgu is not None and pd is not None and F % 128 == 0 and x2.shape[0] > 0:
+    if not grad and pgu is not None and pd is not None and F % 128 == 0 and x2.shape[0] > 0 and not _capi.has_tangent(x):
         y = _capi.mxfp4_swiglu_mlp(_matrix(x2, "x"), pgu._pair(), pd._pair(), F, O)
     else:
         y = MXFP4SwiGLUFn.apply(x2, wgu, wd, (pgu, pd), grad)

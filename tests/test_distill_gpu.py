@@ -759,3 +759,15 @@ def test_rest_bucket_over_whole_masked_slices(mask, T):
         _check_each(s, ids, t, lab, lse, T, 0.5)
         s[1] = s[1, -1]  # nothing but the mask
         _check_each(s, ids, t, None, lse, T)
+
+
+def test_forward_mode_is_refused_as_by_the_other_layers():
+    """There is no forward-mode derivative: a tangent is refused and not lost, with or without ``requires_grad``."""
+    from torch.autograd import forward_ad
+
+    s, ids, t, _, _ = _case(3, 50, 4, 41, dtype=torch.float32)
+    for x in (s, s.clone().requires_grad_(True)):
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward"):
+                distillation_loss(forward_ad.make_dual(x, torch.ones_like(x)), ids, t)
+            assert torch.equal(distillation_loss(s, ids, t), distillation_loss(s.clone(), ids, t))  # no tangent: as ever

@@ -571,3 +571,21 @@ def test_training_step_captured_and_replayed():
         got = [t.clone() for t in out]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)
+
+
+def test_forward_mode_is_refused_as_by_the_other_layers():
+    """There is no forward-mode derivative: a tangent is refused and not lost, on held weights too."""
+    from torch.autograd import forward_ad
+
+    x, w, wgu, wd = _randn(3, 64, 1), _randn(8, 64, 2), _randn(256, 64, 3), _randn(8, 128, 4)
+    held = [quantize_fp_to_mxfp4(v) for v in (w, wgu, wd)]
+    want = mxfp4_linear(x, held[0]), mxfp4_swiglu(x, *held[1:])
+    bias = torch.zeros(8, device=DEV)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        b = forward_ad.make_dual(bias, torch.ones_like(bias))
+        for call in (lambda: mxfp4_linear(d, held[0]), lambda: mxfp4_swiglu(d, *held[1:]), lambda: mxfp4_linear(d, w),
+                     lambda: mxfp4_swiglu(d, wgu, wd), lambda: mxfp4_linear(x, held[0], b)):
+            with pytest.raises(RuntimeError, match="forward"):
+                call()
+        assert torch.equal(mxfp4_linear(x, held[0]), want[0]) and torch.equal(mxfp4_swiglu(x, *held[1:]), want[1])
