@@ -189,16 +189,16 @@ struct Ref {
   // one value's exponential in log2 and as (s - m)/T: the multiply-add's, and where that says no more than "far below"
   // (a masked label or entry has a finite loss), the difference
   __device__ __forceinline__ float log2_of(float s) const { return far ? (s - m) * k : fmaf(s, k, add()); }
-  __device__ __forceinline__ float log_of(float s) const {
-    const float z = log2_of(s);
-    return far || z == neg_inf() ? (s - m) * kLn2 * k : z * kLn2;
+  __device__ __forceinline__ float log_at(float s, float z) const {
+    if (__builtin_expect(far || z == neg_inf(), 0)) return (s - m) * kLn2 * k;
+    return z * kLn2;
   }
+  __device__ __forceinline__ float log_of(float s) const { return log_at(s, log2_of(s)); }
   // log2 of the factor from sums relative to `o` to sums relative to this one: the difference of the two rounded
   // products (not contracted into one multiply-add, which would leave the rounding of m k in the sums: 2^-14 for
   // |m| / T of 1000)
-  __device__ __forceinline__ float log2_from(const Ref& o) const {
-    return far || o.far ? (o.m - m) * k : __fsub_rn(__fmul_rn(o.m, k), __fmul_rn(m, k));
-  }
+  __device__ __forceinline__ float near_log2_from(const Ref& o) const { return __fsub_rn(__fmul_rn(o.m, k), __fmul_rn(m, k)); }
+  __device__ __forceinline__ float log2_from(const Ref& o) const { return far || o.far ? (o.m - m) * k : near_log2_from(o); }
   __device__ __forceinline__ float log_from(const Ref& o) const {
     return far || o.far ? (o.m - m) * kLn2 * k : log2_from(o) * kLn2;
   }
@@ -508,7 +508,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
           const int pos = e_pos[j];
           if (pos == -1 || pos == -2) continue;
           const float z = rT.log2_of(e_s[j]), p = expf(e_p[j]);
-          if (p > 0.f) dot += p * (e_p[j] - rT.log_of(e_s[j]));
+          if (p > 0.f) dot += p * (e_p[j] - rT.log_at(e_s[j], z));
           else if (p != p) dot = p;
           psum += p;
           if (pos >= 0) {
@@ -611,19 +611,32 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
           __syncwarp();
           gemm::cluster_sync_all();
           all = c.parts[par][0];
-          for (int k = 1; k < csize; ++k) all.m = fmaxf(all.m, c.parts[par][k].m);
+          bool odd = false;  // references that are far, or a rest with one of its own
+          for (int k = 0; k < csize; ++k) {
+            const float qm = c.parts[par][k].m;
+            all.m = fmaxf(all.m, qm);
+            odd |= Ref<PW>::at_t(qm, kT, k1).far || (PW == 0 && Ref<PW>::at_1(qm, k1).far) || (a.lse && c.parts[par][k].rest_m != qm);
+          }
           const auto RT = Ref<PW>::at_t(all.m, kT, k1), R1 = Ref<PW>::at_1(all.m, k1);
           all.sum = all.sum1 = all.rest = all.dot = all.psum = 0.f;
           all.label = neg_inf();
           for (int k = 0; k < csize; ++k) {
             const Part q = c.parts[par][k];
-            const auto o = Ref<PW>::at_t(q.m, kT, k1);
             const bool any = q.m != neg_inf();
-            const float f = any ? ex2(RT.log2_from(o)) : 1.f, f1 = any ? ex2(R1.log2_from(Ref<PW>::at_1(q.m, k1))) : 1.f;
+            auto o = Ref<PW>::at_t(q.m, kT, k1), o1 = Ref<PW>::at_1(q.m, k1);
+            float d = any ? RT.near_log2_from(o) : 0.f, d1 = any ? R1.near_log2_from(o1) : 0.f, dl = d * kLn2;
+            if (odd && any) {
+              d = RT.log2_from(o);
+              d1 = R1.log2_from(o1);
+              dl = RT.log_from(o);
+            }
+            const float f = ex2(d);
+            float rest_q = q.rest * f;
+            if (odd && q.rest_m != q.m) rest_q = q.rest > 0.f ? q.rest * ex2(RT.log2_from(Ref<PW>::at_t(q.rest_m, kT, k1))) : 0.f;
             all.sum += q.sum * f;
-            all.sum1 += q.sum1 * f1;
-            all.rest += q.rest_m == q.m ? q.rest * f : q.rest > 0.f ? q.rest * ex2(RT.log2_from(Ref<PW>::at_t(q.rest_m, kT, k1))) : 0.f;
-            all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot - (any ? q.psum * RT.log_from(o) : 0.f) : 0.f;
+            if (two) all.sum1 += q.sum1 * ex2(d1);
+            all.rest += rest_q;
+            all.dot += q.psum != 0.f || q.dot != 0.f ? q.dot - q.psum * dl : 0.f;
             all.psum += q.psum;
             all.label = fmaxf(all.label, q.label);
           }
