@@ -589,3 +589,68 @@ def test_forward_mode_is_refused_as_by_the_other_layers():
             with pytest.raises(RuntimeError, match="forward"):
                 call()
         assert torch.equal(mxfp4_linear(x, held[0]), want[0]) and torch.equal(mxfp4_swiglu(x, *held[1:]), want[1])
+
+
+# ---------------------------------------------------------------------------
+# the one-call training passes against their parts
+# ---------------------------------------------------------------------------
+def _tensor(pair, shape):
+    return MXFP4Tensor(*pair, shape)
+
+
+def _within(got, a, b, dtype):
+    """Whether got is the product of two value matrices within the accumulation error."""
+    v, mag = O.product(a, b)
+    return bool(((got.double() - v).abs() <= _tolerance(v, mag, a.shape[1], dtype)).all())
+
+
+@pytest.mark.parametrize("T,K,F,N", [(1, 64, 128, 96), (3, 256, 32, 40), (16, 512, 384, 512), (40, 100, 160, 77),
+                                     (130, 256, 256, 300), (300, 320, 640, 256), (513, 512, 128, 260), (1300, 512, 1152, 640),
+                                     (100, 4096, 128, 64), (20, 700, 1408, 90)])
+def test_gated_training_step_equals_its_parts(T, K, F, N):
+    """The block's forward and backward bit for bit from the quantisers and the product, each product against fp64 on the codes
+    that went into it; the same bound refuses a gradient of zeros and one with gate and up exchanged."""
+    x, dy = _randn(T, K, 1).requires_grad_(True), _randn(T, N, 4, scale=1e-2)
+    wgu, wd = _randn(2 * F, K, 2, scale=0.05).requires_grad_(True), _randn(N, F, 3, scale=0.05).requires_grad_(True)
+    y = mxfp4_swiglu(x, wgu, wd)
+    y.backward(dy)
+    (qx, qxt), (qgu, qgut), (qd, qdt), (qy, qyt) = (quantize_fp_to_mxfp4_dual(m.detach()) for m in (x, wgu, wd, dy))
+    gu = mxfp4_matmul(qx, qgu)
+    rows, cols = _capi.mxfp4_swiglu_quant(gu, cols=True)
+    h, ht = _tensor(rows, (T, F)), _tensor(cols, (F, T))
+    dh = mxfp4_matmul(qy, qdt)
+    rows, cols = _capi.mxfp4_swiglu_bwd_quant(dh, gu)
+    p, pt = _tensor(rows, (T, 2 * F)), _tensor(cols, (2 * F, T))
+    assert torch.equal(y, mxfp4_matmul(h, qd))
+    for got, a, b in ((x.grad, p, qgut), (wgu.grad, pt, qxt), (wd.grad, qyt, ht)):
+        assert torch.equal(got, mxfp4_matmul(a, b))
+        av, bv = a.dequantize(torch.float32).double(), b.dequantize(torch.float32).double()
+        assert _within(got, av, bv, torch.bfloat16)
+        assert not _within(torch.zeros_like(got), av, bv, torch.bfloat16)
+    swapped = p.dequantize(torch.float32).double()
+    swapped = torch.cat([swapped[:, F:], swapped[:, :F]], 1)
+    back = qgut.dequantize(torch.float32).double()
+    assert not _within(x.grad, swapped, back, torch.bfloat16)
+    assert not _within(wgu.grad, swapped.t(), qxt.dequantize(torch.float32).double(), torch.bfloat16)
+    assert _capi.device_status() == 0
+
+
+@pytest.mark.parametrize("need", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1), (1, 0, 1)])
+def test_gradients_of_some_inputs_equal_those_of_all(need):
+    T, K, F, N = 70, 256, 192, 130
+    args = [_randn(T, K, 1), _randn(2 * F, K, 2, scale=0.05), _randn(N, F, 3, scale=0.05)]
+    dy = _randn(T, N, 4)
+    leaves = [a.clone().requires_grad_(True) for a in args]
+    every = torch.autograd.grad(mxfp4_swiglu(*leaves), leaves, dy)
+    some = [a.clone().requires_grad_(bool(k)) for a, k in zip(args, need)]
+    got = torch.autograd.grad(mxfp4_swiglu(*some), [a for a, k in zip(some, need) if k], dy)
+    for a, b in zip(got, [g for g, k in zip(every, need) if k]):
+        assert torch.equal(a, b)
+    lin = [args[0], args[1], torch.randn(2 * F, device=DEV, generator=_gen(5))]
+    dy = _randn(T, 2 * F, 6)
+    leaves = [a.clone().requires_grad_(True) for a in lin]
+    every = torch.autograd.grad(mxfp4_linear(*leaves), leaves, dy)
+    some = [a.clone().requires_grad_(bool(k)) for a, k in zip(lin, need)]
+    got = torch.autograd.grad(mxfp4_linear(*some), [a for a, k in zip(some, need) if k], dy)
+    for a, b in zip(got, [g for g, k in zip(every, need) if k]):
+        assert torch.equal(a, b)
