@@ -654,3 +654,36 @@ def test_gradients_of_some_inputs_equal_those_of_all(need):
     got = torch.autograd.grad(mxfp4_linear(*some), [a for a, k in zip(some, need) if k], dy)
     for a, b in zip(got, [g for g, k in zip(every, need) if k]):
         assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# layers made from trained ones
+# ---------------------------------------------------------------------------
+def test_layers_from_trained_int8_layers():
+    from firefly_b200 import BitLinear
+    from firefly_b200.swiglu import SwiGLUMLP
+
+    lin = BitLinear(96, 40, bias=True).to(DEV)
+    with torch.no_grad():
+        lin.bias.normal_(generator=_gen(1))
+    x, dy = _randn(9, 96, 2).requires_grad_(True), _randn(9, 40, 3)
+    w = lin.int_weight.float() * lin.weight_scale[:, None]
+    held = MXFP4Linear.from_bitlinear(lin, input_grad=True)
+    want = mxfp4_linear(x, w, lin.bias.detach())
+    assert torch.equal(held(x), want)
+    assert torch.equal(*(torch.autograd.grad(y, x, dy)[0] for y in (held(x), want)))
+    with torch.no_grad():
+        lin.bias.add_(1.0)  # the held layer has its own
+    assert torch.equal(held(x), want) and not list(held.parameters())
+    with pytest.raises(ValueError, match="transposed"):
+        MXFP4Linear.from_bitlinear(lin)(x)
+    mlp = SwiGLUMLP(64, 96).to(DEV)
+    blk = MXFP4SwiGLU.from_swiglu_mlp(mlp, input_grad=True)
+    x, dy = _randn(2, 5 * 64, 4).view(2, 5, 64).requires_grad_(True), _randn(2, 5 * 64, 5).view(2, 5, 64)
+    ws = [m.int_weight.float() * m.weight_scale[:, None] for m in (mlp.gate_up, mlp.down)]
+    want = mxfp4_swiglu(x, *ws)
+    assert torch.equal(blk(x), want)
+    assert torch.equal(*(torch.autograd.grad(y, x, dy)[0] for y in (blk(x), want)))
+    mlp.down = BitLinear(96, 64, bias=True).to(DEV)
+    with pytest.raises(ValueError, match="bias"):
+        MXFP4SwiGLU.from_swiglu_mlp(mlp)
