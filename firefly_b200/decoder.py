@@ -207,9 +207,11 @@ class DecoderLayer(nn.Module):
         self.fused = fused
 
     def mlp(self, x: torch.Tensor) -> torch.Tensor:
-        """down(gelu(up(x))): the fused GELU MLP op, or the composition of the two BitLinear
-        layers and torch's GELU (``fused=False``, an up bias, or ffn not a multiple of 32)."""
-        if self.fused and self.up.bias is None and self.up.out_features % 32 == 0:
+        """down(gelu(up(x))): the fused GELU MLP op, or the composition of the two layers and torch's
+        GELU (``fused=False``, an up bias, ffn not a multiple of 32, or another layer, such as an
+        ``MXFP4Linear``, in the place of a BitLinear)."""
+        int8 = isinstance(self.up, BitLinear) and isinstance(self.down, BitLinear)
+        if self.fused and int8 and self.up.bias is None and self.up.out_features % 32 == 0:
             y = GeluMLPFn.apply(x.reshape(-1, x.shape[-1]), self.up.int_weight, self.up.weight_scale,
                                 self.up._registered_handle, self.down.int_weight, self.down.weight_scale,
                                 self.down.bias, self.down._registered_handle)

@@ -18,8 +18,9 @@ ops computes, with the elementwise work moved into the quantisers:
   it (otherwise ``ff_swiglu_bwd_quant_i8`` does that from dh); ``dX`` is one GEMM over
   ``K = 2f``.
 
-The unfused composition (``fused=False``, or ffn not a multiple of 8) runs the same
-BitLinear kernels with torch's elementwise ops in between.
+The unfused composition (``fused=False``, ffn not a multiple of 8, or another layer, such as an
+``MXFP4Linear``, in the place of a BitLinear) runs the layers' own kernels with torch's
+elementwise ops in between.
 """
 from __future__ import annotations
 
@@ -120,7 +121,8 @@ class SwiGLUMLP(nn.Module):
         self.fused = fused
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        if self.fused and self.ffn % 8 == 0:
+        int8 = isinstance(self.gate_up, BitLinear) and isinstance(self.down, BitLinear)
+        if self.fused and int8 and self.ffn % 8 == 0:
             if x.shape[-1] != self.gate_up.in_features:
                 raise ValueError(f"expected input last dim {self.gate_up.in_features}, got {x.shape[-1]}")
             y = SwiGLUMLPFn.apply(x.reshape(-1, x.shape[-1]), self.gate_up.int_weight,

@@ -687,3 +687,45 @@ def test_layers_from_trained_int8_layers():
     mlp.down = BitLinear(96, 64, bias=True).to(DEV)
     with pytest.raises(ValueError, match="bias"):
         MXFP4SwiGLU.from_swiglu_mlp(mlp)
+
+
+def test_a_trained_decoder_runs_in_four_bits():
+    """MXFP4 layers in the places of a decoder's (and a SwiGLU block's) int8 layers, all of them or one: the fused int8
+    operators step aside, and the result is that of the layers one after another."""
+    from firefly_b200.decoder import DecoderConfig, build_decoder
+    from firefly_b200.swiglu import SwiGLUMLP
+    from torch.nn import functional as F
+
+    cfg = DecoderConfig(vocab=96, d_model=64, heads=2, ffn=128, layers=2, max_seq=16)
+    model = build_decoder(cfg, DEV, seed=1)
+    ids = torch.randint(0, cfg.vocab, (2, 16), device=DEV, generator=_gen(2))
+    with torch.no_grad():
+        before = model(ids)
+    for names in (("up",), ("down",), ("qkv", "proj", "up", "down")):
+        model = build_decoder(cfg, DEV, seed=1)
+        for layer in model.layers:
+            for name in names:
+                setattr(layer, name, MXFP4Linear.from_bitlinear(getattr(layer, name), input_grad=True))
+        got = model(ids)
+        assert got.shape == before.shape and torch.isfinite(got).all()
+        layer = model.layers[0]
+        x = _randn(2, 16 * 64, 3, scale=0.1).view(2, 16, 64).requires_grad_(True)
+        y = layer.mlp(x)
+        ref = layer.down(F.gelu(layer.up(x), approximate="tanh"))
+        assert torch.equal(y, ref)
+        dy = _randn(2, 16 * 64, 4).view(2, 16, 64)
+        assert torch.equal(*(torch.autograd.grad(t, x, dy)[0] for t in (y, ref)))
+    model.lm_head = MXFP4Linear.from_bitlinear(model.lm_head)
+    with torch.no_grad():
+        top = model(ids).float().topk(8, dim=-1)
+    student = build_decoder(cfg, DEV, seed=3)
+    student.distill_loss(ids, ids, top.indices, top.values).backward()
+    for lin in student.bit_modules():
+        assert lin.consume_weight_grad() is not None
+    mlp = SwiGLUMLP(64, 128).to(DEV)
+    x = _randn(5, 64, 5)
+    for name in ("gate_up", "down"):
+        setattr(mlp, name, MXFP4Linear.from_bitlinear(getattr(mlp, name)))
+        with torch.no_grad():
+            g, u = mlp.gate_up(x).chunk(2, dim=-1)
+            assert torch.equal(mlp(x), mlp.down(F.silu(g) * u))
