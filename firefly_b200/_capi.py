@@ -225,11 +225,11 @@ def _raw_stream(dev: torch.device) -> int:
 
 
 def has_tangent(*tensors: torch.Tensor | None) -> bool:
-    """Whether one of the tensors carries a forward-mode tangent."""
-    for t in tensors:
-        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-            return True
-    return False
+    """Whether one of the tensors carries a forward-mode tangent (nothing is looked at outside a dual level: the
+    smallest calls are bound by the host)."""
+    if forward_ad._current_level < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def capture_id(dev: torch.device) -> int:
