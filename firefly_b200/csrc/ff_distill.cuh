@@ -25,8 +25,8 @@
 // works out the next row's entries.
 // Maxima, sums and probabilities are fp32; the gradient is rounded once.
 //
-// Measured: 16384 x 32000 bf16 (T = 2, labels, gradient) 426 us, its bytes 322 us at copy speed; 1500 x 131071
-// (clusters of four) 207 us, its bytes 120 us; 64 x 32000 fp32 without gradient 7 us.  Three rows at a time are
+// Measured (a call's three launches): 16384 x 32000 bf16 (T = 2, labels, gradient) 438 us, its bytes 322 us at copy
+// speed; 1500 x 131071 (clusters of four) 225 us, its bytes 120 us; 64 x 32000 fp32 without gradient 7 us.  Three rows at a time are
 // in different phases on an SM, and neither the exponentials (half of the special-function unit's rate) nor the
 // copies nor the stores bound it alone: leaving out either pass over the slice takes off about a quarter.  With
 // the first version's separate phases, and exponentials of their own at both temperatures, 770 us; with 384 or

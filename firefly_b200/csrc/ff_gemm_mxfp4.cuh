@@ -40,7 +40,7 @@ struct Epi {
   int out_f32;
   int vec;        // 16-byte stores of rows allowed
   int tma_store;  // bf16 output through TMA (pair kernel)
-  // SwiGLU epilogue: codes and scales of h [M, F] and, when gu is given, the activations [g | u] in bf16
+  // SwiGLU epilogue: codes and scales of h [M, F]
   uint8_t* hq;
   uint8_t* hs;
   int64_t ldh, hchunks, F;
@@ -889,7 +889,7 @@ inline int narrow_clusters(int csize) {
 // arrive from HBM; 0.84 us with gate and up rows), and the cluster size that gives it.  A CTA takes
 // `turns` items of `kbs` k-blocks; the exchange of a turn runs beside the next turn's k-blocks, the last
 // one after them.  Measured on 1 to 128 rows, 512 to 22016 x 1024 to 11008, clusters of 1 to 8: an
-// exchange takes 5 + rows/16 (9/c + 1) k-blocks, e.g. 2.9 us for one row and 14 us for 128 in clusters
+// exchange takes 5 + rows/16 (9/c + 1) k-blocks, e.g. 2.3 us for one row and 14 us for 128 in clusters
 // of 4; clusters of 1 need none (a local one for the activation).
 template <int MP, int NW>
 inline double narrow_cost(const Epi& ep, int64_t K, int* csize, int* clusters) {

@@ -14,8 +14,10 @@
 // Layout: codes [rows, ld bytes] with the blocks of a row in order (16 bytes each); scales in
 // chunks of 512 bytes that cover 128 rows x 4 blocks, the order in which the tensor core takes
 // them: byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4 of chunk
-// (row / 128) * chunks + block / 4, chunks = 2 * ceil(cols / 256).  Chunks of the padding hold
-// S = 0 (a finite scale for the zero codes that a tile load fills in).
+// (row / 128) * chunks + block / 4, chunks = 2 * ceil(cols / 256).  Blocks behind a row's last hold
+// S = 0 (a finite scale for the zero codes that a tile load fills in).  The bytes of rows behind the
+// matrix's last (up to the next 128) are 0 from ff_mxfp4_quant; from the SwiGLU kernels some are not
+// written: they scale rows of a product that are not stored.
 #pragma once
 
 #include "ff_common.cuh"
@@ -360,8 +362,9 @@ __global__ void __launch_bounds__(THREADS, DT == FF_DTYPE_F32 ? 2 : 4) mx_quant_
 // The same for 16-bit inputs whose rows are 16-byte aligned: persistent CTAs, three per SM, each with two
 // tile buffers, so that the next tile arrives (cp.async) while one is quantised.
 // 8192 x 4096 bf16, both orientations: 27 us with 3.8 TB/s of algorithmic bytes (30 us with one tile per CTA; a
-// copy of as many bytes takes 18 us); along the rows alone 21 us.  Instruction issue bounds it: 14.8 instructions
-// per value for both orientations, the ALU pipe 63% busy.
+// copy of as many bytes takes 18 us); along the rows alone 21 us.  No unit is full (14.8 instructions
+// per value for both orientations, issue slots 64% and the ALU pipe 63% busy): a tile's wait, its rows and its columns
+// follow one another between barriers, with 20 warps on an SM to fill the gaps.
 template <int DT>
 __host__ __device__ constexpr int pipe_smem() {
   return 2 * TILE * row_bytes<DT>() + TILE * 4 + 4 * TILE * 4;
@@ -410,8 +413,10 @@ __global__ void __launch_bounds__(THREADS, 3) mx_quant_pipe_kernel(const void* x
   }
 }
 
-// sigmoid(g) = 1 / (1 + 2^(-g log2 e)) in fp32, on the special-function unit (relative error below
-// 2^-20 for the |g| where it is not 0 or 1): exact at both ends (2^.. = inf gives 0, and 0 gives 1)
+// sigmoid(g) = 1 / (1 + 2^(-g log2 e)) in fp32, on the special-function unit: exact at both ends (2^.. = inf
+// gives 0, and 0 gives 1), between them off by at most 1.25 |g| 2^-24 (the rounded product and constant in the
+// exponent; only the side where the value is small has all of it) and 2^-21 (both approximations and the sum):
+// 2^-17 at g = -86.  What follows is rounded to bf16, half a step of which is 2^-8 of it.
 __device__ __forceinline__ float ex2_rcp(float t) {
   float e, s;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
@@ -432,8 +437,8 @@ __device__ __forceinline__ uint32_t swiglu_word(uint32_t wg, uint32_t wu) {
 
 // h = bf16(silu(g) * u) of the bf16 gate/up activations gu = [g | u], quantised like mx_quant_kernel;
 // h itself is not written.  All 16 pieces of a thread are in flight before the first is used, three CTAs per
-// SM: 8192 x 11008 97 us, 4.7 TB/s (127 us with addresses worked out per piece); bound by instruction issue
-// (22 per value) and the latency of a tile's loads.
+// SM: 8192 x 11008 97 us, 4.7 TB/s (127 us with addresses worked out per piece); 22 instructions per value, issue slots
+// 62% and the ALU pipe 49% busy: the latency of a tile's loads, and its phases one after another.
 __global__ void __launch_bounds__(THREADS, 3) mx_swiglu_quant_kernel(const __nv_bfloat16* gu, int64_t ld, int64_t F,
                                                                   int64_t tiles_c, Out o) {
   extern __shared__ __align__(16) uint8_t smem[];
