@@ -937,8 +937,10 @@ inline int fill(const char* name, const FfDistillRows* in, Args* a) {
   FF_REQUIRE(in->temperature > 0.f && in->temperature < 1e30f && in->alpha >= 0.f && in->alpha <= 1.f, FF_ERR_INVALID_ARG,
              "%s: temperature=%g (positive), alpha=%g (0 to 1)", name, in->temperature, in->alpha);
   if (in->rows > 0)
-    FF_REQUIRE(in->logits && in->ids && in->teacher_logits && aligned(in->logits, dtype_size(in->dtype)), FF_ERR_INVALID_ARG,
-               "%s: null or unaligned pointer", name);
+    FF_REQUIRE(in->logits && in->ids && in->teacher_logits && aligned(in->logits, dtype_size(in->dtype)) &&
+                   aligned(in->ids, in->ids_64 ? 8 : 4) && aligned(in->teacher_logits, dtype_size(in->teacher_dtype)) &&
+                   aligned(in->labels, in->labels_64 ? 8 : 4) && aligned(in->teacher_lse, 4),
+               FF_ERR_INVALID_ARG, "%s: null or unaligned pointer", name);
   *a = Args{};
   a->logits = in->logits;
   a->rows = in->rows;
@@ -981,7 +983,9 @@ extern "C" int ff_distill_loss(const FfDistillRows* in, int reduction, float* ro
     if (reduction != FF_REDUCE_NONE) FF_CUDA_TRY(cudaMemsetAsync(loss, 0, 4, st), "ff_distill_loss");
     return FF_OK;
   }
-  FF_REQUIRE(row_loss, FF_ERR_INVALID_ARG, "ff_distill_loss: null row_loss");
+  FF_REQUIRE(row_loss && ff::aligned(row_loss, 4) && ff::aligned(loss, 4) && ff::aligned(held, 4) && ff::aligned(counts, 4) &&
+                 ff::aligned(grad, ff::dtype_size(in->dtype)),
+             FF_ERR_INVALID_ARG, "ff_distill_loss: null row_loss or an unaligned output");
   if (reduction == FF_REDUCE_MEAN) {
     distill_count_kernel<<<COUNT_CTAS, 256, 0, st>>>(a, counts);
     rc = ff::check_launch("ff_distill_loss count");
@@ -1010,7 +1014,9 @@ extern "C" int ff_distill_grad(const FfDistillRows* in, int reduction, const flo
   FF_REQUIRE(ldg >= a.V && (reduction != FF_REDUCE_MEAN || counts) && !(held && reduction == FF_REDUCE_NONE),
              FF_ERR_INVALID_ARG, "ff_distill_grad: ldg=%lld, counts with the mean, held with a scalar", (long long)ldg);
   if (a.rows == 0) return FF_OK;
-  FF_REQUIRE(grad && upstream, FF_ERR_INVALID_ARG, "ff_distill_grad: null pointer");
+  FF_REQUIRE(grad && upstream && ff::aligned(grad, ff::dtype_size(in->dtype)) && ff::aligned(upstream, 4) && ff::aligned(held, 4) &&
+                 ff::aligned(counts, 4),
+             FF_ERR_INVALID_ARG, "ff_distill_grad: null or unaligned pointer");
   a.mean = reduction == FF_REDUCE_MEAN;
   a.counts = counts;
   a.grad = grad;

@@ -1016,6 +1016,13 @@ inline int check_operand(const char* name, const char* which, const Operand& o, 
   return FF_OK;
 }
 
+// outputs and bias in whole elements
+inline int check_out(const char* name, const void* D, int kind, const float* bias) {
+  FF_REQUIRE(aligned(D, kind == FF_OUT_F32 ? 4 : 2) && aligned(bias, 4), FF_ERR_INVALID_ARG,
+             "%s: an output or the bias is not aligned to its elements", name);
+  return FF_OK;
+}
+
 }  // namespace mxg
 }  // namespace ff
 
@@ -1032,7 +1039,7 @@ extern "C" int ff_mxfp4_gemm(const uint8_t* A, int64_t lda, const uint8_t* sA, c
              "ff_mxfp4_gemm: dimension too large (M=%lld N=%lld K=%lld)", (long long)M, (long long)N, (long long)K);
   const Operand a{A, lda, sA}, b{B, ldb, sB};
   int rc;
-  if ((rc = check_operand("ff_mxfp4_gemm", "A", a, K)) || (rc = check_operand("ff_mxfp4_gemm", "B", b, K))) return rc;
+  if ((rc = check_out("ff_mxfp4_gemm", D, out_kind, bias)) || (rc = check_operand("ff_mxfp4_gemm", "A", a, K)) || (rc = check_operand("ff_mxfp4_gemm", "B", b, K))) return rc;
   Epi ep{};
   ep.D = D;
   ep.ldd = ldd;
@@ -1107,7 +1114,7 @@ extern "C" int ff_mxfp4_linear(const void* x, int dtype, int64_t ldx, const uint
              (long long)ws_bytes);
   const Operand a = part_at(ws, M, K), b{W, ldw, sW};
   int rc;
-  if ((rc = check_operand("ff_mxfp4_linear", "W", b, K))) return rc;
+  if ((rc = check_out("ff_mxfp4_linear", D, out_kind, bias)) || (rc = check_operand("ff_mxfp4_linear", "W", b, K))) return rc;
   rc = ff_mxfp4_quant(x, dtype, M, K, ldx, const_cast<uint8_t*>(a.q), a.ld, const_cast<uint8_t*>(a.s), nullptr, 0, nullptr, nullptr,
                       nullptr, stream);
   if (rc) return rc;
@@ -1140,7 +1147,7 @@ extern "C" int ff_mxfp4_swiglu_mlp(const void* x, int dtype, int64_t ldx, const 
              "ff_mxfp4_swiglu_mlp: workspace of %lld bytes (16-byte aligned) needed, got %lld", (long long)need, (long long)ws_bytes);
   const Operand a = part_at(ws, M, K), h = part_at(ws + part_bytes(M, K), M, F), gu{GU, ldgu, sGU}, w{W, ldw, sW};
   int rc;
-  if ((rc = check_operand("ff_mxfp4_swiglu_mlp", "gate_up", gu, K)) || (rc = check_operand("ff_mxfp4_swiglu_mlp", "down", w, F)))
+  if ((rc = check_out("ff_mxfp4_swiglu_mlp", D, out_kind, nullptr)) || (rc = check_operand("ff_mxfp4_swiglu_mlp", "gate_up", gu, K)) || (rc = check_operand("ff_mxfp4_swiglu_mlp", "down", w, F)))
     return rc;
   rc = ff_mxfp4_quant(x, dtype, M, K, ldx, const_cast<uint8_t*>(a.q), a.ld, const_cast<uint8_t*>(a.s), nullptr, 0, nullptr, nullptr,
                       nullptr, stream);
@@ -1225,7 +1232,8 @@ extern "C" int ff_mxfp4_linear_train(const void* x, int x_dtype, int64_t ldx, co
   const char* name = "ff_mxfp4_linear_train";
   int rc;
   if ((rc = check_dims(name, M, N, K)) || (rc = check_ws(name, "tmp", tmp, tmp_bytes, part_bytes(M, K) + part_bytes(N, K))) ||
-      (rc = check_ws(name, "saved", saved, saved_bytes, (need_dw ? part_bytes(K, M) : 0) + (need_dx ? part_bytes(K, N) : 0))))
+      (rc = check_ws(name, "saved", saved, saved_bytes, (need_dw ? part_bytes(K, M) : 0) + (need_dx ? part_bytes(K, N) : 0))) ||
+      (rc = check_out(name, y, FF_OUT_BF16, bias)))
     return rc;
   FF_REQUIRE(y, FF_ERR_INVALID_ARG, "%s: null pointer", name);
   Arena t{tmp, tmp_bytes}, k{saved, saved_bytes};
@@ -1249,7 +1257,8 @@ extern "C" int ff_mxfp4_linear_bwd(const void* dy, int dtype, int64_t lddy, cons
   const int64_t sums = db ? (ff_mxfp4_colsum_ws_elems(M, N) * 4 + 15) / 16 * 16 : 0;
   if ((rc = check_dims(name, M, N, K)) ||
       (rc = check_ws(name, "saved", saved, saved_bytes, (saved_dw ? part_bytes(K, M) : 0) + (saved_dx ? part_bytes(K, N) : 0))) ||
-      (rc = check_ws(name, "tmp", tmp, tmp_bytes, (dx ? part_bytes(M, N) : 0) + (cols ? part_bytes(N, M) : 0) + sums)))
+      (rc = check_ws(name, "tmp", tmp, tmp_bytes, (dx ? part_bytes(M, N) : 0) + (cols ? part_bytes(N, M) : 0) + sums)) ||
+      (rc = check_out(name, dx, dx_kind, db)) || (rc = check_out(name, dw, dw_kind, nullptr)))
     return rc;
   FF_REQUIRE((!dx || (saved_dx && float_kind(dx_kind))) && (!dw || (saved_dw && float_kind(dw_kind))), FF_ERR_INVALID_ARG,
              "%s: a gradient whose operand was not saved, or a bad output kind", name);
@@ -1279,9 +1288,10 @@ extern "C" int ff_mxfp4_swiglu_train(const void* x, int x_dtype, int64_t ldx, co
       (rc = check_ws(name, "tmp", tmp, tmp_bytes, part_bytes(M, K) + part_bytes(2 * F, K) + part_bytes(M, F) + part_bytes(N, F))) ||
       (rc = check_ws(name, "saved", saved, saved_bytes,
                      (need_dgu ? part_bytes(K, M) : 0) + (need_dx ? part_bytes(K, 2 * F) : 0) + (need_dd ? part_bytes(F, M) : 0) +
-                         (back ? part_bytes(F, N) : 0))))
+                         (back ? part_bytes(F, N) : 0))) ||
+      (rc = check_out(name, y, FF_OUT_BF16, nullptr)))
     return rc;
-  FF_REQUIRE(y && gu, FF_ERR_INVALID_ARG, "%s: null pointer", name);
+  FF_REQUIRE(y && gu && ff::aligned(gu, 16), FF_ERR_INVALID_ARG, "%s: null pointer, or gu not 16-byte aligned", name);
   Arena t{tmp, tmp_bytes}, k{saved, saved_bytes};
   const Operand qx = t.take(M, K), qgu = t.take(2 * F, K), qh = t.take(M, F), qd = t.take(N, F);
   Operand xt{}, gut{}, ht{}, dt{};
@@ -1313,11 +1323,13 @@ extern "C" int ff_mxfp4_swiglu_bwd(const void* dy, int dtype, int64_t lddy, cons
                          (back ? part_bytes(F, N) : 0))) ||
       (rc = check_ws(name, "tmp", tmp, tmp_bytes,
                      (back ? part_bytes(M, N) : 0) + (need_dd ? part_bytes(N, M) : 0) + (need_dx ? part_bytes(M, 2 * F) : 0) +
-                         (need_dgu ? part_bytes(2 * F, M) : 0))))
+                         (need_dgu ? part_bytes(2 * F, M) : 0))) ||
+      (rc = check_out(name, dx, dx_kind, nullptr)) || (rc = check_out(name, dwgu, gu_kind, nullptr)) ||
+      (rc = check_out(name, dwd, d_kind, nullptr)))
     return rc;
   FF_REQUIRE((!need_dx || (dx && float_kind(dx_kind))) && (!need_dgu || (dwgu && float_kind(gu_kind))) &&
-                 (!need_dd || (dwd && float_kind(d_kind))) && (!back || (gu && dh)),
-             FF_ERR_INVALID_ARG, "%s: null pointer or bad output kind", name);
+                 (!need_dd || (dwd && float_kind(d_kind))) && (!back || (gu && dh && ff::aligned(gu, 16) && ff::aligned(dh, 16))),
+             FF_ERR_INVALID_ARG, "%s: null pointer, bad output kind, or gu or dh not 16-byte aligned", name);
   Arena k{mut(saved), saved_bytes}, t{tmp, tmp_bytes};
   Operand xt{}, gut{}, ht{}, dt{}, q{}, qt{}, p{}, pt{};
   if (need_dgu) xt = k.take(K, M);

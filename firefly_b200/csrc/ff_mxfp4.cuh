@@ -720,6 +720,8 @@ extern "C" int ff_mxfp4_quant(const void* x, int dtype, int64_t rows, int64_t co
   FF_REQUIRE(ldx >= cols, FF_ERR_INVALID_ARG, "ff_mxfp4_quant: ldx=%lld < cols=%lld", (long long)ldx, (long long)cols);
   FF_REQUIRE(!colsum || (q_cols_t && colsum_ws), FF_ERR_INVALID_ARG,
              "ff_mxfp4_quant: column sums come with the column codes and need a workspace");
+  FF_REQUIRE(ff::aligned(x, ff::dtype_size(dtype)) && ff::aligned(colsum, 4) && ff::aligned(colsum_ws, 4), FF_ERR_INVALID_ARG,
+             "ff_mxfp4_quant: x or the column sums are not aligned to their elements");
   cudaStream_t st = ff::as_stream(stream);
   if (rows == 0) {
     if (colsum) FF_CUDA_TRY(cudaMemsetAsync(colsum, 0, (size_t)cols * 4, st), "ff_mxfp4_quant");
@@ -793,7 +795,8 @@ extern "C" int ff_mxfp4_dequant(const uint8_t* q, int64_t ldq, const uint8_t* s,
   int rc = make_out("ff_mxfp4_dequant", rows, cols, const_cast<uint8_t*>(q), ldq, const_cast<uint8_t*>(s), nullptr, 0, nullptr, &o);
   if (rc) return rc;
   FF_REQUIRE(dtype >= FF_DTYPE_F32 && dtype <= FF_DTYPE_F16, FF_ERR_INVALID_ARG, "ff_mxfp4_dequant: bad dtype %d", dtype);
-  FF_REQUIRE(ldo >= cols, FF_ERR_INVALID_ARG, "ff_mxfp4_dequant: ldo=%lld < cols=%lld", (long long)ldo, (long long)cols);
+  FF_REQUIRE(ldo >= cols && ff::aligned(out, ff::dtype_size(dtype)), FF_ERR_INVALID_ARG,
+             "ff_mxfp4_dequant: ldo=%lld < cols=%lld, or an output that is not aligned to its elements", (long long)ldo, (long long)cols);
   if (rows == 0) return FF_OK;
   FF_REQUIRE(q && s && out, FF_ERR_INVALID_ARG, "ff_mxfp4_dequant: null pointer");
   const int64_t per_row = (cols + 7) / 8;

@@ -526,6 +526,7 @@ FF_API int ff_update_int8_weight(int8_t* w, const int32_t* dq, int64_t n, void* 
  * the nearest (ties to even) and saturated at 6; two codes to a byte, the earlier value in the low
  * nibble.  A block with an infinity or a NaN gets S = 255 (NaN) and codes 0.
  *
+ * Every pointer is aligned to its elements (others are refused), and further where it is said.
  * Codes: [rows, ld BYTES], ld a multiple of 16 and at least 16 * ceil(cols / 32), 16-byte aligned.
  * Scales: ff_mxfp4_scale_bytes(rows, cols) bytes, 16-byte aligned, in 512-byte chunks of 128 rows x
  * 4 blocks: the scale of (row, block) is byte (row % 32) * 16 + (row / 32 % 4) * 4 + block % 4 of
@@ -631,6 +632,7 @@ FF_API int ff_mxfp4_swiglu_bwd(const void* dy, int dtype, int64_t lddy, const vo
  * A row whose label is ignore_index (without labels: a row without entries) has loss and gradient 0 and
  * is not counted by the mean; the mean of no rows is 0.  A token id or label beyond the vocabulary
  * raises FF_DEVICE_BADARG and is treated as absent / ignored.  A token may occur in several entries.
+ * Every pointer is aligned to its elements (others are refused).
  */
 #define FF_REDUCE_NONE 0
 #define FF_REDUCE_MEAN 1

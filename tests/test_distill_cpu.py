@@ -82,3 +82,21 @@ def test_a_vocabulary_that_does_not_fit_is_refused():
     lib, p, n = _capi.lib(), ctypes.c_void_p(4096), None
     assert lib.ff_distill_loss(_rows(vocab=1000000, ld_logits=1000000), 0, p, n, n, 0, n, n, n) == _capi.FF_ERR_UNSUPPORTED
     assert b"does not fit" in lib.ff_last_error()
+
+
+def test_pointers_that_are_not_aligned_to_their_elements_are_refused():
+    lib, bad = _capi.lib(), _capi.FF_ERR_INVALID_ARG
+    p, n, odd = ctypes.c_void_p(4096), None, ctypes.c_void_p(4097)
+    for kw in (dict(logits=4098, dtype=0), dict(ids=4100), dict(ids=4098, ids_64=0), dict(teacher_logits=4098),
+               dict(teacher_logits=4097, teacher_dtype=1), dict(labels=4098), dict(labels=4100, labels_64=1), dict(teacher_lse=4098)):
+        assert lib.ff_distill_loss(_rows(**kw), 0, p, n, n, 0, n, n, n) == bad, kw
+        assert lib.ff_distill_grad(_rows(**kw), 0, p, n, 0, n, p, 100, n) == bad, kw
+    assert lib.ff_distill_loss(_rows(), 0, odd, n, n, 0, n, n, n) == bad
+    assert lib.ff_distill_loss(_rows(), 1, p, odd, n, 0, n, p, n) == bad
+    assert lib.ff_distill_loss(_rows(), 1, p, p, odd, 100, p, p, n) == bad
+    assert lib.ff_distill_loss(_rows(), 1, p, p, p, 100, odd, p, n) == bad
+    assert lib.ff_distill_loss(_rows(), 1, p, p, n, 0, n, odd, n) == bad
+    assert lib.ff_distill_grad(_rows(), 1, odd, n, 0, p, p, 100, n) == bad
+    assert lib.ff_distill_grad(_rows(), 1, p, odd, 0, p, p, 100, n) == bad
+    assert lib.ff_distill_grad(_rows(), 1, p, n, 0, odd, p, 100, n) == bad
+    assert lib.ff_distill_grad(_rows(), 1, p, n, 0, p, odd, 100, n) == bad

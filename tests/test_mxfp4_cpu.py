@@ -146,3 +146,33 @@ def test_serving_entries_refuse_before_any_launch():
     assert g(p, 1, 64, p, 16, p, p, 64, p, p, 8, 2, 3, 64, 128, 8, p, need, n) == bad
     assert g(p, 1, 64, p, 32, p, p, 48, p, p, 8, 2, 3, 64, 128, 8, p, need, n) == bad
     assert g(p, 1, 64, p, 32, p, p, 64, p, p, 7, 2, 3, 64, 128, 8, p, need, n) == bad
+
+
+def test_pointers_that_are_not_aligned_to_their_elements_are_refused():
+    lib, bad = _capi.lib(), _capi.FF_ERR_INVALID_ARG
+    p, n, odd, two = ctypes.c_void_p(4096), None, ctypes.c_void_p(4097), ctypes.c_void_p(4098)
+    q = lib.ff_mxfp4_quant
+    assert q(odd, 1, 4, 64, 64, p, 32, p, n, 0, n, n, n, n) == bad
+    assert q(two, 0, 4, 64, 64, p, 32, p, n, 0, n, n, n, n) == bad
+    assert q(p, 1, 4, 64, 64, p, 32, p, p, 16, p, two, p, n) == bad          # sums
+    assert q(p, 1, 4, 64, 64, p, 32, p, p, 16, p, p, two, n) == bad
+    assert lib.ff_mxfp4_dequant(p, 32, p, 4, 64, odd, 1, 64, n) == bad
+    assert lib.ff_mxfp4_dequant(p, 32, p, 4, 64, two, 0, 64, n) == bad
+    for d, kind, bias in ((odd, 2, n), (two, 1, n), (p, 2, two)):
+        assert lib.ff_mxfp4_gemm(p, 32, p, p, 32, p, bias, d, 8, kind, 4, 8, 64, n) == bad
+        assert lib.ff_mxfp4_linear(p, 1, 64, p, 32, p, bias, d, 8, kind, 3, 8, 64, p, 1 << 20, n) == bad
+    assert lib.ff_mxfp4_swiglu_mlp(p, 1, 64, p, 32, p, p, 64, p, odd, 8, 2, 3, 64, 128, 8, p, 1 << 20, n) == bad
+    big = 1 << 24
+    f = lib.ff_mxfp4_linear_train
+    assert f(p, 1, 64, p, 1, 64, n, odd, 3, 8, 64, 1, 1, p, big, p, big, n) == bad
+    assert f(p, 1, 64, p, 1, 64, two, p, 3, 8, 64, 1, 1, p, big, p, big, n) == bad
+    b = lib.ff_mxfp4_linear_bwd
+    for dx, dw, db in ((odd, p, p), (p, odd, p), (p, p, two)):
+        assert b(p, 1, 8, p, big, 1, 1, dx, 2, dw, 2, db, 3, 8, 64, p, big, n) == bad
+    assert lib.ff_mxfp4_swiglu_train(p, 1, 64, p, 1, 64, p, 1, 128, p, odd, 3, 64, 128, 8, 1, 1, 1, p, big, p, big, n) == bad
+    assert lib.ff_mxfp4_swiglu_train(p, 1, 64, p, 1, 64, p, 1, 128, two, p, 3, 64, 128, 8, 1, 1, 1, p, big, p, big, n) == bad
+    g = lib.ff_mxfp4_swiglu_bwd
+    for gu, dh in ((two, p), (p, two)):
+        assert g(p, 1, 8, gu, dh, p, big, 1, 1, 1, p, 2, p, 2, p, 2, 3, 64, 128, 8, p, big, n) == bad
+    for dx, dgu, dd in ((odd, p, p), (p, odd, p), (p, p, odd)):
+        assert g(p, 1, 8, p, p, p, big, 1, 1, 1, dx, 2, dgu, 2, dd, 2, 3, 64, 128, 8, p, big, n) == bad
