@@ -183,8 +183,8 @@ class MXFP4LinearFn(torch.autograd.Function):
         xd, wd, bd = ctx.dtypes
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
         dev = dy.device
-        if T == 0:
-            return (torch.zeros((0, K), dtype=xd, device=dev) if need_dx else None,
+        if T == 0 or O == 0:
+            return (torch.zeros((T, K), dtype=xd, device=dev) if need_dx else None,
                     torch.zeros((O, K), dtype=wd, device=dev) if need_dw else None,
                     torch.zeros((O,), dtype=bd, device=dev) if need_db else None, None, None)
         if ctx.whole:
@@ -241,8 +241,8 @@ class MXFP4SwiGLUFn(torch.autograd.Function):
         xd, gud, dd = ctx.dtypes
         need_dx, need_gu, need_d = ctx.needs_input_grad[:3]
         dev = dy.device
-        if T == 0:
-            return (torch.zeros((0, K), dtype=xd, device=dev) if need_dx else None,
+        if T == 0 or O == 0:
+            return (torch.zeros((T, K), dtype=xd, device=dev) if need_dx else None,
                     torch.zeros((2 * F, K), dtype=gud, device=dev) if need_gu else None,
                     torch.zeros((O, F), dtype=dd, device=dev) if need_d else None, None, None)
         if ctx.whole:

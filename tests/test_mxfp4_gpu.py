@@ -729,3 +729,18 @@ def test_a_trained_decoder_runs_in_four_bits():
         with torch.no_grad():
             g, u = mlp.gate_up(x).chunk(2, dim=-1)
             assert torch.equal(mlp(x), mlp.down(F.silu(g) * u))
+
+
+def test_no_outputs():
+    """Weights without rows: empty results, gradients of zeros."""
+    x = _randn(7, 64, 1).requires_grad_(True)
+    w, b = _randn(5, 64, 2)[:0].requires_grad_(True), torch.zeros(0, device=DEV, requires_grad=True)
+    y = mxfp4_linear(x, w, b)
+    assert y.shape == (7, 0)
+    dx, dw, db = torch.autograd.grad(y.sum(), [x, w, b])
+    assert dx.shape == (7, 64) and not dx.any() and dw.shape == (0, 64) and db.shape == (0,)
+    wgu, wd = _randn(64, 64, 3).requires_grad_(True), _randn(5, 32, 4)[:0].requires_grad_(True)
+    y = mxfp4_swiglu(x, wgu, wd)
+    assert y.shape == (7, 0)
+    dx, dgu, dd = torch.autograd.grad(y.sum(), [x, wgu, wd])
+    assert dx.shape == (7, 64) and not dx.any() and dgu.shape == (64, 64) and not dgu.any() and dd.shape == (0, 32)
