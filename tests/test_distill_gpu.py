@@ -771,3 +771,41 @@ def test_forward_mode_is_refused_as_by_the_other_layers():
             with pytest.raises(RuntimeError, match="forward"):
                 distillation_loss(forward_ad.make_dual(x, torch.ones_like(x)), ids, t)
             assert torch.equal(distillation_loss(s, ids, t), distillation_loss(s.clone(), ids, t))  # no tangent: as ever
+
+
+@pytest.mark.parametrize("V,n", [(700, 3000), (9000, 2000), (40000, 900)])
+@pytest.mark.parametrize("labels", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_every_kind_one_after_another(V, n, labels, dtype):
+    """Ordinary rows, rows whose rest is far below, masked slices, nothing but a mask, no rest, repeated tokens and ignored rows in
+    turn on the same CTAs: each as by itself, and the same wherever it stands."""
+    T = 2.0
+    s, ids, t, lab, _ = _case(8, V, 9, 45, labels=True, pad=False, dtype=torch.float32)
+    lse = torch.logsumexp(t.double() / T, 1).float() + 0.1
+    s[1].scatter_(0, ids[1], s[1, ids[1]] + 500)  # far rest
+    s[2, V // 2:] = -1e10
+    s[3] = -1e10
+    ids[4, 3:6] = ids[4, 0]
+    lab = lab.clamp(min=0)
+    lab[5] = -100
+    ids[6] = -1
+    s[7].scatter_(0, ids[7], s[7, ids[7]] - 500)  # next to nothing on the entries
+    s, lab = s.to(dtype), lab if labels else None
+    _check_each(s, ids, t, lab, lse, T, 0.5 if labels else 1.0)
+    kind = torch.randint(0, 8, (n,), device=DEV, generator=torch.Generator(device=DEV).manual_seed(46))
+    kind[:8] = torch.arange(8, device=DEV)
+    first = torch.stack([torch.nonzero(kind == k)[0, 0] for k in range(8)])
+    lab_n = None if lab is None else lab[kind]
+    x = s[kind].requires_grad_(True)
+    kw = dict(teacher_lse=lse[kind], temperature=T, alpha=0.5 if labels else 1.0)
+    rows = distillation_loss(x, ids[kind], t[kind], lab_n, reduction="none", **kw)
+    loss = distillation_loss(x, ids[kind], t[kind], lab_n, reduction="sum", **kw)
+    loss.backward()
+    assert torch.equal(rows, rows[first][kind]) and torch.equal(x.grad, x.grad[first][kind])
+    # each row as in the batch of eight, whose rows may be cut into other slices
+    want, grad, ok, d_row, tol, _ = _bounds(s, ids, t, lab, lse, T, 0.5 if labels else 1.0)
+    assert bool(((rows[first].double() - want).abs() <= d_row).all())
+    info = torch.finfo(dtype)
+    tol = tol * (1 + info.eps) + info.eps / 2 * grad.abs() + info.smallest_normal * info.eps
+    assert bool(((x.grad[first].double() - grad).abs() <= tol).all())
+    assert _capi.device_status() == 0
