@@ -12,7 +12,8 @@
 //             + (1 - alpha) (softmax(s)_v - [v = y]).
 // log q_rest and q_v / q_rest have the rest's own maximum as their reference where q_rest is below 2^-60 of the row.  Where
 // the entries cover the vocabulary there is no rest term; where the student has all other tokens at -inf it is infinite,
-// unless p_rest is below 1e-5, the rounding of 1 - sum p.  p_rest is not negative: w is 1, or sum p where a rounded lse or a token given twice make that more than 1.
+// unless p_rest is below 1e-5, the rounding of 1 - sum p.  p_rest is not negative, so w is 1, or sum p where a rounded
+// lse or a token given twice make that more than 1 or there is no rest term.
 // A row whose label is ignore_index, or without labels a row without entries, counts nothing.
 //
 // One cluster of 1 to 8 CTAs per row, each holding its slice of the row in shared memory (bulk
@@ -46,7 +47,7 @@ constexpr int MAX_TOP = 4096;
 constexpr int MAX_SMEM = 227 * 1024;
 constexpr int COUNT_CTAS = FF_DISTILL_WS_ELEMS;
 // a share below which the rest is summed relative to its own maximum: exponentials end at 2^-126, so a sum above this is
-// complete to 2^-60 of itself per token
+// complete to 2^-66 of itself per token
 constexpr float kLittle = 8.673617379884035e-19f;  // 2^-60
 
 struct Args {
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__(THREADS + 32, 3) distill_kernel(Args a) {
         if (grow && live) {
           const float up = a.upstream ? __ldg(a.upstream + r * a.up_stride) * inv_count : inv_count;
           const float fk = has ? up * a.alpha * a.T : 0.f, f1 = label >= 0 ? up * (1.f - a.alpha) : 0.f;
-          // log sum exp(s/T) stands in the loss with the weight sum p + p_rest: 1 unless the teacher's log-sum-exp is off
+          // log sum exp(s/T) stands in the loss with the weight sum p + p_rest (1 with a rest term)
           const float mass = a.lse && p_rest == 0.f ? c.t_sum[buf] : 1.f;
           const float gq = mass * fk / all.sum, g1 = f1 / sum1_all;  // factors of exp(..) for q and the softmax at 1
           // Outside the entries: q (1 - p_rest / q_rest).  With next to no q there, q itself is nothing beside
